@@ -4,6 +4,7 @@ The library is loaded on first use. A missing library is an error, never a
 silent fallback: build it with ``python -m analysis_spec_b200.build``.
 """
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -15,13 +16,16 @@ F32, BF16, F16 = 0, 1, 2
 
 DEVICE_ERROR_KINDS = {1: 'remap index', 2: 'compact index', 3: 'move index', 4: 'tree parent index',
                       5: 'padding owner index', 6: 'wait timeout', 7: 'scheduling packet',
-                      8: 'seen index', 9: 'history index', 10: 'row table'}
+                      8: 'seen index', 9: 'history index', 10: 'row table', 11: 'page table',
+                      12: 'rotation index', 13: 'token index'}
 
 _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int32
 _pi64 = ctypes.POINTER(ctypes.c_int64)
 _pp = ctypes.POINTER(ctypes.c_void_p)
+_f32 = ctypes.c_float
+_b = ctypes.c_char_p  # packed int64 arrays (pack_i64): cheaper to build than a ctypes array
 
 # name -> argtypes (every function returns int status)
 SIGNATURES = {
@@ -65,6 +69,14 @@ SIGNATURES = {
     'speckv_acceptance_counts': [_p, _i64, _i64, _i64, _p, _p],
     'speckv_attention_set_ctas': [_i32],
     'speckv_attention_set_chunks': [_i32],
+    'speckv_paged_append': [_p, _p, _p, _p, _p, _p, _b, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _i64, _p, _p,
+                            _i64, _i64, _i32, _i64, _i64, _i64, _i64, _i64, _i32, _p],
+    'speckv_paged_attention': [_p, _p, _p, _b, _p, _i64, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _i64, _f32,
+                               _i32, _p],
+    'speckv_token_logprobs': [_p, _i32, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _f32,
+                              _i32, _p, _p, _p, _p, _p, _p],
+    'speckv_token_logprobs_backward': [_p, _i32, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _f32, _i32, _p, _p,
+                                       _p, _p, _p, _p, _p, _p],
 }
 
 # entries with a prepare / launch split (speckv_<name>_prepare + speckv_plan_launch)
@@ -195,6 +207,11 @@ def prepare(name, *args):
 
 def ptr_array(values):
     return (ctypes.c_void_p * len(values))(*values)
+
+
+def pack_i64(*values):
+    """An int64 array argument as bytes."""
+    return struct.pack(f'{len(values)}q', *values)
 
 
 def i64_array(values):

@@ -51,6 +51,18 @@ def dense_mask_visibility(attention_mask, mask, batch, rows, kv_len):
     return vis
 
 
+def prompt_mask(prompt, query):
+    """Causal additive mask (batch, 1, rows, rows) of `query`'s rows over themselves, kept in the
+    dict `prompt` (one per forward), so that its visibility bits are built once for all layers."""
+    batch, rows = query.shape[0], query.shape[2]
+    if prompt.get('shape') != (batch, rows, query.dtype):
+        hidden = torch.ones((rows, rows), dtype=torch.bool, device=query.device).triu(1)
+        mask = torch.zeros((rows, rows), dtype=query.dtype, device=query.device)
+        mask.masked_fill_(hidden, torch.finfo(query.dtype).min)
+        prompt.update(shape=(batch, rows, query.dtype), mask=mask.expand(batch, 1, rows, rows))
+    return prompt['mask']
+
+
 def _pending_rows(key):
     """(layer, (key_states, value_states, position)) when `key` is a view of an
     OPDStaticCache(fuse_append=True) layer whose latest rows are not stored yet, else None."""
@@ -82,10 +94,14 @@ def tree_verify_attention(module, query, key, value, attention_mask, dropout=0.0
 
     K/V views of an ``OPDStaticCache(fuse_append=True)`` whose latest rows are still pending
     take the fused append + attention kernel on the visibility-bits path; any other path
-    stores the rows first."""
+    stores the rows first. K/V of a ``PagedKVCache`` take the one-token paged attention, which
+    sees each sequence's own positions and reads no mask."""
     if dropout:
         raise ValueError('tree_verify_attention is an inference kernel (dropout must be 0)')
     scale = scaling if scaling is not None else query.shape[-1] ** -0.5
+    pages = getattr(key, '_speckv_pages', None)  # K/V pools of a PagedKVCache: (page table, lengths)
+    if pages is not None:
+        return _ops.paged_attention(query, key, value, *pages, scale), None
     rows_table = getattr(key, '_speckv_rows', None)  # K/V of a row-table cache: every pool row
     pending = _pending_rows(key)
     vis = attention_mask if hasattr(attention_mask, 'first_col') else getattr(attention_mask, '_speckv_visibility',
@@ -96,6 +112,10 @@ def tree_verify_attention(module, query, key, value, attention_mask, dropout=0.0
     if mask is not None and mask.shape[-1] > key.shape[-2]:
         mask = mask[:, :, :, :key.shape[-2]]
     causal = is_causal if is_causal is not None else getattr(module, 'is_causal', True)
+    if mask is None and causal and query.shape[2] > 1:
+        prompt = getattr(key, '_speckv_prompt', None)  # the prompts of a PagedKVCache: one mask for every layer
+        if prompt is not None and key.shape[-2] == query.shape[2]:
+            mask = attention_mask = prompt_mask(prompt, query)
     if mask is None and causal and query.shape[2] > 1:
         raise ValueError('tree_verify_attention needs an explicit mask for multi-query causal attention')
     if (mask is not None and mask.dim() == 4 and mask.dtype != torch.bool and query.shape[-1] == 128 and

@@ -12,6 +12,7 @@ import torch
 
 from . import _ops
 from . import tree_kernels as _default_kernels
+from .token_logprobs import token_logprobs
 
 
 @dataclass
@@ -110,6 +111,13 @@ class VerifiedPath:
             raise ValueError("invalid committed path width")
         plugin = kernels if kernels is not None else _default_kernels
         return plugin.pad_verified_path(self, past_length, width, eos_token_id, workspace)
+
+    def log_probs(self, logits, *, top=0, temperature=1.0):
+        """Log-probabilities of the emitted tokens under the verify forward's logits (batch,
+        packed rows, vocabulary), with entropy and top alternatives: one launch that reads the
+        accepted rows only (no reference counterpart on this path: a GRPO trainer recomputes
+        them with a further forward). Padding columns give 0 / -1."""
+        return token_logprobs(logits, self.tokens, rows=self.packed_indices, top=top, temperature=temperature)
 
     def host_bookkeeping(self, past_length):
         """One small D2H packet: per-sequence lengths, absolute KV indices and tokens."""

@@ -52,6 +52,9 @@ extern "C" {
 #define SPECKV_DERR_SEEN_INDEX 8 /* draft expansion: seen position outside [0, columns) */
 #define SPECKV_DERR_HISTORY_INDEX 9 /* history append: owner row or source position out of range */
 #define SPECKV_DERR_ROW_TABLE 10    /* row table entry outside the pools' rows; value = the entry */
+#define SPECKV_DERR_PAGE_TABLE 11   /* page outside the pools, or a position the page table cannot name */
+#define SPECKV_DERR_ROTATION_INDEX 12 /* rotation position outside the cos / sin tables */
+#define SPECKV_DERR_TOKEN_INDEX 13  /* token outside the vocabulary, or source row outside the logits */
 
 #define SPECKV_HISTORY_MAX_FIELDS 4
 
@@ -535,6 +538,91 @@ int speckv_attention_set_chunks(int32_t on);
  * timeout path without a GPU fault; keep both 0 otherwise. No reference
  * counterpart (the reference's kernels have no bounded waits). */
 int speckv_attention_test_hooks(int64_t wait_limit_ns, int32_t withhold_q_arrival);
+
+/* ---- Paged KV cache ------------------------------------------------------
+ * One K and one V pool of pages per layer, (num_pages, kv_heads, page_size, dim) with any
+ * (page, head, position) element strides and unit stride on dim. page_table[b][i] (int64,
+ * device, table_stride entries between sequences) is the pool page that holds positions
+ * [i * page_size, (i + 1) * page_size) of sequence b, i < table_pages; entries past a
+ * sequence's length are not read. Sequences hold their own positions from 0 on: no shared
+ * length and no padding. An entry outside [0, num_pages), or a position past table_pages *
+ * page_size, sets device error SPECKV_DERR_PAGE_TABLE; those rows are neither stored nor
+ * attended. The reference has no such cache: its sequences share one physical length
+ * (helper/opd_static_cache.py:17-174). */
+
+/* Stores K / V rows of new tokens, with the rotary position rotation applied to K on the way
+ * and, with query non-NULL, to the queries in the same launch:
+ *   slot = starts[b] + t                        for t < counts[b] (rows when counts is NULL)
+ *   key_pages[page][h][slot % page_size][:]   = rotate(key[b][h][t][:], position)
+ *   value_pages[page][h][slot % page_size][:] = value[b][h][t][:]
+ *   query_out[b][h][t][:]                     = rotate(query[b][h][t][:], position)
+ * position = positions[b][t] (element strides positions_stride_b / _t), or the slot when
+ * positions is NULL (tree rows sit at a slot other than their position). rotate turns the pairs
+ * (j, j + rotation_dim / 2), or (2j, 2j + 1) with interleaved = 1, j < rotation_dim / 2:
+ *   x' = x cos - y sin,  y' = y cos + x sin
+ * by row `position` of cos / sin, contiguous (rotation_positions, rotation_dim / 2) fp32 tables;
+ * cos = sin = NULL stores without a rotation. Dims past rotation_dim are copied. Rows t >=
+ * counts[b] are padding: nothing is read or stored for them and their query_out rows are zeros;
+ * so are those of tokens refused with SPECKV_DERR_PAGE_TABLE or (position outside the tables)
+ * SPECKV_DERR_ROTATION_INDEX. Two live tokens must not name one slot, and query_out must not
+ * overlap key / value / query.
+ * strides: 18 element strides, (b, h, t) of key, value, query and query_out, then (page, head,
+ * position) of key_pages and value_pages. Replaces, for a paged cache, apply_rotary_pos_emb
+ * followed by Cache.update (transformers models/qwen2/modeling_qwen2.py:215-225). */
+int speckv_paged_append(const void* key, const void* value, const void* query, void* query_out, void* key_pages,
+                        void* value_pages, const int64_t* strides, const int64_t* page_table, int64_t table_stride,
+                        int64_t table_pages, int64_t num_pages, int64_t page_size, const int64_t* starts,
+                        const int64_t* counts, const int64_t* positions, int64_t positions_stride_b,
+                        int64_t positions_stride_t, const float* cos, const float* sin, int64_t rotation_positions,
+                        int64_t rotation_dim, int32_t interleaved, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                        int64_t rows, int64_t dim, int32_t dtype, void* stream);
+
+/* Attention of one new token per sequence over a paged cache:
+ *   out[b][0][hq][:] = softmax_c(q[b][hq] . k_c * scale) v_c,   c < lengths[b]
+ * with KV head hq / (q_heads / kv_heads). lengths is a device array of batch int64; a sequence of
+ * length 0 (or less) gives zeros. out is contiguous (batch, 1, q_heads, dim). strides: 8 element
+ * strides, (b, h) of query and (page, head, position) of key_pages and value_pages. Head dims to
+ * 256. */
+int speckv_paged_attention(const void* query, const void* key_pages, const void* value_pages, const int64_t* strides,
+                           const int64_t* page_table, int64_t table_stride, int64_t table_pages, int64_t num_pages,
+                           int64_t page_size, const int64_t* lengths, void* out, int64_t batch, int64_t q_heads,
+                           int64_t kv_heads, int64_t dim, float scale, int32_t dtype, void* stream);
+
+/* ---- Log-probabilities of tokens ------------------------------------------ */
+
+#define SPECKV_MAX_TOP 32
+
+/* For output row (b, r), b < batch, r < per_batch, with x = logits[b][rows ? rows[b][r] : r][:]
+ * (vocab entries at unit stride) and z = x * inv_temperature:
+ *   lse = log sum_i exp(z_i),  logprobs = z[tokens[b][r]] - lse,  entropy = lse - sum_i p_i z_i
+ *   top_ids[k] = the `top` largest x, equal ones by the lower index (-0 equals 0, NaN below every
+ *   number),  top_logprobs[k] = z[top_ids[k]] - lse
+ * Outputs are contiguous over (b, r); logprobs is NULL exactly when tokens is. A row whose token or
+ * source row is negative is skipped: it is not read, its outputs are 0 and its ids -1; so is one
+ * whose token is >= vocab or whose source row is >= source_rows, which also sets device error
+ * SPECKV_DERR_TOKEN_INDEX. A row of -inf alone: logprobs and top_logprobs -inf, entropy 0. A row
+ * with a NaN or +inf: NaN. lse is kept for the gradient. Without rows, source_rows == per_batch.
+ * The numbers that the reference's sampler and GRPO loss take from the logits with log_softmax,
+ * gather, argmax and topk (helper/opd_sampling.py:162-170, helper/fastgrpo_training.py). */
+int speckv_token_logprobs(const void* logits, int32_t dtype, int64_t stride_b, int64_t stride_r,
+                          const int64_t* tokens, int64_t tokens_stride_b, int64_t tokens_stride_r,
+                          const int64_t* rows, int64_t rows_stride_b, int64_t rows_stride_r, int64_t batch,
+                          int64_t per_batch, int64_t source_rows, int64_t vocab, float inv_temperature, int32_t top,
+                          float* logprobs, float* entropy, float* lse, float* top_logprobs, int64_t* top_ids,
+                          void* stream);
+
+/* Gradient of speckv_token_logprobs (without rows) with respect to the logits, from the
+ * gradients of logprobs, entropy and top_logprobs (contiguous fp32, each may be NULL):
+ *   grad[b][r][i] = inv_temperature * (g_lp (d(i, token) - p_i) - g_H p_i (log p_i + entropy)
+ *                                      + sum_k g_top[k] (d(i, top_ids[k]) - p_i))
+ * grad_logits is contiguous (batch, per_batch, vocab) in the logits' dtype; skipped rows and rows
+ * of -inf alone get zeros. entropy, lse and top_ids are the forward's. */
+int speckv_token_logprobs_backward(const void* logits, int32_t dtype, int64_t stride_b, int64_t stride_r,
+                                   const int64_t* tokens, int64_t tokens_stride_b, int64_t tokens_stride_r,
+                                   int64_t batch, int64_t per_batch, int64_t vocab, float inv_temperature,
+                                   int32_t top, const float* entropy, const float* lse, const int64_t* top_ids,
+                                   const float* grad_logprobs, const float* grad_entropy,
+                                   const float* grad_top_logprobs, void* grad_logits, void* stream);
 
 #ifdef __cplusplus
 }

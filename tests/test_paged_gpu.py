@@ -1,0 +1,523 @@
+"""Append into a paged cache (rotation on the way) and the one-token attention over it, against
+plain implementations in 64 bits.
+
+Tolerances (u = eps / 2 of the dtype, the worst case of one rounding; the kernels work in fp32):
+* a rotated element x c - y s: two products and a difference, 3 roundings of at most
+  2^-24 (|x| + |y|), then one rounding to the dtype: u |ref| + 2^-22 (|x| + |y|), plus half the
+  smallest fp16 step, 2^-25.
+* the attention: a score sums D products in fp32, off by at most D 2^-23 sum |q k| scale =: ds
+  (2^-23: matrix instructions may round their sums toward zero), so a weight exp(s - max) is off
+  by at most 2 ds + 2^-20 of itself, is held in two 16-bit parts (2^-16), and n of them are added
+  (n 2^-24). Normalised weights sum to 1, so the output is off by at most
+  2 (2 ds + 2^-20 + 2^-16 + n 2^-24) max |v|, then u |ref| for the rounding.
+"""
+import math
+
+import pytest
+import torch
+
+from analysis_spec_b200 import _ops
+from analysis_spec_b200.paged_cache import PagedKVCache, paged_append, paged_attention, rotation_tables
+from analysis_spec_b200.token_logprobs import token_logprobs
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def gen(seed):
+    return torch.Generator(device='cuda').manual_seed(seed)
+
+
+def randn(*shape, dtype, g):
+    return torch.randn(*shape, device='cuda', generator=g).to(dtype)
+
+
+def pools(pages, hkv, page, dim, dtype, g, fill=math.nan):
+    return (torch.full((pages, hkv, page, dim), fill, device='cuda', dtype=dtype),
+            torch.full((pages, hkv, page, dim), fill, device='cuda', dtype=dtype))
+
+
+def turned(x, cos, sin, interleaved):
+    """x (..., dim) float64, cos / sin (..., rot / 2); returns (rotated, |x| + |y| of each element)."""
+    half = cos.shape[-1]
+    i = torch.arange(half, device=x.device)
+    a, b = (2 * i, 2 * i + 1) if interleaved else (i, i + half)
+    out, size = x.clone(), x.abs()
+    out[..., a] = x[..., a] * cos - x[..., b] * sin
+    out[..., b] = x[..., b] * cos + x[..., a] * sin
+    size[..., a] = size[..., b] = x[..., a].abs() + x[..., b].abs()
+    return out, size
+
+
+def check_rounded(got, ref, size, dtype):
+    u = torch.finfo(dtype).eps / 2
+    tol = u * ref.abs() + 2.0 ** -22 * size + (2.0 ** -25 if dtype == torch.float16 else 0)
+    bad = ((got.double() - ref).abs() > tol)
+    assert not bad.any(), (bad.sum().item(), (got.double() - ref).abs().max().item())
+
+
+# ---- append ------------------------------------------------------------------------------------
+
+def run_append(batch, rows, hq, hkv, dim, rot, page, past, dtype, interleaved, ragged, placed, query=True, seed=0):
+    g = gen(seed)
+    per = -(-(past + rows) // page)
+    total = batch * per + 2
+    kp, vp = pools(total, hkv, page, dim, dtype, g)
+    table = torch.randperm(total, device='cuda', generator=g)[:batch * per].view(batch, per).contiguous()
+    # one fused projection output, sliced and viewed by head: strided, not dense
+    fused = randn(batch, rows, (hq + 2 * hkv) * dim, dtype=dtype, g=g)
+    q, k, v = (x.unflatten(-1, (-1, dim)).transpose(1, 2) for x in fused.split((hq * dim, hkv * dim, hkv * dim), -1))
+    starts = torch.randint(0, past + 1, (batch,), device='cuda', generator=g)
+    counts = torch.randint(0, rows + 1, (batch,), device='cuda', generator=g) if ragged else None
+    positions = torch.randint(0, 50, (batch, rows), device='cuda', generator=g) if placed else None
+    tables = rotation_tables(max(past + rows, 50), rot, theta=5000.0) if rot else None
+    out = paged_append(k, v, kp, vp, table, starts, counts=counts, query=q if query else None, rotation=tables,
+                       positions=positions, interleaved=interleaved)
+    assert _ops.device_error() is None
+    want_k, want_v = (torch.full(kp.shape, math.nan, device='cuda', dtype=torch.float64) for _ in range(2))
+    size_k = torch.zeros_like(want_k)
+    for b in range(batch):
+        n = rows if counts is None else int(counts[b])
+        slot = int(starts[b]) + torch.arange(n, device='cuda')
+        where = slot if positions is None else positions[b, :n]
+        kk, qq = k[b, :, :n].double(), q[b, :, :n].double()
+        ks, qs = kk.abs(), qq.abs()
+        if rot:
+            c, s = tables[0][where].double(), tables[1][where].double()
+            (kk, ks), (qq, qs) = turned(kk, c, s, interleaved), turned(qq, c, s, interleaved)
+        at = table[b][slot // page]
+        want_k[at, :, slot % page] = kk.transpose(0, 1)
+        size_k[at, :, slot % page] = ks.transpose(0, 1)
+        want_v[at, :, slot % page] = v[b, :, :n].double().transpose(0, 1)
+        if query:
+            check_rounded(out[b, :, :n], qq, qs, dtype)
+            assert not out[b, :, n:].any()  # padding rows: zeros
+    assert torch.equal(vp.double().nan_to_num(9e9), want_v.nan_to_num(9e9))  # copied; nothing else touched
+    assert torch.equal(kp.isnan(), want_k.isnan())
+    check_rounded(kp.double().nan_to_num(0.0), want_k.nan_to_num(0.0), size_k, dtype)
+    if not query:
+        assert out is None
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('batch,rows,hq,hkv,dim,rot,page,past', [
+    (1, 1, 16, 2, 128, 128, 16, 0), (8, 1, 28, 4, 128, 128, 64, 700), (3, 61, 16, 2, 128, 128, 16, 100),
+    (2, 37, 8, 8, 64, 32, 32, 5), (2, 5, 6, 3, 256, 256, 128, 300), (4, 7, 12, 1, 128, 64, 16, 40),
+    (3, 4, 6, 2, 40, 20, 3, 11), (2, 9, 3, 1, 24, 14, 1, 6), (5, 1, 4, 4, 80, 80, 24, 60), (1, 300, 40, 8, 96, 96, 7, 9)])
+def test_append_and_rotation(batch, rows, hq, hkv, dim, rot, page, past, dtype):
+    run_append(batch, rows, hq, hkv, dim, rot, page, past, dtype, interleaved=False, ragged=rows > 1, placed=False)
+    run_append(batch, rows, hq, hkv, dim, rot, page, past, dtype, interleaved=True, ragged=rows > 1, placed=True, seed=1)
+
+
+def test_append_without_rotation_or_query():
+    run_append(3, 20, 4, 2, 128, 0, 16, 30, torch.bfloat16, False, True, False, query=False)
+    run_append(3, 20, 4, 2, 128, 0, 16, 30, torch.bfloat16, False, False, False)
+    run_append(2, 6, 4, 2, 72, 0, 5, 9, torch.float16, False, True, False)
+    run_append(2, 6, 4, 2, 128, 128, 16, 9, torch.float16, False, True, True, query=False)
+
+
+def test_append_strided_pages_positions_and_query_in_place():
+    g = gen(3)
+    both = torch.full((9, 2, 2, 16, 128), math.nan, device='cuda', dtype=torch.bfloat16)  # K and V of a page together
+    flat = torch.full((9, 16, 2, 128), math.nan, device='cuda', dtype=torch.bfloat16)      # position before head
+    table = torch.tensor([[8, 0, 3], [1, 7, 5]], device='cuda')[:, :2]                     # a wider table's columns
+    q, k, v = (randn(2, h, 5, 128, dtype=torch.bfloat16, g=g) for h in (4, 2, 2))
+    starts = torch.tensor([13, 0], device='cuda')
+    tables = rotation_tables(64, 128)
+    positions = torch.randint(0, 64, (5, 2), device='cuda', generator=g).T
+    ref = paged_append(k, v, both[:, 0], both[:, 1], table, starts, query=q, rotation=tables, positions=positions)
+    plain = pools(9, 2, 16, 128, torch.bfloat16, g)
+    want = paged_append(k, v, *plain, table, starts, query=q, rotation=tables, positions=positions.contiguous())
+    assert torch.equal(ref, want)
+    for i in range(2):
+        assert torch.equal(both[:, i].nan_to_num(9.0), plain[i].nan_to_num(9.0))
+    q2 = q.clone()
+    got = paged_append(k, v, flat.transpose(1, 2), plain[1], table, starts, query=q2, rotation=tables,
+                       positions=positions, query_out=q2)
+    assert got is q2 and torch.equal(q2, want)
+    assert torch.equal(flat.transpose(1, 2).nan_to_num(9.0), plain[0].nan_to_num(9.0))
+    assert _ops.device_error() is None
+
+
+@pytest.mark.parametrize('dim', [128, 40])
+def test_append_reports_what_it_cannot_place(dim):
+    g = gen(4)
+    k, v, q = (randn(3, 2, 4, dim, dtype=torch.bfloat16, g=g) for _ in range(3))
+    tables = rotation_tables(30, dim)
+    good = torch.tensor([[0], [1], [2]], device='cuda')
+
+    def run(table, starts, positions=None):
+        kp, vp = pools(3, 2, 16, dim, torch.bfloat16, g)
+        out = paged_append(k, v, kp, vp, table, torch.tensor(starts, device='cuda'), query=q, rotation=tables,
+                           positions=positions)
+        return kp, vp, out, _ops.device_error()
+
+    for bad in (3, -1, 1 << 40):  # a page outside the pools
+        table = good.clone()
+        table[1] = bad
+        kp, vp, out, err = run(table, [0, 0, 0])
+        assert err is not None and err[0] == 'page table'
+        assert kp[1].isnan().all() and vp[1].isnan().all() and not out[1].any()
+        assert not kp[0, :, :4].isnan().any() and out[2].any()
+    kp, vp, out, err = run(good, [0, 14, -2])  # rows past the table's positions, and before the first
+    assert err[0] == 'page table'
+    assert not kp[1, :, 14:].isnan().any() and kp[1, :, :14].isnan().all() and not out[1, :, 2:].any()
+    assert not kp[2, :, :2].isnan().any() and kp[2, :, 2:].isnan().all() and not out[2, :, :2].any()
+    positions = torch.zeros(3, 4, dtype=torch.long, device='cuda')
+    positions[0, 1], positions[2, 3] = 30, -1  # outside the rotation tables
+    kp, vp, out, err = run(good, [0, 0, 0], positions)
+    assert err[0] == 'rotation index'
+    assert kp[0, :, 1].isnan().all() and vp[2, :, 3].isnan().all() and not out[0, :, 1].any()
+    assert not kp[0, :, 2].isnan().any()
+    assert _ops.device_error() is None
+
+
+# ---- attention -----------------------------------------------------------------------------------
+
+def filled(batch, hkv, dim, page, lengths, dtype, g, scale=1.0, extra=2, slack=0):
+    """Pools that hold NaN wherever no live position is, and the table (entries past the length: -7)."""
+    per = max(1, max(-(-n // page) for n in lengths)) + slack
+    kp, vp = pools(batch * per + extra, hkv, page, dim, dtype, g)
+    order = torch.randperm(batch * per + extra, device='cuda', generator=g)
+    table = torch.full((batch, per), -7, dtype=torch.long, device='cuda')
+    at = 0
+    for b, n in enumerate(lengths):
+        used = -(-n // page)
+        table[b, :used] = order[at:at + used]
+        at += used
+        slot = torch.arange(n, device='cuda')
+        where = table[b][slot // page]
+        kp[where, :, slot % page] = scale * randn(n, hkv, dim, dtype=dtype, g=g)
+        vp[where, :, slot % page] = randn(n, hkv, dim, dtype=dtype, g=g)
+    return kp, vp, table
+
+
+def check_attention(out, q, kp, vp, table, lengths, scale, page, dtype):
+    batch, hq, _, dim = q.shape
+    hkv = kp.shape[1]
+    u = torch.finfo(dtype).eps / 2
+    assert out.shape == (batch, 1, hq, dim)
+    for b, n in enumerate(lengths):
+        if n <= 0:
+            assert not out[b].any()
+            continue
+        slot = torch.arange(n, device='cuda')
+        where = table[b][slot // page]
+        k = kp[where, :, slot % page].double().transpose(0, 1)
+        v = vp[where, :, slot % page].double().transpose(0, 1)
+        qq = q[b, :, 0].double().view(hkv, hq // hkv, dim)
+        s = torch.einsum('hgd,hnd->hgn', qq, k) * scale
+        ref = torch.einsum('hgn,hnd->hgd', torch.softmax(s, -1), v)
+        ds = dim * 2.0 ** -23 * torch.einsum('hgd,hnd->hgn', qq.abs(), k.abs()).amax(-1, keepdim=True) * abs(scale)
+        vmax = v.abs().amax(1, keepdim=True)
+        tol = u * ref.abs() + 2 * (2 * ds + 2.0 ** -20 + 2.0 ** -16 + n * 2.0 ** -24) * vmax
+        err = (out[b, 0].double().view_as(ref) - ref).abs()
+        assert (err <= tol).all(), (b, n, (err - tol).max().item(), err.max().item())
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('hq,hkv,dim,page,lengths', [
+    (16, 2, 128, 16, [1, 0, 200, 15, 16, 17, 33, 640]), (28, 4, 128, 64, [1000, 63, 64, 65, 129]),
+    (40, 8, 128, 128, [4097]), (8, 8, 64, 32, [5, 90, 0, 31, 32, 257]), (12, 1, 128, 16, [100, 1500]),
+    (16, 1, 64, 16, [77, 300]), (4, 2, 256, 16, [1, 19, 500]), (20, 1, 128, 32, [40, 333]), (32, 1, 256, 64, [130]),
+    (6, 2, 128, 1, [50, 3]), (5, 1, 64, 3, [1, 100, 7]), (7, 7, 128, 24, [230, 24, 25]), (14, 2, 128, 8, [64, 9]),
+    (6, 2, 40, 16, [19, 100]), (3, 1, 80, 5, [33, 0, 4]), (2, 2, 192, 16, [70]), (1, 1, 8, 2, [9])])
+def test_attention_over_pages(hq, hkv, dim, page, lengths, dtype):
+    g = gen(hq * 7 + page)
+    batch = len(lengths)
+    kp, vp, table = filled(batch, hkv, dim, page, lengths, dtype, g)
+    q = randn(batch, 1, hq * dim, dtype=dtype, g=g).view(batch, 1, hq, dim).transpose(1, 2)
+    out = paged_attention(q, kp, vp, table, torch.tensor(lengths, device='cuda'))
+    check_attention(out, q, kp, vp, table, lengths, dim ** -0.5, page, dtype)
+    assert _ops.device_error() is None
+
+
+@pytest.mark.parametrize('hq,hkv,batch', [(8, 1, 1), (16, 2, 3), (4, 4, 40), (28, 4, 70)])
+def test_attention_splits_long_and_ragged_lengths(hq, hkv, batch):
+    """One long sequence beside short ones: shares of it end anywhere inside a page or a tile."""
+    g = gen(hq + batch)
+    lengths = [int(x) for x in torch.randint(0, 400, (batch,), generator=torch.Generator().manual_seed(batch))]
+    lengths[batch // 2] = 9001
+    kp, vp, table = filled(batch, hkv, 128, 16, lengths, torch.bfloat16, g)
+    q = randn(batch, hq, 1, 128, dtype=torch.bfloat16, g=g)
+    n = torch.tensor(lengths, device='cuda')
+    out = paged_attention(q, kp, vp, table, n)
+    check_attention(out, q, kp, vp, table, lengths, 128 ** -0.5, 16, torch.bfloat16)
+    assert all(torch.equal(out, paged_attention(q, kp, vp, table, n)) for _ in range(3))  # same order, same bits
+    assert _ops.device_error() is None
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('scale', [8.0, -1.0, 0.0])
+def test_attention_peaked_flat_and_negative_scales(dtype, scale):
+    g = gen(5)
+    lengths = [300, 47]
+    kp, vp, table = filled(2, 2, 128, 16, lengths, dtype, g, scale=0.2)
+    q = randn(2, 16, 1, 128, dtype=dtype, g=g)
+    out = paged_attention(q, kp, vp, table, torch.tensor(lengths, device='cuda'), scale)
+    check_attention(out, q, kp, vp, table, lengths, scale, 16, dtype)
+
+
+def test_attention_rising_scores_and_lowest_values():
+    """Every key beats the ones before it (the running maximum moves each step); keys whose score is
+    hugely negative; a key that holds -inf products (weight 0); one with NaN (its row is NaN)."""
+    g = gen(6)
+    n, dim = 1111, 128
+    kp, vp, table = filled(1, 1, dim, 16, [n], torch.float32, g)
+    q = torch.zeros(1, 2, 1, dim, device='cuda')
+    q[0, 0, 0, 0], q[0, 1, 0, 1] = 1.0, 1.0
+    slot = torch.arange(n, device='cuda')
+    kp[table[0][slot // 16], 0, slot % 16, 0] = slot.float()
+    low = torch.full((n,), -1e30, device='cuda')
+    low[700] = 0.5
+    kp[table[0][slot // 16], 0, slot % 16, 1] = low
+    out = paged_attention(q, kp, vp, table, torch.tensor([n], device='cuda'), 1.0)
+    v = vp[table[0][slot // 16], 0, slot % 16].double()
+    ref = torch.softmax(slot.double(), 0) @ v
+    assert (out[0, 0, 0].double() - ref).abs().max() < 1e-4 * v.abs().max()  # scores to 1111: 2^-14 of them, once
+    assert torch.equal(out[0, 0, 1], v[700].float())
+    kp[table[0][0], 0, 3, 1] = -math.inf
+    assert torch.equal(paged_attention(q[:, 1:], kp, vp, table, torch.tensor([n], device='cuda'), 1.0)[0, 0, 0],
+                       v[700].float())
+    kp[table[0][0], 0, 3, 1] = math.nan
+    assert paged_attention(q[:, 1:], kp, vp, table, torch.tensor([n], device='cuda'), 1.0).isnan().all()
+    # keys of -inf alone leave nothing to attend: zeros, as a length of 0
+    kp[:, :, :, 1] = -math.inf
+    assert not paged_attention(q[:, 1:], kp, vp, table, torch.tensor([40], device='cuda'), 1.0).any()
+
+
+@pytest.mark.parametrize('dim,dtype', [(128, torch.bfloat16), (64, torch.float32), (40, torch.float16)])
+def test_attention_strided_pages_and_query(dim, dtype):
+    g = gen(7)
+    lengths = [70, 33, 128]
+    kp, vp, table = filled(3, 2, dim, 16, lengths, dtype, g)
+    both = torch.stack((kp, vp), 1)                                 # K and V of a page together
+    flat_k, flat_v = (p.transpose(1, 2).contiguous().transpose(1, 2) for p in (kp, vp))  # position before head
+    fused = randn(3, 1, 10 * dim, dtype=dtype, g=g)
+    q = fused[..., :8 * dim].view(3, 1, 8, dim).transpose(1, 2)     # queries of a fused projection
+    n = torch.tensor(lengths, device='cuda')
+    wide = torch.cat((table, table), 1)[:, :table.shape[1]]
+    ref = paged_attention(q.contiguous(), kp, vp, table, n)
+    check_attention(ref, q, kp, vp, table, lengths, dim ** -0.5, 16, dtype)
+    assert torch.equal(paged_attention(q, both[:, 0], both[:, 1], wide, n), ref)
+    assert torch.equal(paged_attention(q, flat_k, flat_v, table, n), ref)
+    odd = torch.zeros(both.numel() + 1, device='cuda', dtype=dtype)[1:].view(both.shape)  # off 16-byte alignment
+    odd.copy_(both)
+    check_attention(paged_attention(q, odd[:, 0], odd[:, 1], table, n), q, kp, vp, table, lengths, dim ** -0.5, 16, dtype)
+    out = torch.full((3, 1, 8, dim), 7.0, device='cuda', dtype=dtype)
+    assert paged_attention(q, kp, vp, table, n, out=out) is out and torch.equal(out, ref)
+
+
+@pytest.mark.parametrize('dim', [128, 40])
+def test_attention_reports_bad_pages_and_lengths(dim):
+    g = gen(8)
+    kp, vp, table = filled(3, 2, dim, 16, [64, 64, 64], torch.bfloat16, g)
+    q = randn(3, 4, 1, dim, dtype=torch.bfloat16, g=g)
+    n = torch.tensor([64, 64, 64], device='cuda')
+    ref = paged_attention(q, kp, vp, table, n)
+    assert _ops.device_error() is None
+    for bad in (-1, kp.shape[0], 1 << 45):
+        t = table.clone()
+        t[1, 2] = bad
+        out = paged_attention(q, kp, vp, t, n)
+        err = _ops.device_error()
+        assert err is not None and err[0] == 'page table'
+        assert torch.equal(out[0], ref[0]) and torch.equal(out[2], ref[2])
+        # the positions of that page are not attended
+        keep = torch.cat((table[1:2, :2], table[1:2, 3:]), 1)
+        want = paged_attention(q[1:2], kp, vp, keep, torch.tensor([48], device='cuda'))
+        assert (out[1] - want[0]).abs().max() <= 2.0 ** -7 * want.abs().max()  # other order of sums: 2 roundings
+    out = paged_attention(q, kp, vp, table, torch.tensor([65, 64, -3], device='cuda'))  # past the table; below zero
+    assert _ops.device_error()[0] == 'page table'
+    assert torch.equal(out[0], ref[0]) and torch.equal(out[1], ref[1]) and not out[2].any()
+
+
+def test_pools_beyond_32_bit_offsets():
+    """Pools of more than 2^31 elements, addressed at their far end."""
+    page, dim = 16, 128
+    pages = (2 ** 31 // (page * dim)) + 40
+    kp = torch.empty(pages, 1, page, dim, device='cuda', dtype=torch.bfloat16)
+    vp = torch.empty_like(kp)
+    g = gen(9)
+    table = torch.tensor([[pages - 1, 5, pages - 30]], device='cuda')
+    k, v = (randn(1, 1, 45, dim, dtype=torch.bfloat16, g=g) for _ in range(2))
+    q = randn(1, 8, 1, dim, dtype=torch.bfloat16, g=g)
+    paged_append(k, v, kp, vp, table, torch.zeros(1, dtype=torch.long, device='cuda'))
+    assert torch.equal(kp[pages - 1, 0], k[0, 0, :16]) and torch.equal(vp[pages - 30, 0, :13], v[0, 0, 32:])
+    out = paged_attention(q, kp, vp, table, torch.tensor([45], device='cuda'))
+    small = paged_attention(q, kp[-40:], vp[-40:], table * 0 + torch.tensor([[39, 0, 10]], device='cuda'),
+                            torch.tensor([16], device='cuda'))
+    check_attention(small, q, kp[-40:], vp[-40:], torch.tensor([[39]], device='cuda'), [16], dim ** -0.5, page,
+                    torch.bfloat16)
+    check_attention(out, q, kp, vp, table, [45], dim ** -0.5, page, torch.bfloat16)
+    assert _ops.device_error() is None
+
+
+def test_streams_and_graphs():
+    """A side stream, and two captured graphs of the same buffers replayed on two streams at once."""
+    g = gen(10)
+    lengths = [3000, 17, 900]
+    kp, vp, table = filled(3, 2, 128, 16, lengths, torch.bfloat16, g)
+    n = torch.tensor(lengths, device='cuda')
+    qs = [randn(3, 16, 1, 128, dtype=torch.bfloat16, g=g) for _ in range(2)]
+    want = [paged_attention(q, kp, vp, table, n) for q in qs]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        assert torch.equal(paged_attention(qs[0], kp, vp, table, n), want[0])
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for q in qs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(paged_attention(q, kp, vp, table, n))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                for _ in range(10):
+                    graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+    n.copy_(torch.tensor([5, 1, 0]))  # lengths are read on the device at each replay
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    check_attention(outs[0], qs[0], kp, vp, table, [5, 1, 0], 128 ** -0.5, 16, torch.bfloat16)
+
+
+def test_empty_calls():
+    kp, vp = pools(1, 2, 16, 128, torch.bfloat16, None)
+    table = torch.zeros(0, 1, dtype=torch.long, device='cuda')
+    none = torch.zeros(0, dtype=torch.long, device='cuda')
+    assert paged_attention(kp.new_zeros(0, 4, 1, 128), kp, vp, table, none).shape == (0, 1, 4, 128)
+    k = kp.new_zeros(0, 2, 3, 128)
+    assert paged_append(k, k, kp, vp, table, none) is None
+    k = kp.new_zeros(2, 2, 0, 128)
+    two = torch.zeros(2, dtype=torch.long, device='cuda')
+    assert paged_append(k, k, kp, vp, two[:, None], two, query=k).shape == k.shape
+    assert kp.isnan().all()
+
+
+# ---- together --------------------------------------------------------------------------------------
+
+def test_decode_loop_with_release_and_admission():
+    """Prompts of unequal length, decode steps, a release and an admission, and the greedy token's
+    log-probability of each step, against dense 64-bit attention over each sequence's own rows."""
+    g = gen(11)
+    hq, hkv, dim, page, vocab = 8, 2, 128, 16, 500
+    dtype, scale = torch.bfloat16, 128 ** -0.5
+    cache = PagedKVCache(40, page, batch_capacity=4, max_length=160)
+    tables = rotation_tables(160, dim)
+    head = randn(hq * dim, vocab, dtype=dtype, g=g) * 0.1
+    history = []  # per live sequence: [(k rotated, v)] per layer
+
+    def forward(counts, first, rows):
+        batch = len(counts)
+        cache.begin(counts, first)
+        for layer in range(2):
+            q, k, v = (randn(batch, h, rows, dim, dtype=dtype, g=g) for h in (hq, hkv, hkv))
+            starts = [cache.lengths[first + b] - counts[b] for b in range(batch)]
+            qr = cache.append(k, v, layer, query=q, rotation=tables)
+            kp, vp = cache._pools[layer]
+            for b in range(batch):
+                seq = history[first + b][layer]
+                at = cache.page_table()[first + b]
+                slot = starts[b] + torch.arange(counts[b], device='cuda')
+                kk, size = turned(k[b, :, :counts[b]].double(), tables[0][slot].double(), tables[1][slot].double(), False)
+                check_rounded(kp[at[slot // page], :, slot % page].transpose(0, 1), kk, size, dtype)
+                seq.append((kp[at[slot // page], :, slot % page], v[b, :, :counts[b]].transpose(0, 1)))
+            if rows == 1:
+                out = cache.attend(qr, layer, scale)
+                for b in range(batch):
+                    kk = torch.cat([x[0] for x in history[first + b][layer]])
+                    vv = torch.cat([x[1] for x in history[first + b][layer]])
+                    n = kk.shape[0]
+                    assert n == cache.lengths[first + b]
+                    # the cache holds this sequence's own rows: a one-page pool of them
+                    check_attention(out[b:b + 1], qr[b:b + 1], kk.transpose(0, 1)[None], vv.transpose(0, 1)[None],
+                                    torch.zeros(1, 1, dtype=torch.long, device='cuda'), [n], scale, n, dtype)
+        if rows == 1:
+            logits = (out.reshape(batch, -1) @ head).float()
+            top = token_logprobs(logits, top=1)
+            again = token_logprobs(logits, top.top_ids[:, 0])
+            assert torch.equal(top.top_ids[:, 0], logits.argmax(-1))
+            assert torch.equal(again.logprobs, top.top_logprobs[:, 0])
+            ref = torch.log_softmax(logits.double(), -1).amax(-1)
+            spread = (logits.amax() - logits.amin()).item()
+            assert (again.logprobs.double() - ref).abs().max() <= 2.0 ** -21 * (1 + spread) + (vocab + 32) * 2.0 ** -24
+
+    def admit(lengths):
+        first = cache.admit(len(lengths))
+        history.extend([[[], []] for _ in lengths])
+        forward(lengths, first, max(lengths))
+
+    admit([17, 1, 50])
+    for _ in range(3):
+        forward([1] * 3, 0, 1)
+    keep = cache.release([False, True, False])
+    assert keep == [0, 2]
+    history[:] = [history[i] for i in keep]
+    forward([1, 1], 0, 1)
+    admit([33, 16])
+    for _ in range(2):
+        forward([1] * 4, 0, 1)
+    assert cache.lengths == [23, 56, 35, 18] and cache.free_pages == 40 - (2 + 4 + 3 + 2)
+    assert _ops.device_error() is None
+    cache.reset()
+    assert cache.free_pages == 40 and not cache.lengths
+
+
+def test_transformers_model_decodes_through_pages():
+    """A random-weight Qwen2: right-padded prompts and decode steps through PagedKVCache and the
+    registered attention, against transformers' own cache and SDPA one sequence at a time."""
+    from transformers import DynamicCache, Qwen2Config, Qwen2ForCausalLM
+    from analysis_spec_b200.tree_attention import register
+    name = register()
+    torch.manual_seed(0)
+    cfg = Qwen2Config(vocab_size=512, hidden_size=512, intermediate_size=1024, num_hidden_layers=2,
+                      num_attention_heads=4, num_key_value_heads=2, max_position_embeddings=512, rms_norm_eps=1e-6,
+                      tie_word_embeddings=False)
+    cfg._attn_implementation = 'sdpa'
+    model = Qwen2ForCausalLM(cfg).to('cuda', torch.bfloat16).eval()
+
+    def use(impl):
+        model.config._attn_implementation = impl
+        for layer in model.model.layers:
+            layer.self_attn.config._attn_implementation = impl
+
+    prompts, steps = [7, 20, 13], 4
+    g = torch.Generator().manual_seed(1)
+    ids = torch.randint(0, 512, (3, 20), generator=g).cuda()
+    new = torch.randint(0, 512, (3, steps), generator=g).cuda()
+    want = []
+    with torch.no_grad():
+        for b, n in enumerate(prompts):
+            past = DynamicCache()
+            logits = [model(input_ids=ids[b:b + 1, :n], past_key_values=past, use_cache=True).logits[:, -1]]
+            for t in range(steps):
+                logits.append(model(input_ids=new[b:b + 1, t:t + 1], past_key_values=past, use_cache=True).logits[:, -1])
+            want.append(torch.cat(logits).float())
+        use(name)
+        cache = PagedKVCache(16, 16, batch_capacity=3, max_length=64)
+        cache.prompt_lengths(prompts)
+        positions = torch.arange(20, device='cuda').expand(3, -1)
+        out = model(input_ids=ids, position_ids=positions, past_key_values=cache, use_cache=True).logits.float()
+        got = [[out[b, n - 1]] for b, n in enumerate(prompts)]
+        for t in range(steps):
+            before = torch.tensor(cache.lengths, device='cuda')[:, None]
+            out = model(input_ids=new[:, t:t + 1], position_ids=before, past_key_values=cache, use_cache=True).logits
+            for b in range(3):
+                got[b].append(out[b, 0].float())
+        assert cache.lengths == [n + steps for n in prompts]
+        with pytest.raises(ValueError, match='one token'):
+            model(input_ids=new[:, :2], position_ids=positions[:, :2], past_key_values=cache, use_cache=True)
+    use('sdpa')
+    for b in range(3):
+        w, o = want[b], torch.stack(got[b])
+        assert (o - w).abs().max() <= 0.06 * w.abs().max()  # two bf16 layers: some tens of roundings of 2^-8
+    assert _ops.device_error() is None

@@ -1,0 +1,175 @@
+"""Refusals of the paged cache and the token log-probabilities before any launch, and the paged
+cache's bookkeeping of pages, on CPU."""
+
+import pytest
+import torch
+
+from analysis_spec_b200 import _lib, _ops
+from analysis_spec_b200.build import build
+from analysis_spec_b200.paged_cache import PagedKVCache, paged_append, paged_attention, rotation_tables
+from analysis_spec_b200.token_logprobs import token_logprobs
+
+
+@pytest.fixture(scope='module')
+def lib():
+    build()
+    return _lib.load()
+
+
+S18, S8, P = _lib.pack_i64(*[0] * 18), _lib.pack_i64(*[0] * 8), 16  # pointers that are never followed
+
+
+def test_append_refuses_on_the_host(lib):
+    def call(batch=1, rows=1, heads=2, dim=128, dtype=_lib.BF16, page=16, pages=4, width=2, stride=2, cos=None, sin=None,
+             rot=0, rot_positions=0, query=None, out=None, hq=0, interleaved=0, key=P, table=P, starts=P):
+        _lib.call('speckv_paged_append', key, P, query, out, P, P, S18, table, stride, width, pages, page, starts, None,
+                  None, 0, 0, cos, sin, rot_positions, rot, interleaved, batch, hq, heads, rows, dim, dtype, None)
+    for match, kw in (('bad sizes', dict(dim=0)), ('bad sizes', dict(batch=-1)), ('unsupported dtype', dict(dtype=7)),
+                      ('query without', dict(query=P)), ('come together', dict(cos=P)),
+                      ('rotation of', dict(cos=P, sin=P, rot=130, rot_positions=4)),
+                      ('rotation of', dict(cos=P, sin=P, rot=3, rot_positions=4)),
+                      ('rotation of', dict(cos=P, sin=P, rot=64)), ('interleaved', dict(interleaved=2)),
+                      ('page geometry', dict(page=0)), ('page geometry', dict(pages=0)),
+                      ('page table rows', dict(batch=2, stride=1)), ('page table rows', dict(table=None)),
+                      ('2\\^31 tokens', dict(batch=1 << 16, rows=1 << 16)), ('null pointer', dict(key=None)),
+                      ('null pointer', dict(starts=None)),
+                      ('2\\^31 positions', dict(width=1 << 30, stride=1 << 30, page=16))):
+        with pytest.raises(_lib.SpecKVError, match=match):
+            call(**kw)
+    call(batch=0)
+    call(rows=0)
+
+
+def test_attention_refuses_on_the_host(lib):
+    def call(batch=1, hq=4, hkv=2, dim=128, dtype=_lib.F16, page=16, q=P, lengths=P):
+        _lib.call('speckv_paged_attention', q, P, P, S8, P, 2, 2, 4, page, lengths, P, batch, hq, hkv, dim, 1.0, dtype,
+                  None)
+    for match, kw in (('bad sizes', dict(dim=0)), ('not a multiple', dict(hq=3)), ('unsupported dtype', dict(dtype=-1)),
+                      ('page geometry', dict(page=-4)), ('above 256', dict(dim=257)), ('null pointer', dict(q=None)),
+                      ('null pointer', dict(lengths=None)), ('2\\^20 sequences', dict(batch=(1 << 20) + 1))):
+        with pytest.raises(_lib.SpecKVError, match=match):
+            call(**kw)
+    call(batch=0)
+
+
+def test_logprobs_refuse_on_the_host(lib):
+    def call(batch=1, per=2, source=2, vocab=10, inv_t=1.0, top=0, dtype=_lib.F32, tokens=P, logprobs=P, tops=None,
+             rows=None):
+        _lib.call('speckv_token_logprobs', P, dtype, 0, 0, tokens, 0, 0, rows, 0, 0, batch, per, source, vocab, inv_t,
+                  top, logprobs, P, P, tops, tops, None)
+    for match, kw in (('bad sizes', dict(vocab=0)), ('unsupported dtype', dict(dtype=9)), ('temperature', dict(inv_t=0.0)),
+                      ('temperature', dict(inv_t=float('nan'))), ('temperature', dict(inv_t=float('inf'))),
+                      ('alternatives', dict(top=11)), ('alternatives', dict(top=33, vocab=100)),
+                      ('null pointer', dict(top=3)), ('null pointer', dict(tokens=None)),
+                      ('null pointer', dict(logprobs=None)), ('rows of logits', dict(source=3)),
+                      ('2\\^31 rows', dict(batch=1 << 20, per=1 << 20, source=1 << 20))):
+        with pytest.raises(_lib.SpecKVError, match=match):
+            call(**kw)
+    call(batch=0)
+
+    def back(entropy=P, g_top=None, top=0, ids=None, g_lp=P, tokens=P):
+        _lib.call('speckv_token_logprobs_backward', P, _lib.F32, 0, 0, tokens, 0, 0, 1, 2, 10, 1.0, top, entropy, P, ids,
+                  g_lp, None, g_top, P, None)
+    for kw in (dict(entropy=None), dict(g_top=P), dict(g_top=P, top=2), dict(tokens=None)):
+        with pytest.raises(_lib.SpecKVError, match='null pointer'):
+            back(**kw)
+
+
+def test_front_end_refuses_cpu_tensors():
+    x = torch.zeros(2, 2, 1, 128)
+    pool, table, n = torch.zeros(4, 2, 16, 128), torch.zeros(2, 2, dtype=torch.long), torch.zeros(2, dtype=torch.long)
+    for go in (lambda: paged_append(x, x, pool, pool, table, n), lambda: paged_attention(x, pool, pool, table, n),
+               lambda: token_logprobs(torch.zeros(2, 5), n)):
+        with pytest.raises(RuntimeError, match='no CPU path'):
+            go()
+
+
+def test_score_operands_are_checked():
+    x, t = torch.zeros(3, 7), torch.zeros(3, dtype=torch.long)
+
+    def check(logits=x, tokens=t, rows=None, top=0, temperature=1.0):
+        return _ops._score_operands('token_logprobs', logits, tokens, rows, top, temperature)
+    for match, kw in (('dtype', dict(logits=x.double())), ('unit stride', dict(logits=torch.zeros(7, 3).T)),
+                      ('vocabulary', dict(logits=torch.zeros(1, 1, 3, 7))), ('alternatives', dict(top=8)),
+                      ('alternatives', dict(top=-1)), ('temperature', dict(temperature=0.0)),
+                      ('temperature', dict(temperature=-1.0)), ('temperature', dict(temperature=float('nan'))),
+                      ('temperature', dict(temperature=float('inf'))), ('tokens', dict(tokens=t[:2])),
+                      ('tokens', dict(tokens=t.int())), ('rows', dict(rows=t[None])),
+                      ('rows', dict(logits=x[None], rows=t))):
+        with pytest.raises(ValueError, match=match):
+            check(**kw)
+    (batch, per, source), ls, ts, rs, shape = check(torch.zeros(2, 3, 7), torch.zeros(2, 5, dtype=torch.long),
+                                                    torch.zeros(2, 5, dtype=torch.long))
+    assert (batch, per, source, ls, ts, rs, tuple(shape)) == (2, 5, 3, (21, 7), (5, 1), (5, 1), (2, 5))
+    assert check()[1] == (0, 7) and check(x[0], t[0])[0] == (1, 1, 1)
+    with pytest.raises(ValueError, match='carries no gradient'):
+        token_logprobs(torch.zeros(1, 3, 7, requires_grad=True), rows=torch.zeros(1, 2, dtype=torch.long))
+
+
+def test_page_bookkeeping(monkeypatch):
+    """Pages handed out and back, table and lengths on the device, refusals that change nothing."""
+    cache = PagedKVCache(8, 4, batch_capacity=3, max_length=20)
+    with pytest.raises(ValueError, match='batch capacity'):
+        cache.admit(4)
+    assert cache.admit(2) == 0
+    cache.begin([5, 9], device='cpu')
+    assert cache.lengths == [5, 9] and cache.free_pages == 3
+    table = cache.page_table()
+    assert table.shape == (2, 5) and len({*table[0, :2].tolist(), *table[1, :3].tolist()}) == 5
+    first, starts, counts, lengths = cache._step
+    assert (first, starts.tolist(), counts.tolist(), lengths.tolist()) == (0, [0, 0], [5, 9], [5, 9])
+    before = cache.page_table().clone()
+    cache.begin()  # one token each, inside the pages held
+    assert cache.lengths == [6, 10] and cache.free_pages == 3 and torch.equal(cache.page_table(), before)
+    assert cache._step[1].tolist() == [5, 9]
+    assert cache.admit(1) == 2
+    with pytest.raises(RuntimeError, match='pages needed'):
+        cache.begin([16], first=2)
+    with pytest.raises(ValueError, match='max_length'):
+        cache.begin([21], first=2)
+    with pytest.raises(ValueError, match='token counts'):
+        cache.begin([-1], first=2)
+    assert cache.lengths == [6, 10, 0] and cache.free_pages == 3
+    cache.begin([12], first=2)
+    assert cache.free_pages == 0 and cache._step[0] == 2
+    last = cache.page_table()[2].tolist()
+    assert cache.release([True, False, False]) == [2, 1]
+    assert cache.lengths == [12, 10] and cache.free_pages == 2 and cache.page_table()[0].tolist() == last
+    with pytest.raises(RuntimeError, match='begin'):
+        cache._begun(2)
+    with pytest.raises(ValueError, match='entry per live'):
+        cache.release([True])
+    cache.reset()
+    assert cache.free_pages == 8 and cache.statistics()['sequences'] == 0
+    assert sorted(cache._free) == list(range(8))
+    for bad in ((0, 4, 1, 4), (4, 0, 1, 4), (4, 4, 0, 4), (4, 4, 1, 0)):
+        with pytest.raises(ValueError, match='positive'):
+            PagedKVCache(bad[0], bad[1], batch_capacity=bad[2], max_length=bad[3])
+
+
+def test_rotation_tables_hold_far_positions():
+    cos, sin = rotation_tables(200001, 64, theta=1e6, device='cpu')
+    assert cos.shape == sin.shape == (200001, 32) and cos.dtype == torch.float32
+    angle = 200000 * 1e6 ** (-2 * 3 / 64)
+    assert abs(cos[200000, 3].item() - __import__('math').cos(angle)) < 1e-6  # fp32 rounding of an exact cosine
+    with pytest.raises(ValueError, match='even'):
+        rotation_tables(4, 3, device='cpu')
+
+
+def test_paged_update_refuses_multi_token_steps(monkeypatch):
+    """The transformers protocol on CPU, with the launch replaced by a recorder."""
+    calls = []
+    monkeypatch.setattr(_ops, 'paged_append', lambda *a: calls.append(a))
+    cache = PagedKVCache(8, 4, batch_capacity=2, max_length=16)
+    k = torch.zeros(2, 1, 3, 8)
+    cache.prompt_lengths([3, 1])
+    assert cache.update(k, k, 0)[0] is k and cache.update(k, k, 1)[0] is k
+    assert cache.lengths == [3, 1] and len(calls) == 2 and calls[0][6].tolist() == [3, 1]
+    assert cache.get_seq_length() == 3 and cache.get_mask_sizes(1) == (4, 0) and len(cache) == 2
+    with pytest.raises(ValueError, match='one token'):
+        cache.update(k, k, 0)
+    keys, values = cache.update(k[:, :, :1], k[:, :, :1], 0)
+    assert keys.shape == (8, 1, 4, 8) and keys._speckv_pages[1].tolist() == [4, 2]
+    assert cache.lengths == [4, 2]
+    with pytest.raises(ValueError, match='live request count'):
+        cache.update(k[:1, :, :1], k[:1, :, :1], 0)

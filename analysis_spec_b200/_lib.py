@@ -72,7 +72,8 @@ SIGNATURES = {
     'speckv_paged_append': [_p, _p, _p, _p, _p, _p, _b, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _i64, _p, _p,
                             _i64, _i64, _i32, _i64, _i64, _i64, _i64, _i64, _i32, _p],
     'speckv_paged_attention': [_p, _p, _p, _b, _p, _i64, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _i64, _f32,
-                               _i32, _p],
+                               _i32, _p, _i64, _p],
+    'speckv_paged_attention_workspace': [_i64, _i64, _i64, _i32],  # returns bytes, not a status
     'speckv_token_logprobs': [_p, _i32, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _f32,
                               _i32, _p, _p, _p, _p, _p, _p],
     'speckv_token_logprobs_backward': [_p, _i32, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _f32, _i32, _p, _p,
@@ -105,6 +106,7 @@ def load():
             lib.speckv_last_error.restype = ctypes.c_char_p
             lib.speckv_remap_scratch_bytes.argtypes = [_i64, _i64, _i64, _i64, _i32]
             lib.speckv_remap_scratch_bytes.restype = ctypes.c_int64
+            lib.speckv_paged_attention_workspace.restype = ctypes.c_int64
             for name in PREPARED:  # same arguments without the stream, then the plan out-pointer
                 fn = getattr(lib, name + '_prepare')
                 fn.argtypes = SIGNATURES[name][:-1] + [_pp]

@@ -860,6 +860,9 @@ def paged_append(key, value, key_pages, value_pages, page_table, starts, counts=
     return query_out
 
 
+_PAGED_WORKSPACE = {}  # (device, q_heads, kv_heads, head_dim, dtype) -> bytes
+
+
 @_on_device
 def paged_attention(query, key_pages, value_pages, page_table, lengths, scale, out=None):
     """speckv_paged_attention (see paged_cache.paged_attention)."""
@@ -882,10 +885,17 @@ def paged_attention(query, key_pages, value_pages, page_table, lengths, scale, o
         raise ValueError(f'{fn}: out must be a contiguous (batch, 1, q_heads, head_dim) tensor of the query dtype')
     if batch == 0:
         return out
+    # a workspace of this call alone: other streams and captured graphs have their own
+    kv_heads, code = key_pages.shape[1], _DTYPE_CODE[dtype]
+    key = (query.get_device(), q_heads, kv_heads, dim, code)
+    need = _PAGED_WORKSPACE.get(key)
+    if need is None:
+        need = _PAGED_WORKSPACE[key] = _lib.load().speckv_paged_attention_workspace(q_heads, kv_heads, dim, code)
+    workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
     _lib.call('speckv_paged_attention', query.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(),
               _lib.pack_i64(qs[0], qs[1], *ks[:3], *vs[:3]), page_table.data_ptr(), page_table.stride(0),
               page_table.shape[1], key_pages.shape[0], key_pages.shape[2], lengths.data_ptr(), out.data_ptr(), batch,
-              q_heads, key_pages.shape[1], dim, float(scale), _DTYPE_CODE[dtype], _stream(query))
+              q_heads, kv_heads, dim, float(scale), code, _ptr(workspace), need, _stream(query))
     return out
 
 

@@ -582,11 +582,20 @@ int speckv_paged_append(const void* key, const void* value, const void* query, v
  * with KV head hq / (q_heads / kv_heads). lengths is a device array of batch int64; a sequence of
  * length 0 (or less) gives zeros. out is contiguous (batch, 1, q_heads, dim). strides: 8 element
  * strides, (b, h) of query and (page, head, position) of key_pages and value_pages. Head dims to
- * 256. */
+ * 256: 64, 128 and 256 in bf16 / fp16 with 16-byte aligned rows take the tensor-core kernel, which
+ * cuts the live positions of all sequences into equal shares and joins what is cut, other views a
+ * CUDA-core kernel. workspace (16-byte aligned, workspace_bytes at least
+ * speckv_paged_attention_workspace of the same shape on the same device; it holds nothing between
+ * calls) may be shared by calls that cannot run at the same time. */
 int speckv_paged_attention(const void* query, const void* key_pages, const void* value_pages, const int64_t* strides,
                            const int64_t* page_table, int64_t table_stride, int64_t table_pages, int64_t num_pages,
                            int64_t page_size, const int64_t* lengths, void* out, int64_t batch, int64_t q_heads,
-                           int64_t kv_heads, int64_t dim, float scale, int32_t dtype, void* stream);
+                           int64_t kv_heads, int64_t dim, float scale, int32_t dtype, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of speckv_paged_attention on the current device, whatever the batch and lengths
+ * (0 for a shape that needs none). */
+int64_t speckv_paged_attention_workspace(int64_t q_heads, int64_t kv_heads, int64_t dim, int32_t dtype);
 
 /* ---- Log-probabilities of tokens ------------------------------------------ */
 

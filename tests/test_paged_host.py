@@ -43,7 +43,7 @@ def test_append_refuses_on_the_host(lib):
 def test_attention_refuses_on_the_host(lib):
     def call(batch=1, hq=4, hkv=2, dim=128, dtype=_lib.F16, page=16, q=P, lengths=P):
         _lib.call('speckv_paged_attention', q, P, P, S8, P, 2, 2, 4, page, lengths, P, batch, hq, hkv, dim, 1.0, dtype,
-                  None)
+                  None, 0, None)
     for match, kw in (('bad sizes', dict(dim=0)), ('not a multiple', dict(hq=3)), ('unsupported dtype', dict(dtype=-1)),
                       ('page geometry', dict(page=-4)), ('above 256', dict(dim=257)), ('null pointer', dict(q=None)),
                       ('null pointer', dict(lengths=None)), ('2\\^20 sequences', dict(batch=(1 << 20) + 1))):

@@ -916,8 +916,8 @@ def _score_operands(fn, logits, tokens, rows, top, temperature):
         raise ValueError(f'{fn}: logits must be ([batch,] [rows,] vocabulary) with unit stride on the vocabulary')
     if not 0 <= top <= min(MAX_TOP, logits.shape[-1]):
         raise ValueError(f'{fn}: {top} alternatives of {logits.shape[-1]} (at most {MAX_TOP})')
-    if not (temperature > 0 and 1.0 / temperature > 0 and 1.0 / temperature < 3e38):
-        raise ValueError(f'{fn}: temperature must be positive and finite, got {temperature}')
+    if not 1e-29 <= temperature <= 1e29:
+        raise ValueError(f'{fn}: temperature must be positive and finite (1e-29 to 1e29), got {temperature}')
     lead = logits.shape[:-1]
     batch, source = (1, 1) if len(lead) == 0 else (1, lead[0]) if len(lead) == 1 else lead
     shape = lead
@@ -934,12 +934,12 @@ def _score_operands(fn, logits, tokens, rows, top, temperature):
 
 @_on_device
 def token_logprobs(logits, tokens=None, rows=None, top=0, temperature=1.0):
-    """speckv_token_logprobs: (logprobs or None, entropy, lse, top_logprobs or None, top_ids or None)."""
+    """speckv_token_logprobs: (logprobs or None, entropy, stats, top_logprobs or None, top_ids or None)."""
     fn = 'token_logprobs'
     _one_device(fn, logits, tokens, rows)
     (batch, per, source), ls, ts, rs, shape = _score_operands(fn, logits, tokens, rows, top, temperature)
     entropy = torch.empty(shape, device=logits.device, dtype=torch.float32)
-    lse = torch.empty_like(entropy)
+    stats = torch.empty((*shape, 2), device=logits.device, dtype=torch.float32)
     logprobs = torch.empty_like(entropy) if tokens is not None else None
     top_logprobs = top_ids = None
     if top:
@@ -947,12 +947,12 @@ def token_logprobs(logits, tokens=None, rows=None, top=0, temperature=1.0):
         top_ids = torch.empty((*shape, top), device=logits.device, dtype=torch.long)
     _lib.call('speckv_token_logprobs', logits.data_ptr(), _DTYPE_CODE[logits.dtype], ls[0], ls[1], _ptr(tokens), ts[0],
               ts[1], _ptr(rows), rs[0], rs[1], batch, per, source, logits.shape[-1], 1.0 / temperature, top,
-              _ptr(logprobs), entropy.data_ptr(), lse.data_ptr(), _ptr(top_logprobs), _ptr(top_ids), _stream(logits))
-    return logprobs, entropy, lse, top_logprobs, top_ids
+              _ptr(logprobs), entropy.data_ptr(), stats.data_ptr(), _ptr(top_logprobs), _ptr(top_ids), _stream(logits))
+    return logprobs, entropy, stats, top_logprobs, top_ids
 
 
 @_on_device
-def token_logprobs_backward(logits, tokens, entropy, lse, top_ids, temperature, grad_logprobs=None, grad_entropy=None,
+def token_logprobs_backward(logits, tokens, entropy, stats, top_ids, temperature, grad_logprobs=None, grad_entropy=None,
                             grad_top_logprobs=None):
     """speckv_token_logprobs_backward: the gradient with respect to the logits (contiguous)."""
     fn = 'token_logprobs_backward'
@@ -966,13 +966,13 @@ def token_logprobs_backward(logits, tokens, entropy, lse, top_ids, temperature, 
                 raise ValueError(f'{fn}: gradient of {name} must be float32 of shape {tuple(want)}')
             g = g.contiguous()
         grads.append(g)
-    for t in (entropy, lse, top_ids):
+    for t in (entropy, stats, top_ids):
         if t is not None and not t.is_contiguous():
-            raise ValueError(f'{fn}: entropy, lse and top_ids are the forward\'s contiguous outputs')
-    _one_device(fn, logits, tokens, entropy, lse, top_ids, *grads)
+            raise ValueError(f'{fn}: entropy, stats and top_ids are the forward\'s contiguous outputs')
+    _one_device(fn, logits, tokens, entropy, stats, top_ids, *grads)
     grad = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
     _lib.call('speckv_token_logprobs_backward', logits.data_ptr(), _DTYPE_CODE[logits.dtype], ls[0], ls[1],
               _ptr(tokens), ts[0], ts[1], batch, per, logits.shape[-1], 1.0 / temperature, top, entropy.data_ptr(),
-              lse.data_ptr(), _ptr(top_ids), _ptr(grads[0]), _ptr(grads[1]), _ptr(grads[2]), grad.data_ptr(),
+              stats.data_ptr(), _ptr(top_ids), _ptr(grads[0]), _ptr(grads[1]), _ptr(grads[2]), grad.data_ptr(),
               _stream(logits))
     return grad

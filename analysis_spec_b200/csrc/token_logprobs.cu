@@ -29,7 +29,7 @@ struct ScoreArgs {
   int top;
   float* logprobs;
   float* entropy;
-  float* lse;
+  float* stats;              // (rows, 2): reference r, log2 of the sum of 2^((x - r) log2(e) / T)
   float* top_logprobs;
   int64_t* top_ids;
   unsigned long long* err;
@@ -72,23 +72,239 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int kScoreThreads = 256;
+__device__ __forceinline__ float order_value(uint32_t key) {
+  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
 
-template <typename F> __device__ __forceinline__ float block_reduce(float x, float* buf, F f) {
-  for (int off = 16; off > 0; off >>= 1) x = f(x, __shfl_xor_sync(0xffffffffu, x, off));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = x;
-  __syncthreads();
-  x = buf[0];
-  for (int w = 1; w < kScoreThreads / 32; ++w) x = f(x, buf[w]);
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Maximum of two numbers; NaN when one of them is.
+__device__ __forceinline__ float max_nan(float x, float y) {
+  float z;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+  return z;
+}
+
+// 16 bytes of logits: their values, and their maximum (NaN when one is).
+template <typename T> struct Vector;
+template <> struct Vector<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void values(const uint4& v, float (&x)[4]) {
+    x[0] = __uint_as_float(v.x);
+    x[1] = __uint_as_float(v.y);
+    x[2] = __uint_as_float(v.z);
+    x[3] = __uint_as_float(v.w);
+  }
+  static __device__ __forceinline__ float top(const uint4& v) {
+    return max_nan(max_nan(__uint_as_float(v.x), __uint_as_float(v.y)),
+                   max_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&x)[4]) {
+    return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+  }
+};
+template <> struct Vector<__nv_bfloat16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ __nv_bfloat162 pair(uint32_t u) { return *reinterpret_cast<__nv_bfloat162*>(&u); }
+  static __device__ __forceinline__ void values(const uint4& v, float (&x)[8]) {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // a bf16 is the upper half of an fp32
+      x[2 * i] = __uint_as_float(u[i] << 16);
+      x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ float top(const uint4& v) {
+    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(pair(v.x), pair(v.y)), __hmax2_nan(pair(v.z), pair(v.w)));
+    return max_nan(__low2float(m), __high2float(m));
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&x)[8]) {
+    uint4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      (&r.x)[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return r;
+  }
+};
+template <> struct Vector<__half> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ __half2 pair(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+  static __device__ __forceinline__ void values(const uint4& v, float (&x)[8]) {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(pair(u[i]));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  }
+  static __device__ __forceinline__ float top(const uint4& v) {
+    const __half2 m = __hmax2_nan(__hmax2_nan(pair(v.x), pair(v.y)), __hmax2_nan(pair(v.z), pair(v.w)));
+    return max_nan(__low2float(m), __high2float(m));
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&x)[8]) {
+    uint4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+      (&r.x)[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return r;
+  }
+};
+
+__device__ __forceinline__ uint4 load_stream(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+
+// A row as single entries up to the first 16-byte boundary, 16-byte vectors, and single entries.
+struct RowSplit {
+  int head, vectors, tail;  // entries, vectors, entries
+  __device__ __forceinline__ RowSplit(const void* row, int vocab, int size) {
+    const int n = 16 / size;
+    head = min(vocab, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / size);
+    vectors = (vocab - head) / n;
+    tail = vocab - head - vectors * n;
+  }
+};
+
+constexpr float kEmpty = -150.f;   // 2^-150 is 0 in fp32: where distances to the reference end
+constexpr float kSlack = 10.f;     // a distance may pass the reference by 2^10 before it moves
+
+// Two fp32 numbers in one register pair, as the packed fp32 instructions take them.
+typedef unsigned long long Two;
+__device__ __forceinline__ Two two(float x, float y) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void parts(Two v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ Two add2(Two x, Two y) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  return r;
+}
+__device__ __forceinline__ Two mul2(Two x, Two y) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  return r;
+}
+__device__ __forceinline__ Two fma2(Two x, Two y, Two z) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+  return r;
+}
+
+// Sums of a thread over its entries, by a reference r (one of its entries) that stays within
+// 2^kSlack of their maximum: y = (x - r) log2(e) / T, s = sum 2^y, t = sum 2^y y. The difference is
+// taken before the product, so that logits of any size (a mask's lowest value among them) keep
+// their distances. best / at: the largest entry and the first entry of the vector that holds it.
+struct Running {
+  float r = -INFINITY, limit = -INFINITY, best = -INFINITY;
+  Two s = 0ull, t = 0ull;  // of the even and the odd entries
+  int at = -1;
+  bool bad = false;  // NaN or +inf seen
+
+  __device__ __forceinline__ void move(float top, float c, float slack) {
+    if (top != top || top == INFINITY) {
+      bad = true;
+      return;
+    }
+    if (top > r) {
+      const float d = fmaxf((r - top) * c, kEmpty), f = exp2_fast(d);  // before the first move s = t = 0
+      t = mul2(two(f, f), fma2(two(d, d), s, t));
+      s = mul2(two(f, f), s);
+      r = top;
+      limit = top + slack;
+    }
+  }
+  __device__ __forceinline__ void add(float x0, float x1, float c) {
+    float y0, y1;
+    parts(mul2(add2(two(x0, x1), two(-r, -r)), two(c, c)), y0, y1);
+    // -inf, and NaN, which is known from the maximum, end at 2^-150
+    y0 = fmaxf(y0, kEmpty);
+    y1 = fmaxf(y1, kEmpty);
+    const Two e = two(exp2_fast(y0), exp2_fast(y1));
+    s = add2(s, e);
+    t = fma2(e, two(y0, y1), t);
+  }
+  __device__ __forceinline__ void track(float top, int index) {
+    if (top > best || at < 0) {
+      best = top;
+      at = index;
+    }
+  }
+};
+
+// Joins the sums of two references.
+__device__ __forceinline__ void join_sums(float& r, float& s, float& t, float r2, float s2, float t2, float c) {
+  const float to = fmaxf(r, r2);  // -inf for both: no entry, sums of 0
+  const float d = fmaxf((r - to) * c, kEmpty), d2 = fmaxf((r2 - to) * c, kEmpty);
+  const float f = exp2_fast(d), f2 = exp2_fast(d2);
+  t = f * fmaf(d, s, t) + f2 * fmaf(d2, s2, t2);
+  s = f * s + f2 * s2;
+  r = to;
+}
+
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t n;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
+  return n;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t n;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(n));
+  return n;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Address of CTA `rank`'s copy of a shared variable.
+__device__ __forceinline__ uint32_t remote(const void* p, uint32_t rank) {
+  uint32_t local = (uint32_t)__cvta_generic_to_shared(p), at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(local), "r"(rank));
+  return at;
+}
+__device__ __forceinline__ float remote_float(const void* p, uint32_t rank) {
+  float x;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(remote(p, rank)) : "memory");
   return x;
+}
+__device__ __forceinline__ unsigned long long remote_u64(const void* p, uint32_t rank) {
+  unsigned long long x;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(x) : "r"(remote(p, rank)) : "memory");
+  return x;
+}
+
+// 32 keys of a warp, largest in lane 0 (bitonic sort).
+__device__ __forceinline__ unsigned long long sort_warp(unsigned long long key) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+    for (int step = size >> 1; step > 0; step >>= 1) {
+      const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, step);
+      const bool larger = ((lane & step) == 0) == ((lane & size) == 0);  // this lane keeps the larger key
+      if ((other > key) == larger) key = other;
+    }
+  return key;
 }
 
 __device__ __forceinline__ void write_skipped(const ScoreArgs& a, long long n) {
   if (threadIdx.x == 0) {
     if (a.logprobs != nullptr) a.logprobs[n] = 0.f;
     a.entropy[n] = 0.f;
-    a.lse[n] = 0.f;
+    a.stats[2 * n] = a.stats[2 * n + 1] = 0.f;
   }
   for (int j = threadIdx.x; j < a.top; j += blockDim.x) {
     a.top_logprobs[n * a.top + j] = 0.f;
@@ -96,98 +312,365 @@ __device__ __forceinline__ void write_skipped(const ScoreArgs& a, long long n) {
   }
 }
 
-// CTA per row: the maximum, then the sums, then k scans for the alternatives.
-template <typename T>
-__global__ void __launch_bounds__(kScoreThreads) token_logprobs_kernel(ScoreArgs a) {
-  __shared__ float buf[kScoreThreads / 32];
-  __shared__ unsigned long long best;
-  const long long n = blockIdx.x;
+// A cluster of CTAs per row, an equal run of its vectors each (one CTA for many rows).
+//
+// One pass over the logits. The alternatives come out of it exactly, whatever the logits: of the
+// threads' largest entries take the k first in the order (value, index). An entry of the top k
+// lies in one of those k threads' entries, else k threads would each hold an entry before it. So
+// those threads' entries alone are read again (k / THREADS of the row, from L2), and the ones not
+// below the k-th key are ranked.
+template <typename T, int THREADS, bool TOP>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel(ScoreArgs a) {
+  typedef Vector<T> Vec;
+  constexpr int WARPS = THREADS / 32, N = Vec::N, AHEAD = 4;
+  __shared__ float s_r[WARPS], s_s[WARPS], s_t[WARPS];
+  __shared__ float s_part[3];
+  __shared__ int s_bad, s_count;
+  __shared__ unsigned long long s_keys[TOP ? WARPS : 1][TOP ? 32 : 1], s_first[TOP ? SPECKV_MAX_TOP : 1],
+      s_list[TOP ? THREADS : 1], s_result[TOP ? SPECKV_MAX_TOP : 1], s_best;
+  const uint32_t ctas = cluster_size(), rank = cluster_rank();
+  const long long n = blockIdx.x / ctas;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, vocab = (int)a.vocab;
   long long offset = 0, token = -1;
   if (!score_row(a, n, offset, token)) {
-    write_skipped(a, n);
-    return;
+    if (rank == 0) write_skipped(a, n);
+    return;  // every CTA of the cluster returns here
   }
   const T* x = static_cast<const T*>(a.logits) + offset;
-  float m = -INFINITY;
-  bool nan = false;
-  for (long long i = threadIdx.x; i < a.vocab; i += kScoreThreads) {
-    const float z = load_f<T>(x[i]);
-    nan |= z != z || z == INFINITY;
-    m = fmaxf(m, z);
+  const RowSplit row(x, vocab, sizeof(T));
+  const int lo = (int)((long long)row.vectors * rank / ctas), hi = (int)((long long)row.vectors * (rank + 1) / ctas);
+  const T* vectors = x + row.head;
+  const float c = a.inv_t * kLog2e, slack = fminf(kSlack / c, 1e30f);
+  if (tid == 0) s_bad = s_count = 0;
+
+  Running w;
+  auto single = [&](int i) {
+    const float v = load_f<T>(x[i]);
+    if (!(v <= w.limit)) w.move(v, c, slack);
+    w.add(v, -INFINITY, c);
+    if (TOP) w.track(v, i);
+  };
+  if (rank == 0 && tid < row.head) single(tid);
+  auto step = [&](const uint4& v, int i) {
+    const float top = Vec::top(v);
+    if (!(top <= w.limit)) w.move(top, c, slack);
+    float f[N];
+    Vec::values(v, f);
+#pragma unroll
+    for (int e = 0; e < N; e += 2) w.add(f[e], f[e + 1], c);
+    if (TOP) w.track(top, row.head + i * N);
+  };
+  {
+    uint4 next[AHEAD];
+    int i = lo + tid;
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+      if (i + u * THREADS < hi) next[u] = load_stream(vectors + (long long)(i + u * THREADS) * N);
+    for (; i + (2 * AHEAD - 1) * THREADS < hi; i += AHEAD * THREADS)
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const uint4 v = next[u];
+        next[u] = load_stream(vectors + (long long)(i + (u + AHEAD) * THREADS) * N);
+        step(v, i + u * THREADS);
+      }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+      if (i + u * THREADS < hi) step(next[u], i + u * THREADS);
+    for (i += AHEAD * THREADS; i < hi; i += THREADS) step(load_stream(vectors + (long long)i * N), i);
   }
-  nan = __syncthreads_or(nan);
-  m = block_reduce(m, buf, [](float u, float v) { return fmaxf(u, v); });
-  const float base = m == -INFINITY ? 0.f : m;
-  float s = 0.f, t = 0.f;
-  for (long long i = threadIdx.x; i < a.vocab; i += kScoreThreads) {
-    const float y = (load_f<T>(x[i]) - base) * a.inv_t;
-    const float e = expf(y);
-    s += e;
-    t += e > 0.f ? e * y : 0.f;
+  if (rank == ctas - 1 && tid < row.tail) single(row.head + row.vectors * N + tid);
+
+  // sums of the CTA
+  float r = w.r, s, t;
+  {
+    float s2, t2;
+    parts(w.s, s, s2);
+    parts(w.t, t, t2);
+    s += s2;
+    t += t2;
   }
-  s = block_reduce(s, buf, [](float u, float v) { return u + v; });
-  t = block_reduce(t, buf, [](float u, float v) { return u + v; });
-  const bool empty = m == -INFINITY && !nan;
-  const float log_s = logf(s);
-  const float lse = nan ? NAN : empty ? -INFINITY : base * a.inv_t + log_s;
-  if (threadIdx.x == 0) {
-    if (a.logprobs != nullptr) {
-      const float y = (load_f<T>(x[token]) - base) * a.inv_t;
-      a.logprobs[n] = nan ? NAN : empty ? -INFINITY : y - log_s;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    const float r2 = __shfl_xor_sync(0xffffffffu, r, off), s2 = __shfl_xor_sync(0xffffffffu, s, off),
+                t2 = __shfl_xor_sync(0xffffffffu, t, off);
+    join_sums(r, s, t, r2, s2, t2, c);
+  }
+  if (lane == 0) {
+    s_r[warp] = r;
+    s_s[warp] = s;
+    s_t[warp] = t;
+  }
+  unsigned long long key = 0;
+  if (TOP) {
+    if (w.at >= 0) key = (unsigned long long)order_key(w.best) << 32 | (0xffffffffu - (uint32_t)w.at);
+    key = sort_warp(key);
+    s_keys[warp][lane] = key;
+  }
+  __syncthreads();
+  if (w.bad) s_bad = 1;
+  if (warp == 0) {
+    // the joins of the warps' sums, in one order
+    r = lane < WARPS ? s_r[lane] : -INFINITY;
+    s = lane < WARPS ? s_s[lane] : 0.f;
+    t = lane < WARPS ? s_t[lane] : 0.f;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+      const float r2 = __shfl_xor_sync(0xffffffffu, r, off), s2 = __shfl_xor_sync(0xffffffffu, s, off),
+                  t2 = __shfl_xor_sync(0xffffffffu, t, off);
+      join_sums(r, s, t, r2, s2, t2, c);
     }
-    a.entropy[n] = nan ? NAN : empty ? 0.f : log_s - t / s;
-    a.lse[n] = lse;
-  }
-  unsigned long long last = ~0ull;
-  for (int j = 0; j < a.top; ++j) {
-    __syncthreads();
-    if (threadIdx.x == 0) best = 0ull;
-    __syncthreads();
-    unsigned long long mine = 0ull;
-    for (long long i = threadIdx.x; i < a.vocab; i += kScoreThreads) {
-      const unsigned long long key = (unsigned long long)order_key(load_f<T>(x[i])) << 32 | (0xffffffffu - (uint32_t)i);
-      if (key < last && key > mine) mine = key;
+    if (lane == 0) {
+      s_part[0] = r;
+      s_part[1] = s;
+      s_part[2] = t;
     }
-    atomicMax(&best, mine);
-    __syncthreads();
-    last = best;
-    if (threadIdx.x == 0) {
-      const long long id = 0xffffffffu - (uint32_t)last;
-      a.top_ids[n * a.top + j] = id;
-      const float y = (load_f<T>(x[id]) - base) * a.inv_t;
-      a.top_logprobs[n * a.top + j] = nan ? NAN : empty ? -INFINITY : y - log_s;
+    if (TOP) {  // the k first of the threads' keys: the warps' sorted lists, merged
+      int head = 0;
+      key = lane < WARPS ? s_keys[lane][0] : 0ull;
+      for (int j = 0; j < a.top; ++j) {
+        const uint32_t high = (uint32_t)(key >> 32), most = __reduce_max_sync(0xffffffffu, high);
+        const uint32_t low = high == most ? (uint32_t)key : 0u, least = __reduce_max_sync(0xffffffffu, low);
+        if (lane == 0) s_first[j] = (unsigned long long)most << 32 | least;
+        if (lane < WARPS && high == most && (uint32_t)key == least) {
+          ++head;
+          key = head < 32 ? s_keys[lane][head] : 0ull;
+        }
+      }
     }
   }
+  __syncthreads();
+  if (TOP) {
+    const int k = a.top;
+    // a thread's key names the vector of its largest entry: that entry is one of N
+    const unsigned long long threshold = s_first[k - 1] == 0ull ? 0ull : s_first[k - 1] - (N - 1);
+    auto offer = [&](int i) {
+      const unsigned long long e = (unsigned long long)order_key(load_f<T>(x[i])) << 32 | (0xffffffffu - (uint32_t)i);
+      if (e >= threshold) {
+        const int place = atomicAdd(&s_count, 1);
+        if (place < THREADS) s_list[place] = e;
+      }
+    };
+    if (!s_bad) {
+      for (int j = warp; j < k; j += WARPS) {
+        if (s_first[j] == 0ull) continue;  // fewer threads than k hold entries
+        const int at = (int)(0xffffffffu - (uint32_t)s_first[j]);
+        const int after = at - row.head - row.vectors * N;
+        const int owner = at < row.head ? at : after >= 0 ? after : ((at - row.head) / N - lo) % THREADS;
+        if (lane == 0) {
+          if (rank == 0 && owner < row.head) offer(owner);
+          if (rank == ctas - 1 && owner < row.tail) offer(row.head + row.vectors * N + owner);
+        }
+        for (int i = lo + owner + lane * THREADS; i < hi; i += 32 * THREADS) {
+          const uint4 v = *reinterpret_cast<const uint4*>(vectors + (long long)i * N);
+          float f[N];
+          Vec::values(v, f);
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            const uint32_t index = (uint32_t)(row.head + i * N + e);
+            const unsigned long long cand = (unsigned long long)order_key(f[e]) << 32 | (0xffffffffu - index);
+            if (cand >= threshold) {
+              const int place = atomicAdd(&s_count, 1);
+              if (place < THREADS) s_list[place] = cand;
+            }
+          }
+        }
+      }
+    }
+    if (tid < SPECKV_MAX_TOP) s_result[tid] = 0ull;
+    __syncthreads();
+    if (!s_bad && s_count <= THREADS) {
+      if (tid < s_count) {
+        const unsigned long long own = s_list[tid];
+        int before = 0;
+        for (int i = 0; i < s_count; ++i) before += s_list[i] > own;
+        if (before < k) s_result[before] = own;
+      }
+    } else {
+      // NaN among the logits (its order is not the threads'), or more entries than the list
+      // holds at or above the threshold: k scans
+      unsigned long long last = ~0ull;
+      for (int j = 0; j < k; ++j) {
+        __syncthreads();
+        if (tid == 0) s_best = 0ull;
+        __syncthreads();
+        unsigned long long mine = 0ull;
+        auto scan = [&](int i) {
+          const unsigned long long e =
+              (unsigned long long)order_key(load_f<T>(x[i])) << 32 | (0xffffffffu - (uint32_t)i);
+          if (e < last && e > mine) mine = e;
+        };
+        if (rank == 0 && tid < row.head) scan(tid);
+        for (int i = lo * N + tid; i < hi * N; i += THREADS) scan(row.head + i);
+        if (rank == ctas - 1 && tid < row.tail) scan(row.head + row.vectors * N + tid);
+        if (mine) atomicMax(&s_best, mine);
+        __syncthreads();
+        last = s_best;
+        if (tid == 0) s_result[j] = last;
+        if (last == 0ull) break;
+      }
+    }
+    __syncthreads();
+  }
+  bool bad = s_bad;
+  r = s_part[0];
+  s = s_part[1];
+  t = s_part[2];
+  if (ctas > 1) {
+    cluster_sync();
+    if (rank == 0) {
+      for (uint32_t o = 1; o < ctas; ++o) {
+        join_sums(r, s, t, remote_float(&s_part[0], o), remote_float(&s_part[1], o), remote_float(&s_part[2], o), c);
+        bad |= __float_as_int(remote_float(&s_bad, o)) != 0;
+      }
+    }
+  }
+  if (rank == 0) {
+    const float log_s = log2f(s);
+    const bool empty = r == -INFINITY && !bad;
+    auto logprob = [&](float v) { return bad ? NAN : empty ? -INFINITY : (v - r) * a.inv_t - log_s * kLn2; };
+    if (tid == 0) {
+      if (a.logprobs != nullptr) a.logprobs[n] = logprob(load_f<T>(x[token]));
+      a.entropy[n] = bad ? NAN : empty ? 0.f : fmaxf(log_s - t / s, 0.f) * kLn2;
+      a.stats[2 * n] = bad ? NAN : r;
+      a.stats[2 * n + 1] = bad ? NAN : empty ? -INFINITY : log_s;
+    }
+    if (TOP) {
+      const int k = a.top;
+      auto emit = [&](int place, unsigned long long e) {
+        const long long at = n * k + place;
+        a.top_ids[at] = 0xffffffffu - (uint32_t)e;
+        a.top_logprobs[at] = logprob(order_value((uint32_t)(e >> 32)));
+      };
+      if (ctas == 1) {
+        if (tid < k) emit(tid, s_result[tid]);
+      } else {
+        // the CTAs' alternatives (at most 8 x 32), ranked
+        for (int i = tid; i < (int)ctas * k; i += THREADS) {
+          const unsigned long long own = remote_u64(&s_result[i % k], i / k);
+          int before = 0;
+          for (int o = 0; o < (int)ctas * k; ++o) before += remote_u64(&s_result[o % k], o / k) > own;
+          if (own != 0ull && before < k) emit(before, own);
+        }
+      }
+    }
+  }
+  if (ctas > 1) cluster_sync();  // the other CTAs' shared memory is read until here
 }
 
-// CTA per row, elements one by one.
+constexpr int kGradThreads = 256;
+constexpr int kGradSpan = 8;  // vectors a thread handles
+
+// CTA per (row, run of vectors). One exponential and one product chain an entry:
+//   dx = p (u + v y) with y = log2 p, u = -(sum of gradients + g_H H) / T,
+//   v = -g_H ln(2) / T; the token and the alternatives add their own gradient afterwards.
 template <typename T>
-__global__ void __launch_bounds__(kScoreThreads) token_logprobs_backward_kernel(ScoreArgs a) {
-  const long long n = blockIdx.x;
+__global__ void __launch_bounds__(kGradThreads) token_logprobs_backward_kernel(ScoreArgs a, int runs) {
+  typedef Vector<T> Vec;
+  constexpr int N = Vec::N;
+  const long long n = blockIdx.x / runs;
+  const int part = (int)(blockIdx.x - n * runs), tid = threadIdx.x, vocab = (int)a.vocab;
   T* g = static_cast<T*>(a.grad) + n * a.vocab;
+  const RowSplit row(g, vocab, sizeof(T));
+  const int lo = part * kGradThreads * kGradSpan, hi = min(row.vectors, lo + kGradThreads * kGradSpan);
+  const int e_lo = part == 0 ? 0 : row.head + lo * N, e_hi = part == runs - 1 ? vocab : row.head + hi * N;
   long long offset = 0, token = -1;
-  const bool live = score_row(a, n, offset, token) && a.lse[n] != -INFINITY;
-  if (!live) {
-    for (long long i = threadIdx.x; i < a.vocab; i += kScoreThreads) g[i] = store_f<T>(0.f);
+  if (!score_row(a, n, offset, token) || a.stats[2 * n] == -INFINITY) {
+    for (int i = lo + tid; i < hi; i += kGradThreads)
+      *reinterpret_cast<uint4*>(g + row.head + (long long)i * N) = make_uint4(0, 0, 0, 0);
+    if (part == 0 && tid < row.head) g[tid] = store_f<T>(0.f);
+    if (part == runs - 1 && tid < row.tail) g[row.head + row.vectors * N + tid] = store_f<T>(0.f);
     return;
   }
   const T* x = static_cast<const T*>(a.logits) + offset;
   const float ga = a.g_logprobs != nullptr ? a.g_logprobs[n] : 0.f;
   const float gh = a.g_entropy != nullptr ? a.g_entropy[n] : 0.f;
-  const float lse = a.lse[n], entropy = a.entropy[n];
   float all = ga;
   if (a.g_top != nullptr)
     for (int j = 0; j < a.top; ++j) all += a.g_top[n * a.top + j];
-  for (long long i = threadIdx.x; i < a.vocab; i += kScoreThreads) {
-    const float logp = load_f<T>(x[i]) * a.inv_t - lse;
-    const float p = expf(logp);
-    float d = p == 0.f ? 0.f : -p * (all + gh * (logp + entropy));
-    if (i == token) d += ga;
-    if (a.g_top != nullptr)
-      for (int j = 0; j < a.top; ++j)
-        if (a.top_ids[n * a.top + j] == i) d += a.g_top[n * a.top + j];
-    g[i] = store_f<T>(d * a.inv_t);
+  const float c = a.inv_t * kLog2e, r = a.stats[2 * n], log_s = a.stats[2 * n + 1];
+  const float u = -a.inv_t * (all + gh * a.entropy[n]), v = -a.inv_t * gh * kLn2;  // NaN rows: u is NaN
+  auto slope = [&](float z) {
+    const float y = fmaxf(fmaf(z - r, c, -log_s), kEmpty);  // -inf: weight 0, not 0 x inf
+    return exp2_fast(y) * fmaf(v, y, u);
+  };
+  const bool aligned = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
+  if (aligned) {
+    constexpr int AHEAD = 4;
+    for (int i = lo + tid; i < hi; i += AHEAD * kGradThreads) {
+      uint4 in[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+        if (i + k * kGradThreads < hi) in[k] = load_stream(x + row.head + (long long)(i + k * kGradThreads) * N);
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+        if (i + k * kGradThreads < hi) {
+          float f[N];
+          Vec::values(in[k], f);
+#pragma unroll
+          for (int e = 0; e < N; ++e) f[e] = slope(f[e]);
+          *reinterpret_cast<uint4*>(g + row.head + (long long)(i + k * kGradThreads) * N) = Vec::pack(f);
+        }
+    }
+  } else {
+    for (int i = row.head + lo * N + tid; i < row.head + hi * N; i += kGradThreads)
+      g[i] = store_f<T>(slope(load_f<T>(x[i])));
   }
+  if (part == 0 && tid < row.head) g[tid] = store_f<T>(slope(load_f<T>(x[tid])));
+  if (part == runs - 1 && tid < row.tail) {
+    const int i = row.head + row.vectors * N + tid;
+    g[i] = store_f<T>(slope(load_f<T>(x[i])));
+  }
+  // the entries that have a gradient of their own, each written once more, whole
+  const int extra = a.g_top != nullptr ? a.top : 0;
+  if (extra == 0 && ga == 0.f) return;
+  __syncthreads();
+  for (int j = tid; j <= extra; j += kGradThreads) {
+    long long id = token;
+    float own = ga;
+    if (j < extra) {
+      id = a.top_ids[n * a.top + j];
+      own = a.g_top[n * a.top + j] + (id == token ? ga : 0.f);
+    } else {
+      for (int k = 0; k < extra; ++k)
+        if (a.top_ids[n * a.top + k] == token) id = -1;  // counted with that alternative
+    }
+    if (id >= e_lo && id < e_hi) g[id] = store_f<T>(fmaf(own, a.inv_t, slope(load_f<T>(x[id]))));
+  }
+}
+
+template <typename T, int THREADS, bool TOP>
+int launch_scores_as(const char* fn, const ScoreArgs& a, int ctas, cudaStream_t s) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ctas;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.batch * a.per * ctas));
+  cfg.blockDim = dim3(THREADS);
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, THREADS, TOP>, a);
+  if (e != cudaSuccess) return fail(SPECKV_ECUDA, "%s: launch failed: %s", fn, cudaGetErrorString(e));
+  return SPECKV_OK;
+}
+
+template <typename T>
+int launch_scores(const char* fn, const ScoreArgs& a, cudaStream_t s) {
+  const long long rows = a.batch * a.per, vectors = a.vocab * sizeof(T) / 16;
+  int ctas = 1;
+  while (ctas < 8 && rows * ctas * 2 <= 296 && vectors / (ctas * 2) >= 512) ctas *= 2;
+  if (rows * ctas >= (1ll << 31)) return fail(SPECKV_ENOSUPPORT, "%s: too many rows", fn);
+  return a.top > 0 ? launch_scores_as<T, 512, true>(fn, a, ctas, s) : launch_scores_as<T, 512, false>(fn, a, ctas, s);
+}
+
+template <typename T>
+int launch_gradient(const char* fn, const ScoreArgs& a, cudaStream_t s) {
+  const long long vectors = a.vocab * (long long)sizeof(T) / 16, span = kGradThreads * kGradSpan;
+  const long long runs = vectors <= span ? 1 : (vectors + span - 1) / span;
+  if (a.batch * a.per * runs >= (1ll << 31)) return fail(SPECKV_ENOSUPPORT, "%s: too many rows", fn);
+  token_logprobs_backward_kernel<T><<<(unsigned)(a.batch * a.per * runs), kGradThreads, 0, s>>>(a, (int)runs);
+  return check_launch(fn);
 }
 
 int check_scores(const char* fn, const void* logits, int32_t dtype, const int64_t* tokens, int64_t batch, int64_t per,
@@ -195,8 +678,8 @@ int check_scores(const char* fn, const void* logits, int32_t dtype, const int64_
   if (batch < 0 || per < 0 || source_rows < 0 || vocab < 1) return fail(SPECKV_EINVAL, "%s: bad sizes", fn);
   if (dtype != SPECKV_F32 && dtype != SPECKV_BF16 && dtype != SPECKV_F16)
     return fail(SPECKV_EINVAL, "%s: unsupported dtype %d", fn, dtype);
-  if (!(inv_temperature > 0.f) || !(inv_temperature <= 3.0e38f))
-    return fail(SPECKV_EINVAL, "%s: 1 / temperature must be positive and finite", fn);
+  if (!(inv_temperature >= 1e-30f) || !(inv_temperature <= 1e30f))
+    return fail(SPECKV_EINVAL, "%s: 1 / temperature must lie in [1e-30, 1e30]", fn);
   if (top < 0 || top > SPECKV_MAX_TOP || top > vocab)
     return fail(SPECKV_EINVAL, "%s: %d alternatives of %lld (at most %d)", fn, top, (long long)vocab, SPECKV_MAX_TOP);
   if (vocab >= (1ll << 31) || batch > (1ll << 31) || per > (1ll << 31) || batch * per >= (1ll << 31))
@@ -213,14 +696,14 @@ extern "C" int speckv_token_logprobs(const void* logits, int32_t dtype, int64_t 
                                      const int64_t* tokens, int64_t tokens_stride_b, int64_t tokens_stride_r,
                                      const int64_t* rows, int64_t rows_stride_b, int64_t rows_stride_r,
                                      int64_t batch, int64_t per_batch, int64_t source_rows, int64_t vocab,
-                                     float inv_temperature, int32_t top, float* logprobs, float* entropy, float* lse,
+                                     float inv_temperature, int32_t top, float* logprobs, float* entropy, float* stats,
                                      float* top_logprobs, int64_t* top_ids, void* stream) {
   const char* fn = "speckv_token_logprobs";
   int st = check_scores(fn, logits, dtype, tokens, batch, per_batch, source_rows, vocab, inv_temperature, top);
   if (st || batch == 0 || per_batch == 0) return st;
   if (rows == nullptr && source_rows != per_batch)
     return fail(SPECKV_EINVAL, "%s: %lld rows of logits for %lld", fn, (long long)source_rows, (long long)per_batch);
-  if (logits == nullptr || entropy == nullptr || lse == nullptr || (tokens == nullptr) != (logprobs == nullptr) ||
+  if (logits == nullptr || entropy == nullptr || stats == nullptr || (tokens == nullptr) != (logprobs == nullptr) ||
       (top > 0 && (top_logprobs == nullptr || top_ids == nullptr)))
     return fail(SPECKV_EINVAL, "%s: null pointer", fn);
   st = check_current_device(fn, {logits, tokens, entropy});
@@ -243,32 +726,30 @@ extern "C" int speckv_token_logprobs(const void* logits, int32_t dtype, int64_t 
   a.top = top;
   a.logprobs = logprobs;
   a.entropy = entropy;
-  a.lse = lse;
+  a.stats = stats;
   a.top_logprobs = top_logprobs;
   a.top_ids = top_ids;
   a.err = device_error_word();
   if (a.err == nullptr) return fail(SPECKV_ECUDA, "%s: no error word on device", fn);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const unsigned grid = (unsigned)(batch * per_batch);
   switch (dtype) {
-    case SPECKV_F32: token_logprobs_kernel<float><<<grid, kScoreThreads, 0, s>>>(a); break;
-    case SPECKV_BF16: token_logprobs_kernel<__nv_bfloat16><<<grid, kScoreThreads, 0, s>>>(a); break;
-    default: token_logprobs_kernel<__half><<<grid, kScoreThreads, 0, s>>>(a); break;
+    case SPECKV_F32: return launch_scores<float>(fn, a, s);
+    case SPECKV_BF16: return launch_scores<__nv_bfloat16>(fn, a, s);
+    default: return launch_scores<__half>(fn, a, s);
   }
-  return check_launch(fn);
 }
 
 extern "C" int speckv_token_logprobs_backward(const void* logits, int32_t dtype, int64_t stride_b, int64_t stride_r,
                                               const int64_t* tokens, int64_t tokens_stride_b, int64_t tokens_stride_r,
                                               int64_t batch, int64_t per_batch, int64_t vocab, float inv_temperature,
-                                              int32_t top, const float* entropy, const float* lse,
+                                              int32_t top, const float* entropy, const float* stats,
                                               const int64_t* top_ids, const float* grad_logprobs,
                                               const float* grad_entropy, const float* grad_top_logprobs,
                                               void* grad_logits, void* stream) {
   const char* fn = "speckv_token_logprobs_backward";
   int st = check_scores(fn, logits, dtype, tokens, batch, per_batch, per_batch, vocab, inv_temperature, top);
   if (st || batch == 0 || per_batch == 0) return st;
-  if (logits == nullptr || entropy == nullptr || lse == nullptr || grad_logits == nullptr ||
+  if (logits == nullptr || entropy == nullptr || stats == nullptr || grad_logits == nullptr ||
       (grad_logprobs != nullptr && tokens == nullptr) ||
       (grad_top_logprobs != nullptr && (top < 1 || top_ids == nullptr)))
     return fail(SPECKV_EINVAL, "%s: null pointer", fn);
@@ -288,7 +769,7 @@ extern "C" int speckv_token_logprobs_backward(const void* logits, int32_t dtype,
   a.inv_t = inv_temperature;
   a.top = top;
   a.entropy = const_cast<float*>(entropy);
-  a.lse = const_cast<float*>(lse);
+  a.stats = const_cast<float*>(stats);
   a.top_ids = const_cast<int64_t*>(top_ids);
   a.g_logprobs = grad_logprobs;
   a.g_entropy = grad_entropy;
@@ -297,11 +778,9 @@ extern "C" int speckv_token_logprobs_backward(const void* logits, int32_t dtype,
   a.err = device_error_word();
   if (a.err == nullptr) return fail(SPECKV_ECUDA, "%s: no error word on device", fn);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const unsigned grid = (unsigned)(batch * per_batch);
   switch (dtype) {
-    case SPECKV_F32: token_logprobs_backward_kernel<float><<<grid, kScoreThreads, 0, s>>>(a); break;
-    case SPECKV_BF16: token_logprobs_backward_kernel<__nv_bfloat16><<<grid, kScoreThreads, 0, s>>>(a); break;
-    default: token_logprobs_backward_kernel<__half><<<grid, kScoreThreads, 0, s>>>(a); break;
+    case SPECKV_F32: return launch_gradient<float>(fn, a, s);
+    case SPECKV_BF16: return launch_gradient<__nv_bfloat16>(fn, a, s);
+    default: return launch_gradient<__half>(fn, a, s);
   }
-  return check_launch(fn);
 }

@@ -23,8 +23,8 @@ class TokenLogprobs(NamedTuple):
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top, temperature):
-        logprobs, entropy, lse, top_logprobs, top_ids = _ops.token_logprobs(logits, tokens, None, top, temperature)
-        ctx.save_for_backward(logits, tokens, entropy, lse, top_ids)
+        logprobs, entropy, stats, top_logprobs, top_ids = _ops.token_logprobs(logits, tokens, None, top, temperature)
+        ctx.save_for_backward(logits, tokens, entropy, stats, top_ids)
         ctx.temperature = temperature
         ctx.set_materialize_grads(False)
         if top_ids is not None:
@@ -34,10 +34,10 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_logprobs, grad_entropy, grad_top_logprobs, _):
-        logits, tokens, entropy, lse, top_ids = ctx.saved_tensors
+        logits, tokens, entropy, stats, top_ids = ctx.saved_tensors
         if grad_logprobs is None and grad_entropy is None and grad_top_logprobs is None:
             return None, None, None, None
-        return _ops.token_logprobs_backward(logits, tokens, entropy, lse, top_ids, ctx.temperature, grad_logprobs,
+        return _ops.token_logprobs_backward(logits, tokens, entropy, stats, top_ids, ctx.temperature, grad_logprobs,
                                             grad_entropy, grad_top_logprobs), None, None, None
 
 

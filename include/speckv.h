@@ -610,14 +610,16 @@ int64_t speckv_paged_attention_workspace(int64_t q_heads, int64_t kv_heads, int6
  * source row is negative is skipped: it is not read, its outputs are 0 and its ids -1; so is one
  * whose token is >= vocab or whose source row is >= source_rows, which also sets device error
  * SPECKV_DERR_TOKEN_INDEX. A row of -inf alone: logprobs and top_logprobs -inf, entropy 0. A row
- * with a NaN or +inf: NaN. lse is kept for the gradient. Without rows, source_rows == per_batch.
+ * with a NaN or +inf: NaN. stats (2 fp32 a row: an entry r of the row and log2 sum_i
+ * 2^((x_i - r) log2(e) inv_temperature)) is kept for the gradient. inv_temperature lies in
+ * [1e-30, 1e30]. Without rows, source_rows == per_batch.
  * The numbers that the reference's sampler and GRPO loss take from the logits with log_softmax,
  * gather, argmax and topk (helper/opd_sampling.py:162-170, helper/fastgrpo_training.py). */
 int speckv_token_logprobs(const void* logits, int32_t dtype, int64_t stride_b, int64_t stride_r,
                           const int64_t* tokens, int64_t tokens_stride_b, int64_t tokens_stride_r,
                           const int64_t* rows, int64_t rows_stride_b, int64_t rows_stride_r, int64_t batch,
                           int64_t per_batch, int64_t source_rows, int64_t vocab, float inv_temperature, int32_t top,
-                          float* logprobs, float* entropy, float* lse, float* top_logprobs, int64_t* top_ids,
+                          float* logprobs, float* entropy, float* stats, float* top_logprobs, int64_t* top_ids,
                           void* stream);
 
 /* Gradient of speckv_token_logprobs (without rows) with respect to the logits, from the
@@ -625,11 +627,11 @@ int speckv_token_logprobs(const void* logits, int32_t dtype, int64_t stride_b, i
  *   grad[b][r][i] = inv_temperature * (g_lp (d(i, token) - p_i) - g_H p_i (log p_i + entropy)
  *                                      + sum_k g_top[k] (d(i, top_ids[k]) - p_i))
  * grad_logits is contiguous (batch, per_batch, vocab) in the logits' dtype; skipped rows and rows
- * of -inf alone get zeros. entropy, lse and top_ids are the forward's. */
+ * of -inf alone get zeros. entropy, stats and top_ids are the forward's. */
 int speckv_token_logprobs_backward(const void* logits, int32_t dtype, int64_t stride_b, int64_t stride_r,
                                    const int64_t* tokens, int64_t tokens_stride_b, int64_t tokens_stride_r,
                                    int64_t batch, int64_t per_batch, int64_t vocab, float inv_temperature,
-                                   int32_t top, const float* entropy, const float* lse, const int64_t* top_ids,
+                                   int32_t top, const float* entropy, const float* stats, const int64_t* top_ids,
                                    const float* grad_logprobs, const float* grad_entropy,
                                    const float* grad_top_logprobs, void* grad_logits, void* stream);
 

@@ -122,6 +122,31 @@ def test_ties_and_orders(dtype, vocab):
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('vocab', [7, 2500, 40000])
+def test_rows_of_extreme_values(dtype, vocab):
+    """Rows that hold only a mask's lowest value, or large equal values, are uniform; gradients too."""
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    x = torch.full((4, vocab), low, device='cuda', dtype=dtype)
+    x[1] = high
+    x[2] = low / 4
+    x[3, vocab // 2] = high  # the distance passes the type's range
+    tokens = torch.full((4,), vocab // 2, device='cuda')
+    x.requires_grad_(True)
+    r = token_logprobs(x, tokens, top=3, temperature=0.5)
+    e = 2.0 ** -21 + (vocab / 128 + 32) * 2.0 ** -24
+    assert (r.logprobs[:3] + math.log(vocab)).abs().max() <= e * math.log(vocab) + e
+    assert (r.entropy[:3] - math.log(vocab)).abs().max() <= e * math.log(vocab) + e
+    assert r.logprobs[3] == 0 and r.entropy[3] == 0
+    assert torch.equal(r.top_ids, order(x.detach(), 3))
+    grad, = torch.autograd.grad(r.logprobs, x, torch.ones(4, device='cuda'))
+    want = torch.full((4, vocab), -2.0 / vocab, device='cuda', dtype=torch.float64)
+    want[:, vocab // 2] += 2.0
+    want[3] = 0.0
+    u = torch.finfo(dtype).eps / 2
+    assert ((grad.double() - want).abs() <= (u + 4 * e) * want.abs() + 2 * e * 2 / vocab + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
 def test_nan_and_infinity(dtype):
     x = some_logits(4, 3000, dtype, gen(1))
     x[0, 1234] = math.nan

@@ -4,7 +4,6 @@ The library is loaded on first use. A missing library is an error, never a
 silent fallback: build it with ``python -m analysis_spec_b200.build``.
 """
 import ctypes
-import struct
 import threading
 from pathlib import Path
 
@@ -25,7 +24,6 @@ _i32 = ctypes.c_int32
 _pi64 = ctypes.POINTER(ctypes.c_int64)
 _pp = ctypes.POINTER(ctypes.c_void_p)
 _f32 = ctypes.c_float
-_b = ctypes.c_char_p  # packed int64 arrays (pack_i64): cheaper to build than a ctypes array
 
 # name -> argtypes (every function returns int status)
 SIGNATURES = {
@@ -69,9 +67,9 @@ SIGNATURES = {
     'speckv_acceptance_counts': [_p, _i64, _i64, _i64, _p, _p],
     'speckv_attention_set_ctas': [_i32],
     'speckv_attention_set_chunks': [_i32],
-    'speckv_paged_append': [_p, _p, _p, _p, _p, _p, _b, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _i64, _p, _p,
+    'speckv_paged_append': [_p, _p, _p, _p, _p, _p, _pi64, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _i64, _p, _p,
                             _i64, _i64, _i32, _i64, _i64, _i64, _i64, _i64, _i32, _p],
-    'speckv_paged_attention': [_p, _p, _p, _b, _p, _i64, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _i64, _f32,
+    'speckv_paged_attention': [_p, _p, _p, _pi64, _p, _i64, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _i64, _f32,
                                _i32, _p, _i64, _p],
     'speckv_paged_attention_workspace': [_i64, _i64, _i64, _i32],  # returns bytes, not a status
     'speckv_token_logprobs': [_p, _i32, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _f32,
@@ -115,6 +113,21 @@ def load():
             lib.speckv_plan_release.restype = None
             _lib = lib
     return _lib
+
+
+_front = None
+
+
+def front():
+    """The native torch front end of the decode-step operators (csrc/front.cpp)."""
+    global _front
+    if _front is None:
+        load()
+        if not LIB_PATH.with_name('_front.so').exists():
+            raise RuntimeError('_front.so is not built; run `python -m analysis_spec_b200.build`')
+        from . import _front as module
+        _front = module
+    return _front
 
 
 class SpecKVError(RuntimeError):
@@ -209,11 +222,6 @@ def prepare(name, *args):
 
 def ptr_array(values):
     return (ctypes.c_void_p * len(values))(*values)
-
-
-def pack_i64(*values):
-    """An int64 array argument as bytes."""
-    return struct.pack(f'{len(values)}q', *values)
 
 
 def i64_array(values):

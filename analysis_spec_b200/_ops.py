@@ -770,209 +770,36 @@ def mask_bits(mask, bits, first_col, nonbinary):
               first_col.data_ptr(), nonbinary.data_ptr(), _stream(mask))
 
 
-def _one_device(fn, first, *others):
-    """Device index of `first`; every other tensor (None is skipped) has to be there too."""
-    dev = first.get_device()
-    if dev < 0:
-        _require_cuda(first)
-    for t in others:
-        if t is not None and t.get_device() != dev:
-            _require_cuda(t)
-            raise ValueError(f'{fn}: tensors on cuda:{dev} and {t.device}')
-    return dev
-
-
-def _check_paged(fn, key_pages, value_pages, page_table, batch):
-    if key_pages.dim() != 4 or key_pages.shape != value_pages.shape or key_pages.dtype != value_pages.dtype:
-        raise ValueError(f'{fn}: key and value pages must be (pages, kv_heads, page_size, head_dim) of one dtype')
-    if key_pages.dtype not in _DTYPE_CODE:
-        raise ValueError(f'{fn}: unsupported dtype {key_pages.dtype}')
-    if key_pages.stride(3) != 1 or value_pages.stride(3) != 1:
-        raise ValueError(f'{fn}: pages need unit stride on head_dim')
-    if page_table.dtype != torch.long or page_table.dim() != 2 or page_table.shape[0] < batch or \
-            (page_table.stride(1) != 1 and page_table.shape[1] > 1):
-        raise ValueError(f'{fn}: page table must be an int64 (batch, pages) tensor with unit column stride')
-
-
-def _per_sequence(fn, name, t, batch):
-    if t.dtype != torch.long or t.dim() != 1 or t.shape[0] < batch or (t.stride(0) != 1 and batch > 1):
-        raise ValueError(f'{fn}: {name} must be a contiguous int64 tensor with an entry per sequence')
-
-
-@_on_device
-def paged_append(key, value, key_pages, value_pages, page_table, starts, counts=None, query=None, rotation=None,
-                 positions=None, interleaved=False, query_out=None):
-    """speckv_paged_append (see paged_cache.paged_append); returns the rotated queries."""
-    fn = 'paged_append'
-    cos, sin = rotation if rotation is not None else (None, None)
-    _one_device(fn, key, value, key_pages, value_pages, page_table, starts, counts, query, cos, sin, positions,
-                query_out)
-    if key.dim() != 4 or key.shape != value.shape:
-        raise ValueError(f'{fn}: key and value must be (batch, kv_heads, rows, head_dim) of one shape')
-    batch, kv_heads, rows, dim = key.shape
-    _check_paged(fn, key_pages, value_pages, page_table, batch)
-    dtype = key_pages.dtype
-    if key.dtype != dtype or value.dtype != dtype:
-        raise ValueError(f'{fn}: key / value dtype differs from the pages')
-    if key_pages.shape[1] != kv_heads or key_pages.shape[3] != dim:
-        raise ValueError(f'{fn}: key / value shape does not match the pages')
-    ks, vs = key.stride(), value.stride()
-    if ks[3] != 1 or vs[3] != 1:
-        raise ValueError(f'{fn}: key and value need unit stride on head_dim')
-    _per_sequence(fn, 'starts', starts, batch)
-    if counts is not None:
-        _per_sequence(fn, 'counts', counts, batch)
-    pos_b = pos_t = 0
-    if positions is not None:
-        if positions.dtype != torch.long or positions.dim() != 2 or positions.shape[0] < batch or \
-                positions.shape[1] < rows:
-            raise ValueError(f'{fn}: positions must be an int64 (batch, rows) tensor')
-        pos_b, pos_t = positions.stride()
-    rot_positions = rot = 0
-    if cos is not None:
-        if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or cos.shape != sin.shape or \
-                not cos.is_contiguous() or not sin.is_contiguous():
-            raise ValueError(f'{fn}: rotation must be a pair of contiguous float32 (positions, rotation_dim / 2) tables')
-        rot_positions, rot = cos.shape[0], 2 * cos.shape[1]
-        if rot < 2 or rot > dim or rot_positions < 1:
-            raise ValueError(f'{fn}: rotation of {rot} of {dim} dims over {rot_positions} positions')
-    q_heads, qs, os = 0, (0, 0, 0, 0), (0, 0, 0, 0)
-    if query is not None:
-        if query.dim() != 4 or query.shape[0] != batch or query.shape[2] != rows or query.shape[3] != dim or \
-                query.dtype != dtype:
-            raise ValueError(f'{fn}: query must be (batch, q_heads, rows, head_dim) of the pages\' dtype')
-        if query_out is None:
-            query_out = torch.empty_like(query)
-        q_heads, qs, os = query.shape[1], query.stride(), query_out.stride()
-        if query_out.shape != query.shape or query_out.dtype != dtype or qs[3] != 1 or os[3] != 1:
-            raise ValueError(f'{fn}: query and its output need one shape and dtype and unit stride on head_dim')
-    elif query_out is not None:
-        raise ValueError(f'{fn}: query_out without query')
-    if batch == 0 or rows == 0:
-        return query_out
-    kps, vps = key_pages.stride(), value_pages.stride()
-    _lib.call('speckv_paged_append', key.data_ptr(), value.data_ptr(), _ptr(query), _ptr(query_out),
-              key_pages.data_ptr(), value_pages.data_ptr(),
-              _lib.pack_i64(*ks[:3], *vs[:3], *qs[:3], *os[:3], *kps[:3], *vps[:3]), page_table.data_ptr(),
-              page_table.stride(0), page_table.shape[1], key_pages.shape[0], key_pages.shape[2], starts.data_ptr(),
-              _ptr(counts), _ptr(positions), pos_b, pos_t, _ptr(cos), _ptr(sin), rot_positions, rot,
-              1 if interleaved else 0, batch, q_heads, kv_heads, rows, dim, _DTYPE_CODE[dtype], _stream(key))
-    return query_out
-
-
-_PAGED_WORKSPACE = {}  # (device, q_heads, kv_heads, head_dim, dtype) -> bytes
-
-
-@_on_device
-def paged_attention(query, key_pages, value_pages, page_table, lengths, scale, out=None):
-    """speckv_paged_attention (see paged_cache.paged_attention)."""
-    fn = 'paged_attention'
-    _one_device(fn, query, key_pages, value_pages, page_table, lengths, out)
-    if query.dim() != 4 or query.shape[2] != 1:
-        raise ValueError(f'{fn}: query must be (batch, q_heads, 1, head_dim): one new token per sequence')
-    batch, q_heads, _, dim = query.shape
-    _check_paged(fn, key_pages, value_pages, page_table, batch)
-    dtype = query.dtype
-    if key_pages.dtype != dtype or key_pages.shape[3] != dim or q_heads % max(key_pages.shape[1], 1):
-        raise ValueError(f'{fn}: query dtype, head_dim or heads do not match the pages')
-    _per_sequence(fn, 'lengths', lengths, batch)
-    qs, ks, vs = query.stride(), key_pages.stride(), value_pages.stride()
-    if qs[3] != 1:
-        raise ValueError(f'{fn}: query needs unit stride on head_dim')
-    if out is None:
-        out = torch.empty((batch, 1, q_heads, dim), device=query.device, dtype=dtype)
-    elif out.shape != (batch, 1, q_heads, dim) or out.dtype != dtype or not out.is_contiguous():
-        raise ValueError(f'{fn}: out must be a contiguous (batch, 1, q_heads, head_dim) tensor of the query dtype')
-    if batch == 0:
-        return out
-    # a workspace of this call alone: other streams and captured graphs have their own
-    kv_heads, code = key_pages.shape[1], _DTYPE_CODE[dtype]
-    key = (query.get_device(), q_heads, kv_heads, dim, code)
-    need = _PAGED_WORKSPACE.get(key)
-    if need is None:
-        need = _PAGED_WORKSPACE[key] = _lib.load().speckv_paged_attention_workspace(q_heads, kv_heads, dim, code)
-    workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
-    _lib.call('speckv_paged_attention', query.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(),
-              _lib.pack_i64(qs[0], qs[1], *ks[:3], *vs[:3]), page_table.data_ptr(), page_table.stride(0),
-              page_table.shape[1], key_pages.shape[0], key_pages.shape[2], lengths.data_ptr(), out.data_ptr(), batch,
-              q_heads, kv_heads, dim, float(scale), code, _ptr(workspace), need, _stream(query))
+def _front(name, *args):
+    """A function of the native front end (_front.so), which checks its operands, makes their GPU
+    current and launches on its current stream; profiled under the entry point's name."""
+    profile = _lib.profile
+    profile.calls += 1
+    if not profile.enabled:
+        return getattr(_lib.front(), name)(*args)
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    out = getattr(_lib.front(), name)(*args)
+    end.record()
+    profile.events.setdefault('speckv_' + name, []).append((start, end))
     return out
 
 
-MAX_TOP = 32  # SPECKV_MAX_TOP
+def paged_append(key, value, key_pages, value_pages, page_table, starts, counts=None, query=None, rotation=None,
+                 positions=None, interleaved=False, query_out=None):
+    """speckv_paged_append (see paged_cache.paged_append); returns the rotated queries."""
+    cos, sin = (None, None) if rotation is None else rotation
+    return _front('paged_append', key, value, key_pages, value_pages, page_table, starts, counts, query, cos, sin,
+                  positions, interleaved, query_out)
 
 
-def _row_strides(t):
-    """(sequence, row) strides of a tensor whose leading dims are (), (rows,) or (batch, rows)."""
-    s = t.stride()
-    return (0, 0) if len(s) == 0 else (0, s[0]) if len(s) == 1 else s[:2]
+def paged_attention(query, key_pages, value_pages, page_table, lengths, scale, out=None):
+    """speckv_paged_attention (see paged_cache.paged_attention)."""
+    return _front('paged_attention', query, key_pages, value_pages, page_table, lengths, scale, out)
 
 
-def _score_operands(fn, logits, tokens, rows, top, temperature):
-    """((batch, rows per sequence, source rows), logits strides, token strides, row-index strides, output shape)."""
-    if logits.dtype not in _DTYPE_CODE:
-        raise ValueError(f'{fn}: unsupported dtype {logits.dtype}')
-    if not 1 <= logits.dim() <= 3 or logits.shape[-1] < 1 or (logits.stride(-1) != 1 and logits.shape[-1] > 1):
-        raise ValueError(f'{fn}: logits must be ([batch,] [rows,] vocabulary) with unit stride on the vocabulary')
-    if not 0 <= top <= min(MAX_TOP, logits.shape[-1]):
-        raise ValueError(f'{fn}: {top} alternatives of {logits.shape[-1]} (at most {MAX_TOP})')
-    if not 1e-29 <= temperature <= 1e29:
-        raise ValueError(f'{fn}: temperature must be positive and finite (1e-29 to 1e29), got {temperature}')
-    lead = logits.shape[:-1]
-    batch, source = (1, 1) if len(lead) == 0 else (1, lead[0]) if len(lead) == 1 else lead
-    shape = lead
-    if rows is not None:
-        if len(lead) != 2 or rows.dim() != 2 or rows.dtype != torch.long or rows.shape[0] != batch:
-            raise ValueError(f'{fn}: rows must be an int64 (batch, n) tensor beside (batch, rows, vocabulary) logits')
-        shape = rows.shape
-    if tokens is not None and (tokens.dtype != torch.long or tokens.shape != shape):
-        raise ValueError(f'{fn}: tokens must be int64 of shape {tuple(shape)}, got {tuple(tokens.shape)}')
-    per = source if rows is None else rows.shape[1]
-    return ((batch, per, source), _row_strides(logits[..., 0]), (0, 0) if tokens is None else _row_strides(tokens),
-            (0, 0) if rows is None else rows.stride(), shape)
-
-
-@_on_device
 def token_logprobs(logits, tokens=None, rows=None, top=0, temperature=1.0):
-    """speckv_token_logprobs: (logprobs or None, entropy, stats, top_logprobs or None, top_ids or None)."""
-    fn = 'token_logprobs'
-    _one_device(fn, logits, tokens, rows)
-    (batch, per, source), ls, ts, rs, shape = _score_operands(fn, logits, tokens, rows, top, temperature)
-    entropy = torch.empty(shape, device=logits.device, dtype=torch.float32)
-    stats = torch.empty((*shape, 2), device=logits.device, dtype=torch.float32)
-    logprobs = torch.empty_like(entropy) if tokens is not None else None
-    top_logprobs = top_ids = None
-    if top:
-        top_logprobs = torch.empty((*shape, top), device=logits.device, dtype=torch.float32)
-        top_ids = torch.empty((*shape, top), device=logits.device, dtype=torch.long)
-    _lib.call('speckv_token_logprobs', logits.data_ptr(), _DTYPE_CODE[logits.dtype], ls[0], ls[1], _ptr(tokens), ts[0],
-              ts[1], _ptr(rows), rs[0], rs[1], batch, per, source, logits.shape[-1], 1.0 / temperature, top,
-              _ptr(logprobs), entropy.data_ptr(), stats.data_ptr(), _ptr(top_logprobs), _ptr(top_ids), _stream(logits))
-    return logprobs, entropy, stats, top_logprobs, top_ids
-
-
-@_on_device
-def token_logprobs_backward(logits, tokens, entropy, stats, top_ids, temperature, grad_logprobs=None, grad_entropy=None,
-                            grad_top_logprobs=None):
-    """speckv_token_logprobs_backward: the gradient with respect to the logits (contiguous)."""
-    fn = 'token_logprobs_backward'
-    top = top_ids.shape[-1] if top_ids is not None else 0
-    (batch, per, _), ls, ts, _, shape = _score_operands(fn, logits, tokens, None, top, temperature)
-    grads = []
-    for name, g, want in (('logprobs', grad_logprobs, shape), ('entropy', grad_entropy, shape),
-                          ('top_logprobs', grad_top_logprobs, (*shape, top))):
-        if g is not None:
-            if g.dtype != torch.float32 or tuple(g.shape) != tuple(want):
-                raise ValueError(f'{fn}: gradient of {name} must be float32 of shape {tuple(want)}')
-            g = g.contiguous()
-        grads.append(g)
-    for t in (entropy, stats, top_ids):
-        if t is not None and not t.is_contiguous():
-            raise ValueError(f'{fn}: entropy, stats and top_ids are the forward\'s contiguous outputs')
-    _one_device(fn, logits, tokens, entropy, stats, top_ids, *grads)
-    grad = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
-    _lib.call('speckv_token_logprobs_backward', logits.data_ptr(), _DTYPE_CODE[logits.dtype], ls[0], ls[1],
-              _ptr(tokens), ts[0], ts[1], batch, per, logits.shape[-1], 1.0 / temperature, top, entropy.data_ptr(),
-              stats.data_ptr(), _ptr(top_ids), _ptr(grads[0]), _ptr(grads[1]), _ptr(grads[2]), grad.data_ptr(),
-              _stream(logits))
-    return grad
+    """speckv_token_logprobs (see token_logprobs.token_logprobs): (logprobs or None, entropy,
+    top_logprobs or None, top_ids or None); with a gradient to logits that require one
+    (speckv_token_logprobs_backward, launched by autograd and not profiled)."""
+    return _front('token_logprobs', logits, tokens, rows, top, temperature)

@@ -1,6 +1,7 @@
-"""Builds libspeckv.so (all CUDA sources under csrc/) for sm_100a with nvcc.
+"""Builds libspeckv.so (all CUDA sources under csrc/) for sm_100a with nvcc, and the CPython
+module _front.so (csrc/front.cpp, the torch front end of the decode-step operators) with g++.
 
-The library is built in-tree next to this file so that it ships with the
+Both are built in-tree next to this file so that they ship with the
 package. A rebuild happens only when a source, header or flag changed (a hash
 of them is kept beside the library).
 """
@@ -15,8 +16,10 @@ HERE = Path(__file__).resolve().parent
 CSRC = HERE / 'csrc'
 INCLUDE = HERE.parent / 'include'
 LIB = HERE / 'libspeckv.so'
+FRONT = HERE / '_front.so'
 OBJDIR = HERE / '_build'
 
+CXX = os.environ.get('CXX', 'g++')
 NVCC = os.environ.get('NVCC', '/usr/local/cuda/bin/nvcc')
 ARCH = ['-gencode', 'arch=compute_100a,code=sm_100a']
 FLAGS = ['-O3', '-std=c++17', '-lineinfo', '-Xcompiler', '-fPIC', '-Xcompiler', '-O2',
@@ -30,7 +33,7 @@ def _sources():
 def _digest():
     h = hashlib.sha256()
     h.update(' '.join(ARCH + FLAGS).encode())
-    for path in sorted(list(CSRC.glob('*')) + list(INCLUDE.glob('*.h'))):
+    for path in sorted([p for p in CSRC.glob('*') if p.suffix != '.cpp'] + list(INCLUDE.glob('*.h'))):
         if path.is_file():
             h.update(path.name.encode())
             h.update(path.read_bytes())
@@ -38,10 +41,11 @@ def _digest():
 
 
 def build(force=False, verbose=False):
-    """Compile and link libspeckv.so; returns its path."""
+    """Compile and link libspeckv.so and _front.so; returns the library's path."""
     stamp = LIB.with_suffix('.so.hash')
     digest = _digest()
     if not force and LIB.exists() and stamp.exists() and stamp.read_text() == digest:
+        build_front(force, verbose)
         return LIB
     OBJDIR.mkdir(exist_ok=True)
 
@@ -64,8 +68,40 @@ def build(force=False, verbose=False):
         raise RuntimeError(f'nvcc link failed:\n{proc.stdout}\n{proc.stderr}')
     os.replace(tmp, LIB)
     stamp.write_text(digest)
+    build_front(force, verbose)
     return LIB
+
+
+def build_front(force=False, verbose=False):
+    """Compile and link _front.so against the installed torch and libspeckv.so; returns its path."""
+    import sysconfig
+
+    import torch
+    include = Path(torch.__file__).resolve().parent / 'include'
+    libdir = Path(torch.__file__).resolve().parent / 'lib'
+    src = CSRC / 'front.cpp'
+    cmd = [CXX, '-std=c++17', '-O2', '-fPIC', '-shared', '-fvisibility=hidden', '-DTORCH_API_INCLUDE_EXTENSION_H',
+           f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}', '-isystem', str(include), '-isystem',
+           str(include / 'torch' / 'csrc' / 'api' / 'include'), '-isystem', str(Path(NVCC).parent.parent / 'include'),
+           '-isystem', sysconfig.get_paths()['include'], str(src), '-o', str(FRONT.with_suffix('.so.tmp')),
+           f'-L{libdir}', '-lc10', '-lc10_cuda', '-ltorch_cpu', '-ltorch', '-ltorch_python', f'-L{HERE}',
+           f'-l:{LIB.name}', '-Wl,-rpath,$ORIGIN']
+    h = hashlib.sha256(' '.join(cmd + [torch.__version__]).encode())
+    for path in (src, INCLUDE / 'speckv.h'):
+        h.update(path.read_bytes())
+    stamp = FRONT.with_suffix('.so.hash')
+    if not force and FRONT.exists() and stamp.exists() and stamp.read_text() == h.hexdigest():
+        return FRONT
+    if verbose:
+        print(' '.join(cmd), file=sys.stderr)
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f'{CXX} failed on {src.name}:\n{proc.stdout}\n{proc.stderr}')
+    os.replace(FRONT.with_suffix('.so.tmp'), FRONT)
+    stamp.write_text(h.hexdigest())
+    return FRONT
 
 
 if __name__ == '__main__':
     print(build(force='--force' in sys.argv, verbose='-v' in sys.argv))
+

@@ -20,27 +20,6 @@ class TokenLogprobs(NamedTuple):
     top_ids: Optional[torch.Tensor]       # int64 (..., top), best first, equal logits by the lower id
 
 
-class _TokenLogprobs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tokens, top, temperature):
-        logprobs, entropy, stats, top_logprobs, top_ids = _ops.token_logprobs(logits, tokens, None, top, temperature)
-        ctx.save_for_backward(logits, tokens, entropy, stats, top_ids)
-        ctx.temperature = temperature
-        ctx.set_materialize_grads(False)
-        if top_ids is not None:
-            ctx.mark_non_differentiable(top_ids)
-        return logprobs, entropy, top_logprobs, top_ids
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_logprobs, grad_entropy, grad_top_logprobs, _):
-        logits, tokens, entropy, stats, top_ids = ctx.saved_tensors
-        if grad_logprobs is None and grad_entropy is None and grad_top_logprobs is None:
-            return None, None, None, None
-        return _ops.token_logprobs_backward(logits, tokens, entropy, stats, top_ids, ctx.temperature, grad_logprobs,
-                                            grad_entropy, grad_top_logprobs), None, None, None
-
-
 def token_logprobs(logits, tokens=None, *, rows=None, top=0, temperature=1.0):
     """Log-probability of each row's token under softmax(logits / temperature), the row's entropy
     and its `top` (at most 32) likeliest entries.
@@ -53,11 +32,4 @@ def token_logprobs(logits, tokens=None, *, rows=None, top=0, temperature=1.0):
     A row of -inf alone has log-probability -inf and entropy 0; NaN or +inf in a row makes its
     numbers NaN. The outputs carry a gradient to ``logits`` (not twice differentiable).
     """
-    temperature = float(temperature)
-    if logits.requires_grad and torch.is_grad_enabled():
-        if rows is not None:
-            raise ValueError('token_logprobs: rows selects verified rows of a rollout and carries no gradient; '
-                             'detach the logits or index them first')
-        return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, top, temperature))
-    logprobs, entropy, _, top_logprobs, top_ids = _ops.token_logprobs(logits, tokens, rows, top, temperature)
-    return TokenLogprobs(logprobs, entropy, top_logprobs, top_ids)
+    return TokenLogprobs(*_ops.token_logprobs(logits, tokens, rows, top, temperature))

@@ -16,7 +16,7 @@ def lib():
     return _lib.load()
 
 
-S18, S8, P = _lib.pack_i64(*[0] * 18), _lib.pack_i64(*[0] * 8), 16  # pointers that are never followed
+S18, S8, P = _lib.i64_array([0] * 18), _lib.i64_array([0] * 8), 16  # pointers that are never followed
 
 
 def test_append_refuses_on_the_host(lib):
@@ -85,25 +85,61 @@ def test_front_end_refuses_cpu_tensors():
 
 
 def test_score_operands_are_checked():
+    """Shapes, dtypes and ranges are refused before the device is looked at."""
     x, t = torch.zeros(3, 7), torch.zeros(3, dtype=torch.long)
-
-    def check(logits=x, tokens=t, rows=None, top=0, temperature=1.0):
-        return _ops._score_operands('token_logprobs', logits, tokens, rows, top, temperature)
     for match, kw in (('dtype', dict(logits=x.double())), ('unit stride', dict(logits=torch.zeros(7, 3).T)),
-                      ('vocabulary', dict(logits=torch.zeros(1, 1, 3, 7))), ('alternatives', dict(top=8)),
-                      ('alternatives', dict(top=-1)), ('temperature', dict(temperature=0.0)),
-                      ('temperature', dict(temperature=-1.0)), ('temperature', dict(temperature=float('nan'))),
-                      ('temperature', dict(temperature=float('inf'))), ('tokens', dict(tokens=t[:2])),
-                      ('tokens', dict(tokens=t.int())), ('rows', dict(rows=t[None])),
-                      ('rows', dict(logits=x[None], rows=t))):
+                      ('vocabulary', dict(logits=torch.zeros(1, 1, 3, 7))), ('vocabulary', dict(logits=x[0, 0])),
+                      ('alternatives', dict(top=8)), ('alternatives', dict(top=-1)),
+                      ('temperature', dict(temperature=0.0)), ('temperature', dict(temperature=-1.0)),
+                      ('temperature', dict(temperature=float('nan'))), ('temperature', dict(temperature=float('inf'))),
+                      ('tokens', dict(tokens=t[:2])), ('tokens', dict(tokens=t.int())), ('rows', dict(rows=t[None])),
+                      ('rows', dict(logits=x[None], rows=t)), ('tokens', dict(logits=x[None], rows=t[None])),
+                      ('carries no gradient', dict(logits=torch.zeros(1, 3, 7, requires_grad=True), rows=t[None],
+                                                   tokens=t[None]))):
         with pytest.raises(ValueError, match=match):
-            check(**kw)
-    (batch, per, source), ls, ts, rs, shape = check(torch.zeros(2, 3, 7), torch.zeros(2, 5, dtype=torch.long),
-                                                    torch.zeros(2, 5, dtype=torch.long))
-    assert (batch, per, source, ls, ts, rs, tuple(shape)) == (2, 5, 3, (21, 7), (5, 1), (5, 1), (2, 5))
-    assert check()[1] == (0, 7) and check(x[0], t[0])[0] == (1, 1, 1)
-    with pytest.raises(ValueError, match='carries no gradient'):
-        token_logprobs(torch.zeros(1, 3, 7, requires_grad=True), rows=torch.zeros(1, 2, dtype=torch.long))
+            token_logprobs(**{'logits': x, 'tokens': t, **kw})
+
+
+def test_paged_operands_are_checked():
+    bf = torch.bfloat16
+    good = dict(key=torch.zeros(2, 2, 3, 64, dtype=bf), value=torch.zeros(2, 2, 3, 64, dtype=bf),
+                key_pages=torch.zeros(4, 2, 16, 64, dtype=bf), value_pages=torch.zeros(4, 2, 16, 64, dtype=bf),
+                page_table=torch.zeros(2, 2, dtype=torch.long), starts=torch.zeros(2, dtype=torch.long))
+    with pytest.raises(RuntimeError, match='no CPU path'):
+        paged_append(**good)
+    q, n = torch.zeros(2, 4, 3, 64, dtype=bf), torch.zeros(2, dtype=torch.long)
+    half = torch.zeros(8, 32)
+    for match, kw in (('one shape', dict(value=good['value'][:1])), ('dtype differs', dict(key=good['key'].half())),
+                      ('dtype', dict(key=good['key'].double(), value=good['value'].double(),
+                                     key_pages=good['key_pages'].double(), value_pages=good['value_pages'].double())),
+                      ('one dtype', dict(value_pages=good['value_pages'].half())),
+                      ('match the pages', dict(key_pages=good['key_pages'][:, :1], value_pages=good['value_pages'][:, :1])),
+                      ('unit stride', dict(key=torch.zeros(2, 2, 64, 3, dtype=bf).transpose(2, 3))),
+                      ('unit stride', dict(key_pages=torch.zeros(4, 2, 64, 16, dtype=bf).transpose(2, 3))),
+                      ('page table', dict(page_table=n[:, None].int())), ('page table', dict(page_table=n[:1, None])),
+                      ('page table', dict(page_table=torch.zeros(2, 2, dtype=torch.long).T)),
+                      ('starts', dict(starts=n[:1])), ('starts', dict(starts=n.int())), ('counts', dict(counts=n[:1])),
+                      ('positions', dict(positions=n[:, None])), ('positions', dict(positions=torch.zeros(2, 3))),
+                      ('rotation', dict(rotation=(half, half[:4]))), ('rotation', dict(rotation=(half.half(), half.half()))),
+                      ('rotation', dict(rotation=(half.T, half.T))), ('rotation', dict(rotation=(half, None))),
+                      ('rotation of 66', dict(rotation=(torch.zeros(8, 33),) * 2)),
+                      ('rotation of 64', dict(rotation=(half[:0], half[:0]))),
+                      ('query must', dict(query=q[:, :, :2])), ('query must', dict(query=q.half())),
+                      ('one shape and dtype', dict(query=q, query_out=q[:, :2])),
+                      ('without query', dict(query_out=q))):
+        with pytest.raises(ValueError, match=match):
+            paged_append(**{**good, **kw})
+    good = dict(query=q[:, :, :1], key_pages=good['key_pages'], value_pages=good['value_pages'],
+                page_table=good['page_table'], lengths=n)
+    with pytest.raises(RuntimeError, match='no CPU path'):
+        paged_attention(**good)
+    for match, kw in (('one new token', dict(query=q)), ('match the pages', dict(query=q[:, :3, :1])),
+                      ('match the pages', dict(query=q[:, :, :1, :32])), ('match the pages', dict(query=q[:, :, :1].half())),
+                      ('lengths', dict(lengths=n[:1])), ('out must', dict(out=q[:, :, :1])),
+                      ('out must', dict(out=torch.zeros(2, 1, 4, 64))),
+                      ('unit stride', dict(query=torch.zeros(2, 4, 64, 2, dtype=bf).transpose(2, 3)[:, :, :1]))):
+        with pytest.raises(ValueError, match=match):
+            paged_attention(**{**good, **kw})
 
 
 def test_page_bookkeeping(monkeypatch):

@@ -347,6 +347,23 @@ def test_gradient_layouts_streams_and_graphs():
         assert (out - want).abs().max() <= 4e-5 * want.abs().max()
 
 
+def test_twice_differentiated_is_refused():
+    x = torch.randn(2, 30, device='cuda', requires_grad=True)
+    r = token_logprobs(x, torch.tensor([1, 2], device='cuda'))
+    grad, = torch.autograd.grad(r.logprobs.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match='not twice differentiable'):
+        torch.autograd.grad(grad.square().sum(), x)
+    r = token_logprobs(x, torch.tensor([1, 2], device='cuda'), top=3)
+    assert r.top_ids.grad_fn is None and not r.top_ids.requires_grad and r.top_logprobs.requires_grad
+    with torch.no_grad():
+        assert not token_logprobs(x, top=1).entropy.requires_grad
+    y = x * 1.0
+    r = token_logprobs(y, torch.tensor([1, 2], device='cuda'))
+    y.add_(1.0)  # the saved logits changed
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        r.entropy.sum().backward()
+
+
 def test_rows_beyond_32_bit_offsets():
     x = torch.zeros(15000, 151644, device='cuda', dtype=torch.bfloat16)  # 2.27e9 entries
     x[14999, 151640] = 9.0

@@ -117,9 +117,135 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_scalar_kernel(App
   }
 }
 
+// 16 bytes of rows: N elements.
+template <typename T> struct Pack {
+  static constexpr int N = 16 / sizeof(T);
+  union {
+    uint4 raw;
+    T e[N];
+  };
+};
+
+// x' = x c - y s, y' = y c + x s of the pairs of two 16-byte pieces of a row: element i of one with
+// element i of the other, or neighbours within each.
+template <typename T, bool INTERLEAVED>
+__device__ __forceinline__ void rotate(Pack<T>& x, Pack<T>& y, const float (&c)[Pack<T>::N],
+                                       const float (&s)[Pack<T>::N]) {
+  constexpr int N = Pack<T>::N;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    T& first = INTERLEAVED ? (i < N / 2 ? x.e[2 * i] : y.e[2 * i - N]) : x.e[i];
+    T& second = INTERLEAVED ? (i < N / 2 ? x.e[2 * i + 1] : y.e[2 * i - N + 1]) : y.e[i];
+    const float u = load_f<T>(first), v = load_f<T>(second);
+    first = store_f<T>(u * c[i] - v * s[i]);
+    second = store_f<T>(v * c[i] + u * s[i]);
+  }
+}
+
+// CTA per token. A thread keeps one slice of the token's cos / sin row in registers and turns that
+// pair of 16-byte pieces in kHeads heads at a time, all loaded before the first is stored; then the
+// pieces that are copied. Needs 16-byte aligned rows and rotation_dim / 2 a multiple of 16 bytes.
+constexpr int kHeads = 4;
+
+template <typename T, bool INTERLEAVED>
+__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(AppendArgs a) {
+  constexpr int N = Pack<T>::N;
+  const uint32_t b = blockIdx.x / (uint32_t)a.rows, t = blockIdx.x - b * (uint32_t)a.rows;
+  const Place p = place_token(a, b, t);
+  const int q_heads = a.query != nullptr ? (int)a.q_heads : 0, kv_heads = (int)a.kv_heads, dim = (int)a.dim;
+  const T* q = static_cast<const T*>(a.query) + b * a.qs[0] + t * a.qs[2];
+  T* qo = static_cast<T*>(a.query_out) + b * a.os[0] + t * a.os[2];
+  if (p.page < 0) {  // padding: its queries are zeros
+    const int pieces = dim / N;
+    for (int i = threadIdx.x; i < q_heads * pieces; i += kAppendThreads)
+      *reinterpret_cast<uint4*>(qo + (i / pieces) * a.os[1] + (i % pieces) * N) = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const T* k = static_cast<const T*>(a.key) + b * a.ks[0] + t * a.ks[2];
+  const T* v = static_cast<const T*>(a.value) + b * a.vs[0] + t * a.vs[2];
+  T* kp = static_cast<T*>(a.key_pages) + p.page * a.kps[0] + p.row * a.kps[2];
+  T* vp = static_cast<T*>(a.value_pages) + p.page * a.vps[0] + p.row * a.vps[2];
+
+  const int half = a.rot / 2, slices = half / N;  // slices <= 128
+  if (slices > 0) {
+    const int slice = threadIdx.x % slices, h0 = threadIdx.x / slices, step = kAppendThreads / slices;
+    if (h0 < step) {
+      const int x = INTERLEAVED ? 2 * slice * N : slice * N, y = INTERLEAVED ? x + N : x + half;
+      float c[N], s[N];
+      const float4* cr = reinterpret_cast<const float4*>(a.cos + p.position * half + slice * N);
+      const float4* sr = reinterpret_cast<const float4*>(a.sin + p.position * half + slice * N);
+#pragma unroll
+      for (int i = 0; i < N / 4; ++i) {
+        const float4 cc = __ldg(cr + i), ss = __ldg(sr + i);
+        c[4 * i] = cc.x, c[4 * i + 1] = cc.y, c[4 * i + 2] = cc.z, c[4 * i + 3] = cc.w;
+        s[4 * i] = ss.x, s[4 * i + 1] = ss.y, s[4 * i + 2] = ss.z, s[4 * i + 3] = ss.w;
+      }
+      const int heads = q_heads + kv_heads;
+      for (int h = h0; h < heads; h += kHeads * step) {
+        Pack<T> px[kHeads], py[kHeads];
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) {
+          const int hi = h + i * step;
+          if (hi < heads) {
+            const T* row = hi < q_heads ? q + hi * a.qs[1] : k + (hi - q_heads) * a.ks[1];
+            px[i].raw = *reinterpret_cast<const uint4*>(row + x);
+            py[i].raw = *reinterpret_cast<const uint4*>(row + y);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) {
+          const int hi = h + i * step;
+          if (hi < heads) {
+            T* row = hi < q_heads ? qo + hi * a.os[1] : kp + (hi - q_heads) * a.kps[1];
+            rotate<T, INTERLEAVED>(px[i], py[i], c, s);
+            *reinterpret_cast<uint4*>(row + x) = px[i].raw;
+            *reinterpret_cast<uint4*>(row + y) = py[i].raw;
+          }
+        }
+      }
+    }
+  }
+  // V, then what lies past the rotation in K and Q
+  const int whole = dim / N, rest = (dim - a.rot) / N;
+  const int v_items = kv_heads * whole, items = v_items + (rest > 0 ? (q_heads + kv_heads) * rest : 0);
+  for (int i = threadIdx.x; i < items; i += kAppendThreads) {
+    const T* from;
+    T* to;
+    if (i < v_items) {
+      const int h = i / whole, e = (i - h * whole) * N;
+      from = v + h * a.vs[1] + e;
+      to = vp + h * a.vps[1] + e;
+    } else {
+      const int j = i - v_items, h = j / rest, e = a.rot + (j - h * rest) * N;
+      from = h < q_heads ? q + h * a.qs[1] + e : k + (h - q_heads) * a.ks[1] + e;
+      to = h < q_heads ? qo + h * a.os[1] + e : kp + (h - q_heads) * a.kps[1] + e;
+    }
+    *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
+  }
+}
+
+// Whether every row begins on a 16-byte boundary and the rotation splits into whole pieces.
+template <typename T> bool in_pieces(const AppendArgs& a) {
+  const int64_t n = 16 / sizeof(T);
+  bool ok = a.dim % n == 0 && a.rot / 2 % n == 0 && a.rot / 2 / n <= kAppendThreads;
+  for (const void* p : {a.key, a.value, a.query, (const void*)a.query_out, (const void*)a.key_pages,
+                        (const void*)a.value_pages, (const void*)a.cos, (const void*)a.sin})
+    ok = ok && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+  for (int i = 0; i < 3; ++i)
+    ok = ok && a.ks[i] % n == 0 && a.vs[i] % n == 0 && a.qs[i] % n == 0 && a.os[i] % n == 0 && a.kps[i] % n == 0 &&
+         a.vps[i] % n == 0;
+  return ok;
+}
+
 template <typename T>
 int launch_append(const AppendArgs& a, cudaStream_t s) {
-  paged_append_scalar_kernel<T><<<(unsigned)(a.batch * a.rows), kAppendThreads, 0, s>>>(a);
+  const unsigned tokens = (unsigned)(a.batch * a.rows);
+  if (!in_pieces<T>(a))
+    paged_append_scalar_kernel<T><<<tokens, kAppendThreads, 0, s>>>(a);
+  else if (a.interleaved)
+    paged_append_kernel<T, true><<<tokens, kAppendThreads, 0, s>>>(a);
+  else
+    paged_append_kernel<T, false><<<tokens, kAppendThreads, 0, s>>>(a);
   return check_launch("speckv_paged_append");
 }
 

@@ -89,98 +89,6 @@ __device__ __forceinline__ float max_nan(float x, float y) {
   return z;
 }
 
-// 16 bytes of logits: their values, and their maximum (NaN when one is).
-template <typename T> struct Vector;
-template <> struct Vector<float> {
-  static constexpr int N = 4;
-  static __device__ __forceinline__ void values(const uint4& v, float (&x)[4]) {
-    x[0] = __uint_as_float(v.x);
-    x[1] = __uint_as_float(v.y);
-    x[2] = __uint_as_float(v.z);
-    x[3] = __uint_as_float(v.w);
-  }
-  static __device__ __forceinline__ float top(const uint4& v) {
-    return max_nan(max_nan(__uint_as_float(v.x), __uint_as_float(v.y)),
-                   max_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
-  }
-  static __device__ __forceinline__ uint4 pack(const float (&x)[4]) {
-    return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
-  }
-};
-template <> struct Vector<__nv_bfloat16> {
-  static constexpr int N = 8;
-  static __device__ __forceinline__ __nv_bfloat162 pair(uint32_t u) { return *reinterpret_cast<__nv_bfloat162*>(&u); }
-  static __device__ __forceinline__ void values(const uint4& v, float (&x)[8]) {
-    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {  // a bf16 is the upper half of an fp32
-      x[2 * i] = __uint_as_float(u[i] << 16);
-      x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-    }
-  }
-  static __device__ __forceinline__ float top(const uint4& v) {
-    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(pair(v.x), pair(v.y)), __hmax2_nan(pair(v.z), pair(v.w)));
-    return max_nan(__low2float(m), __high2float(m));
-  }
-  static __device__ __forceinline__ uint4 pack(const float (&x)[8]) {
-    uint4 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-      (&r.x)[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    return r;
-  }
-};
-template <> struct Vector<__half> {
-  static constexpr int N = 8;
-  static __device__ __forceinline__ __half2 pair(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
-  static __device__ __forceinline__ void values(const uint4& v, float (&x)[8]) {
-    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(pair(u[i]));
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
-    }
-  }
-  static __device__ __forceinline__ float top(const uint4& v) {
-    const __half2 m = __hmax2_nan(__hmax2_nan(pair(v.x), pair(v.y)), __hmax2_nan(pair(v.z), pair(v.w)));
-    return max_nan(__low2float(m), __high2float(m));
-  }
-  static __device__ __forceinline__ uint4 pack(const float (&x)[8]) {
-    uint4 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-      (&r.x)[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    return r;
-  }
-};
-
-__device__ __forceinline__ uint4 load_stream(const void* p) {
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-               : "l"(p));
-  return r;
-}
-
-// A row as single entries up to the first 16-byte boundary, 16-byte vectors, and single entries.
-struct RowSplit {
-  int head, vectors, tail;  // entries, vectors, entries
-  __device__ __forceinline__ RowSplit(const void* row, int vocab, int size) {
-    const int n = 16 / size;
-    head = min(vocab, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / size);
-    vectors = (vocab - head) / n;
-    tail = vocab - head - vectors * n;
-  }
-};
-
-constexpr float kEmpty = -150.f;   // 2^-150 is 0 in fp32: where distances to the reference end
-constexpr float kSlack = 10.f;     // a distance may pass the reference by 2^10 before it moves
-
 // Two fp32 numbers in one register pair, as the packed fp32 instructions take them.
 typedef unsigned long long Two;
 __device__ __forceinline__ Two two(float x, float y) {
@@ -205,43 +113,203 @@ __device__ __forceinline__ Two fma2(Two x, Two y, Two z) {
   return r;
 }
 
+// 32 bytes of logits, one load.
+struct Bytes32 {
+  uint32_t w[8];
+};
+__device__ __forceinline__ Bytes32 load_stream(const void* p) {
+  Bytes32 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]),
+                 "=r"(r.w[7])
+               : "l"(p));
+  return r;
+}
+__device__ __forceinline__ void store_stream(void* p, const Bytes32& v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v.w[0]), "r"(v.w[1]),
+               "r"(v.w[2]), "r"(v.w[3]), "r"(v.w[4]), "r"(v.w[5]), "r"(v.w[6]), "r"(v.w[7])
+               : "memory");
+}
+
+// The logits of one 32-bit word, their largest (NaN when one is), and what the fast sums take
+// for them: kLow stands for anything lower, so that -inf has a weight of 0 and a finite distance.
+template <typename T> struct Word;
+template <> struct Word<float> {
+  static constexpr int N = 1;
+  static constexpr float kLow = -INFINITY;  // the distance is cut instead
+  static __device__ __forceinline__ uint32_t top(uint32_t x, uint32_t y) {
+    return __float_as_uint(max_nan(__uint_as_float(x), __uint_as_float(y)));
+  }
+  static __device__ __forceinline__ float largest(uint32_t x) { return __uint_as_float(x); }
+  static __device__ __forceinline__ uint32_t cut(uint32_t x) { return x; }
+};
+template <> struct Word<__nv_bfloat16> {
+  static constexpr int N = 2;
+  static constexpr float kLow = -1e30f;
+  static __device__ __forceinline__ __nv_bfloat162 pair(uint32_t u) { return *reinterpret_cast<__nv_bfloat162*>(&u); }
+  static __device__ __forceinline__ uint32_t bits(__nv_bfloat162 h) { return *reinterpret_cast<uint32_t*>(&h); }
+  static __device__ __forceinline__ uint32_t top(uint32_t x, uint32_t y) { return bits(__hmax2_nan(pair(x), pair(y))); }
+  static __device__ __forceinline__ void values(uint32_t u, float& x, float& y) {  // the upper half of an fp32
+    x = __uint_as_float(u << 16);
+    y = __uint_as_float(u & 0xffff0000u);
+  }
+  static __device__ __forceinline__ float largest(uint32_t u) {
+    float x, y;
+    values(u, x, y);
+    return max_nan(x, y);
+  }
+  static __device__ __forceinline__ uint32_t cut(uint32_t u) {
+    return bits(__hmax2(pair(u), pair(0xf149f149u)));  // -9.97e29
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) { return bits(__floats2bfloat162_rn(x, y)); }
+};
+template <> struct Word<__half> {
+  static constexpr int N = 2;
+  static constexpr float kLow = -65504.f;
+  static __device__ __forceinline__ __half2 pair(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+  static __device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+  static __device__ __forceinline__ uint32_t top(uint32_t x, uint32_t y) { return bits(__hmax2_nan(pair(x), pair(y))); }
+  static __device__ __forceinline__ void values(uint32_t u, float& x, float& y) {
+    const float2 f = __half22float2(pair(u));
+    x = f.x;
+    y = f.y;
+  }
+  static __device__ __forceinline__ float largest(uint32_t u) {
+    float x, y;
+    values(u, x, y);
+    return max_nan(x, y);
+  }
+  static __device__ __forceinline__ uint32_t cut(uint32_t u) {
+    return bits(__hmax2(pair(u), pair(0xfbfffbffu)));
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) { return bits(__floats2half2_rn(x, y)); }
+};
+
+// Two neighbouring logits of a vector (fp32: words 2 i and 2 i + 1; else word i).
+template <typename T> __device__ __forceinline__ void pair_values(const Bytes32& v, int i, bool cut, float& x, float& y) {
+  if constexpr (Word<T>::N == 1) {
+    x = __uint_as_float(v.w[2 * i]);
+    y = __uint_as_float(v.w[2 * i + 1]);
+  } else {
+    Word<T>::values(cut ? Word<T>::cut(v.w[i]) : v.w[i], x, y);
+  }
+}
+template <typename T> __device__ __forceinline__ float vector_top(const Bytes32& v) {
+  typedef Word<T> W;
+  return W::largest(W::top(W::top(W::top(v.w[0], v.w[1]), W::top(v.w[2], v.w[3])),
+                           W::top(W::top(v.w[4], v.w[5]), W::top(v.w[6], v.w[7]))));
+}
+
+// A row as single entries up to the first 32-byte boundary, 32-byte vectors, and single entries.
+struct RowSplit {
+  int head, vectors, tail;  // entries, vectors, entries
+  __device__ __forceinline__ RowSplit(const void* row, int vocab, int size) {
+    const int n = 32 / size;
+    head = min(vocab, (int)((32 - (reinterpret_cast<uintptr_t>(row) & 31)) & 31) / size);
+    vectors = (vocab - head) / n;
+    tail = vocab - head - vectors * n;
+  }
+};
+
+constexpr float kEmpty = -150.f;   // 2^-150 is 0 in fp32: where distances to the reference end
+constexpr float kSlack = 10.f;     // a distance may pass the reference by 2^10 before it moves
+constexpr float kWide = 1048576.f; // references to 2^20 take the fused product
+
 // Sums of a thread over its entries, by a reference r (one of its entries) that stays within
-// 2^kSlack of their maximum: y = (x - r) log2(e) / T, s = sum 2^y, t = sum 2^y y. The difference is
-// taken before the product, so that logits of any size (a mask's lowest value among them) keep
-// their distances. best / at: the largest entry and the first entry of the vector that holds it.
-struct Running {
-  float r = -INFINITY, limit = -INFINITY, best = -INFINITY;
+// 2^kSlack of their maximum: y = (x - r) c, c = log2(e) / T, s = sum 2^y, t = sum 2^y y.
+// y is one fused product x c - rc with rc = r c rounded; what that rounding left out is put back once
+// at the end. References whose product is so large that the rounding would matter before that
+// (a row of a mask's lowest value, say) take the difference first, vector by vector (wide).
+// best / at: the largest entry of the current run of vectors and the first entry of its vector.
+template <typename T> struct Running {
+  float r = -INFINITY, rc = 0.f, limit = -INFINITY, best = -INFINITY;
   Two s = 0ull, t = 0ull;  // of the even and the odd entries
   int at = -1;
-  bool bad = false;  // NaN or +inf seen
+  bool bad = false, wide = false;  // bad: NaN or +inf seen
 
-  __device__ __forceinline__ void move(float top, float c, float slack) {
+  __device__ __forceinline__ void move(float top, float c, float wide_at) {
     if (top != top || top == INFINITY) {
       bad = true;
       return;
     }
     if (top > r) {
-      const float d = fmaxf((r - top) * c, kEmpty), f = exp2_fast(d);  // before the first move s = t = 0
-      t = mul2(two(f, f), fma2(two(d, d), s, t));
-      s = mul2(two(f, f), s);
+      const float to = top * c;
+      const bool is_wide = !(fabsf(to) <= wide_at);
+      const float d = wide || is_wide ? (r - top) * c : rc - to;
+      if (r == -INFINITY || d <= kEmpty) {
+        s = t = 0ull;
+      } else {
+        const float f = exp2_fast(d);
+        t = mul2(two(f, f), fma2(two(d, d), s, t));
+        s = mul2(two(f, f), s);
+      }
       r = top;
-      limit = top + slack;
+      rc = to;
+      wide = is_wide;
+      limit = wide ? NAN : top + fminf(kSlack / c, 1e30f);
     }
   }
-  __device__ __forceinline__ void add(float x0, float x1, float c) {
-    float y0, y1;
-    parts(mul2(add2(two(x0, x1), two(-r, -r)), two(c, c)), y0, y1);
-    // -inf, and NaN, which is known from the maximum, end at 2^-150
-    y0 = fmaxf(y0, kEmpty);
-    y1 = fmaxf(y1, kEmpty);
+  __device__ __forceinline__ void add(float y0, float y1) {
     const Two e = two(exp2_fast(y0), exp2_fast(y1));
     s = add2(s, e);
     t = fma2(e, two(y0, y1), t);
+  }
+  __device__ __forceinline__ void add_vector(const Bytes32& v, float c) {
+#pragma unroll
+    for (int i = 0; i < 16 / (int)sizeof(T); ++i) {
+      float x0, x1, y0, y1;
+      pair_values<T>(v, i, true, x0, x1);
+      parts(fma2(two(x0, x1), two(c, c), two(-rc, -rc)), y0, y1);
+      if (sizeof(T) == 4) {
+        y0 = fmaxf(y0, kEmpty);
+        y1 = fmaxf(y1, kEmpty);
+      }
+      add(y0, y1);
+    }
+  }
+  __device__ __forceinline__ void add_wide(float x0, float x1, float c) {
+    add(fmaxf((x0 - r) * c, kEmpty), fmaxf((x1 - r) * c, kEmpty));
   }
   __device__ __forceinline__ void track(float top, int index) {
     if (top > best || at < 0) {
       best = top;
       at = index;
+    }
+  }
+  __device__ __forceinline__ void vector(const Bytes32& v, float c, float wide_at) {
+    const float top = vector_top<T>(v);
+    if (!(top <= limit)) {
+      move(top, c, wide_at);
+      if (wide) {
+#pragma unroll
+        for (int i = 0; i < 16 / (int)sizeof(T); ++i) {
+          float x0, x1;
+          pair_values<T>(v, i, false, x0, x1);
+          add_wide(x0, x1, c);
+        }
+        return;
+      }
+    }
+    add_vector(v, c);
+  }
+  __device__ __forceinline__ void single(float x, float c, float wide_at) {
+    if (!(x <= limit)) move(x, c, wide_at);
+    if (wide)
+      add_wide(x, -INFINITY, c);
+    else
+      add(fmaxf(fmaf(x, c, -rc), kEmpty), kEmpty);
+  }
+  // The sums by r itself.
+  __device__ __forceinline__ void finish(float c, float& s1, float& t1) {
+    float s2, t2;
+    parts(s, s1, s2);
+    parts(t, t1, t2);
+    s1 += s2;
+    t1 += t2;
+    if (!wide && r != -INFINITY) {
+      const float d = fmaf(r, c, -rc), f = exp2_fast(-d);
+      t1 = f * fmaf(-d, s1, t1);
+      s1 *= f;
     }
   }
 };
@@ -312,21 +380,27 @@ __device__ __forceinline__ void write_skipped(const ScoreArgs& a, long long n) {
   }
 }
 
+// References that take the fused product: its rounding stays below 2^-4, and what stands for -inf
+// keeps a weight of 0.
+template <typename T> __device__ __forceinline__ float widest(float c) {
+  if (!(c >= 1e-20f && c <= 1e8f)) return -1.f;
+  return fminf(kWide, -Word<T>::kLow * c + kEmpty - kSlack);
+}
+
 // A cluster of CTAs per row, an equal run of its vectors each (one CTA for many rows).
 //
-// One pass over the logits. The alternatives come out of it exactly, whatever the logits: of the
-// threads' largest entries take the k first in the order (value, index). An entry of the top k
-// lies in one of those k threads' entries, else k threads would each hold an entry before it. So
-// those threads' entries alone are read again (k / THREADS of the row, from L2), and the ones not
-// below the k-th key are ranked.
+// One pass over the logits. The alternatives come out of it exactly, whatever the logits: each
+// thread keeps the largest entry of the first and of the second half of its vectors; of those
+// take the k first in the order (value, index). An entry of the top k lies in one of those k half
+// runs, else k of them would each hold an entry before it. So those runs alone are read again
+// (k / (2 THREADS) of the row, from L2), and the entries not below the k-th key are ranked.
 template <typename T, int THREADS, bool TOP>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel(ScoreArgs a) {
-  typedef Vector<T> Vec;
-  constexpr int WARPS = THREADS / 32, N = Vec::N, AHEAD = 4;
+  constexpr int WARPS = THREADS / 32, N = 32 / sizeof(T), AHEAD = 2;
   __shared__ float s_r[WARPS], s_s[WARPS], s_t[WARPS];
   __shared__ float s_part[3];
   __shared__ int s_bad, s_count;
-  __shared__ unsigned long long s_keys[TOP ? WARPS : 1][TOP ? 32 : 1], s_first[TOP ? SPECKV_MAX_TOP : 1],
+  __shared__ unsigned long long s_keys[TOP ? 2 * WARPS : 1][TOP ? 32 : 1], s_first[TOP ? SPECKV_MAX_TOP : 1],
       s_list[TOP ? THREADS : 1], s_result[TOP ? SPECKV_MAX_TOP : 1], s_best;
   const uint32_t ctas = cluster_size(), rank = cluster_rank();
   const long long n = blockIdx.x / ctas;
@@ -339,56 +413,55 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
   const T* x = static_cast<const T*>(a.logits) + offset;
   const RowSplit row(x, vocab, sizeof(T));
   const int lo = (int)((long long)row.vectors * rank / ctas), hi = (int)((long long)row.vectors * (rank + 1) / ctas);
+  const int half = ((hi - lo + THREADS - 1) / THREADS + 1) / 2;  // vectors of a thread's first run
   const T* vectors = x + row.head;
-  const float c = a.inv_t * kLog2e, slack = fminf(kSlack / c, 1e30f);
+  const float c = a.inv_t * kLog2e, wide_at = widest<T>(c);
   if (tid == 0) s_bad = s_count = 0;
 
-  Running w;
+  Running<T> w;
+  float best0 = -INFINITY;
+  int at0 = -1;
   auto single = [&](int i) {
     const float v = load_f<T>(x[i]);
-    if (!(v <= w.limit)) w.move(v, c, slack);
-    w.add(v, -INFINITY, c);
+    w.single(v, c, wide_at);
     if (TOP) w.track(v, i);
   };
   if (rank == 0 && tid < row.head) single(tid);
-  auto step = [&](const uint4& v, int i) {
-    const float top = Vec::top(v);
-    if (!(top <= w.limit)) w.move(top, c, slack);
-    float f[N];
-    Vec::values(v, f);
-#pragma unroll
-    for (int e = 0; e < N; e += 2) w.add(f[e], f[e + 1], c);
-    if (TOP) w.track(top, row.head + i * N);
-  };
   {
-    uint4 next[AHEAD];
+    Bytes32 next[AHEAD];
     int i = lo + tid;
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u)
       if (i + u * THREADS < hi) next[u] = load_stream(vectors + (long long)(i + u * THREADS) * N);
-    for (; i + (2 * AHEAD - 1) * THREADS < hi; i += AHEAD * THREADS)
+    int j = 0;
+    for (; lo + j * THREADS < hi; j += AHEAD, i += AHEAD * THREADS)
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) {
-        const uint4 v = next[u];
-        next[u] = load_stream(vectors + (long long)(i + (u + AHEAD) * THREADS) * N);
-        step(v, i + u * THREADS);
+        if (TOP && j + u == half) {
+          best0 = w.best;
+          at0 = w.at;
+          w.best = -INFINITY;
+          w.at = -1;
+        }
+        if (i + u * THREADS < hi) {
+          const Bytes32 v = next[u];
+          if (i + (u + AHEAD) * THREADS < hi) next[u] = load_stream(vectors + (long long)(i + (u + AHEAD) * THREADS) * N);
+          w.vector(v, c, wide_at);
+          if (TOP) w.track(vector_top<T>(v), row.head + (i + u * THREADS) * N);
+        }
       }
-#pragma unroll
-    for (int u = 0; u < AHEAD; ++u)
-      if (i + u * THREADS < hi) step(next[u], i + u * THREADS);
-    for (i += AHEAD * THREADS; i < hi; i += THREADS) step(load_stream(vectors + (long long)i * N), i);
+    if (TOP && j <= half) {  // the second run has no vectors
+      best0 = w.best;
+      at0 = w.at;
+      w.best = -INFINITY;
+      w.at = -1;
+    }
   }
   if (rank == ctas - 1 && tid < row.tail) single(row.head + row.vectors * N + tid);
 
   // sums of the CTA
   float r = w.r, s, t;
-  {
-    float s2, t2;
-    parts(w.s, s, s2);
-    parts(w.t, t, t2);
-    s += s2;
-    t += t2;
-  }
+  w.finish(c, s, t);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) {
     const float r2 = __shfl_xor_sync(0xffffffffu, r, off), s2 = __shfl_xor_sync(0xffffffffu, s, off),
@@ -402,9 +475,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
   }
   unsigned long long key = 0;
   if (TOP) {
-    if (w.at >= 0) key = (unsigned long long)order_key(w.best) << 32 | (0xffffffffu - (uint32_t)w.at);
-    key = sort_warp(key);
-    s_keys[warp][lane] = key;
+    if (at0 >= 0) key = (unsigned long long)order_key(best0) << 32 | (0xffffffffu - (uint32_t)at0);
+    s_keys[warp][lane] = sort_warp(key);
+    key = w.at >= 0 ? (unsigned long long)order_key(w.best) << 32 | (0xffffffffu - (uint32_t)w.at) : 0ull;
+    s_keys[WARPS + warp][lane] = sort_warp(key);
   }
   __syncthreads();
   if (w.bad) s_bad = 1;
@@ -424,14 +498,14 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
       s_part[1] = s;
       s_part[2] = t;
     }
-    if (TOP) {  // the k first of the threads' keys: the warps' sorted lists, merged
+    if (TOP) {  // the k first of the runs' keys: the sorted lists, merged
       int head = 0;
-      key = lane < WARPS ? s_keys[lane][0] : 0ull;
+      key = lane < 2 * WARPS ? s_keys[lane][0] : 0ull;
       for (int j = 0; j < a.top; ++j) {
         const uint32_t high = (uint32_t)(key >> 32), most = __reduce_max_sync(0xffffffffu, high);
         const uint32_t low = high == most ? (uint32_t)key : 0u, least = __reduce_max_sync(0xffffffffu, low);
         if (lane == 0) s_first[j] = (unsigned long long)most << 32 | least;
-        if (lane < WARPS && high == most && (uint32_t)key == least) {
+        if (lane < 2 * WARPS && high == most && (uint32_t)key == least) {
           ++head;
           key = head < 32 ? s_keys[lane][head] : 0ull;
         }
@@ -443,36 +517,38 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
     const int k = a.top;
     // a thread's key names the vector of its largest entry: that entry is one of N
     const unsigned long long threshold = s_first[k - 1] == 0ull ? 0ull : s_first[k - 1] - (N - 1);
-    auto offer = [&](int i) {
-      const unsigned long long e = (unsigned long long)order_key(load_f<T>(x[i])) << 32 | (0xffffffffu - (uint32_t)i);
+    auto keep = [&](unsigned long long e) {
       if (e >= threshold) {
         const int place = atomicAdd(&s_count, 1);
         if (place < THREADS) s_list[place] = e;
       }
+    };
+    auto offer = [&](int i) {
+      keep((unsigned long long)order_key(load_f<T>(x[i])) << 32 | (0xffffffffu - (uint32_t)i));
     };
     if (!s_bad) {
       for (int j = warp; j < k; j += WARPS) {
         if (s_first[j] == 0ull) continue;  // fewer threads than k hold entries
         const int at = (int)(0xffffffffu - (uint32_t)s_first[j]);
         const int after = at - row.head - row.vectors * N;
-        const int owner = at < row.head ? at : after >= 0 ? after : ((at - row.head) / N - lo) % THREADS;
+        const int place = at < row.head ? 0 : (at - row.head) / N - lo;
+        const int owner = at < row.head ? at : after >= 0 ? after : place % THREADS;
+        const bool second = at >= row.head && (after >= 0 || place / THREADS >= half);
         if (lane == 0) {
-          if (rank == 0 && owner < row.head) offer(owner);
-          if (rank == ctas - 1 && owner < row.tail) offer(row.head + row.vectors * N + owner);
+          if (!second && rank == 0 && owner < row.head) offer(owner);
+          if (second && rank == ctas - 1 && owner < row.tail) offer(row.head + row.vectors * N + owner);
         }
-        for (int i = lo + owner + lane * THREADS; i < hi; i += 32 * THREADS) {
-          const uint4 v = *reinterpret_cast<const uint4*>(vectors + (long long)i * N);
-          float f[N];
-          Vec::values(v, f);
+        const int end = second ? hi : min(hi, lo + owner + half * THREADS);
+        for (int i = lo + owner + ((second ? half : 0) + lane) * THREADS; i < end; i += 32 * THREADS) {
+          const Bytes32 v = load_stream(vectors + (long long)i * N);
+          if (order_key(vector_top<T>(v)) >= (uint32_t)(threshold >> 32))
 #pragma unroll
-          for (int e = 0; e < N; ++e) {
-            const uint32_t index = (uint32_t)(row.head + i * N + e);
-            const unsigned long long cand = (unsigned long long)order_key(f[e]) << 32 | (0xffffffffu - index);
-            if (cand >= threshold) {
-              const int place = atomicAdd(&s_count, 1);
-              if (place < THREADS) s_list[place] = cand;
+            for (int e = 0; e < N / 2; ++e) {
+              float f0, f1;
+              pair_values<T>(v, e, false, f0, f1);
+              keep((unsigned long long)order_key(f0) << 32 | (0xffffffffu - (uint32_t)(row.head + i * N + 2 * e)));
+              keep((unsigned long long)order_key(f1) << 32 | (0xffffffffu - (uint32_t)(row.head + i * N + 2 * e + 1)));
             }
-          }
         }
       }
     }
@@ -558,15 +634,14 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
 }
 
 constexpr int kGradThreads = 256;
-constexpr int kGradSpan = 8;  // vectors a thread handles
+constexpr int kGradSpan = 4;  // 32-byte vectors a thread handles
 
 // CTA per (row, run of vectors). One exponential and one product chain an entry:
-//   dx = p (u + v y) with y = log2 p, u = -(sum of gradients + g_H H) / T,
+//   dx = p (u + v y) with y = log2 p, p = 2^y, u = -(sum of gradients + g_H H) / T,
 //   v = -g_H ln(2) / T; the token and the alternatives add their own gradient afterwards.
 template <typename T>
 __global__ void __launch_bounds__(kGradThreads) token_logprobs_backward_kernel(ScoreArgs a, int runs) {
-  typedef Vector<T> Vec;
-  constexpr int N = Vec::N;
+  constexpr int N = 32 / sizeof(T);
   const long long n = blockIdx.x / runs;
   const int part = (int)(blockIdx.x - n * runs), tid = threadIdx.x, vocab = (int)a.vocab;
   T* g = static_cast<T*>(a.grad) + n * a.vocab;
@@ -575,13 +650,21 @@ __global__ void __launch_bounds__(kGradThreads) token_logprobs_backward_kernel(S
   const int e_lo = part == 0 ? 0 : row.head + lo * N, e_hi = part == runs - 1 ? vocab : row.head + hi * N;
   long long offset = 0, token = -1;
   if (!score_row(a, n, offset, token) || a.stats[2 * n] == -INFINITY) {
-    for (int i = lo + tid; i < hi; i += kGradThreads)
-      *reinterpret_cast<uint4*>(g + row.head + (long long)i * N) = make_uint4(0, 0, 0, 0);
+    const Bytes32 zero{};
+    for (int i = lo + tid; i < hi; i += kGradThreads) store_stream(g + row.head + (long long)i * N, zero);
     if (part == 0 && tid < row.head) g[tid] = store_f<T>(0.f);
     if (part == runs - 1 && tid < row.tail) g[row.head + row.vectors * N + tid] = store_f<T>(0.f);
     return;
   }
   const T* x = static_cast<const T*>(a.logits) + offset;
+  const bool aligned = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(g)) & 31) == 0;
+  Bytes32 in[kGradSpan];
+  if (aligned) {
+#pragma unroll
+    for (int k = 0; k < kGradSpan; ++k)
+      if (lo + tid + k * kGradThreads < hi)
+        in[k] = load_stream(x + row.head + (long long)(lo + tid + k * kGradThreads) * N);
+  }
   const float ga = a.g_logprobs != nullptr ? a.g_logprobs[n] : 0.f;
   const float gh = a.g_entropy != nullptr ? a.g_entropy[n] : 0.f;
   float all = ga;
@@ -593,23 +676,29 @@ __global__ void __launch_bounds__(kGradThreads) token_logprobs_backward_kernel(S
     const float y = fmaxf(fmaf(z - r, c, -log_s), kEmpty);  // -inf: weight 0, not 0 x inf
     return exp2_fast(y) * fmaf(v, y, u);
   };
-  const bool aligned = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
   if (aligned) {
-    constexpr int AHEAD = 4;
-    for (int i = lo + tid; i < hi; i += AHEAD * kGradThreads) {
-      uint4 in[AHEAD];
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k)
-        if (i + k * kGradThreads < hi) in[k] = load_stream(x + row.head + (long long)(i + k * kGradThreads) * N);
+    for (int k = 0; k < kGradSpan; ++k) {
+      const int i = lo + tid + k * kGradThreads;
+      if (i < hi) {
+        Bytes32 out;
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k)
-        if (i + k * kGradThreads < hi) {
-          float f[N];
-          Vec::values(in[k], f);
-#pragma unroll
-          for (int e = 0; e < N; ++e) f[e] = slope(f[e]);
-          *reinterpret_cast<uint4*>(g + row.head + (long long)(i + k * kGradThreads) * N) = Vec::pack(f);
+        for (int e = 0; e < N / 2; ++e) {
+          float x0, x1, y0, y1;
+          pair_values<T>(in[k], e, false, x0, x1);
+          parts(fma2(add2(two(x0, x1), two(-r, -r)), two(c, c), two(-log_s, -log_s)), y0, y1);
+          y0 = fmaxf(y0, kEmpty);
+          y1 = fmaxf(y1, kEmpty);
+          parts(mul2(two(exp2_fast(y0), exp2_fast(y1)), fma2(two(v, v), two(y0, y1), two(u, u))), x0, x1);
+          if constexpr (sizeof(T) == 4) {
+            out.w[2 * e] = __float_as_uint(x0);
+            out.w[2 * e + 1] = __float_as_uint(x1);
+          } else {
+            out.w[e] = Word<T>::pack(x0, x1);
+          }
         }
+        store_stream(g + row.head + (long long)i * N, out);
+      }
     }
   } else {
     for (int i = row.head + lo * N + tid; i < row.head + hi * N; i += kGradThreads)
@@ -657,16 +746,16 @@ int launch_scores_as(const char* fn, const ScoreArgs& a, int ctas, cudaStream_t 
 
 template <typename T>
 int launch_scores(const char* fn, const ScoreArgs& a, cudaStream_t s) {
-  const long long rows = a.batch * a.per, vectors = a.vocab * sizeof(T) / 16;
+  const long long rows = a.batch * a.per, vectors = a.vocab * sizeof(T) / 32;
   int ctas = 1;
-  while (ctas < 8 && rows * ctas * 2 <= 296 && vectors / (ctas * 2) >= 512) ctas *= 2;
+  while (ctas < 8 && rows * ctas * 2 <= 592 && vectors / (ctas * 2) >= 256) ctas *= 2;
   if (rows * ctas >= (1ll << 31)) return fail(SPECKV_ENOSUPPORT, "%s: too many rows", fn);
-  return a.top > 0 ? launch_scores_as<T, 512, true>(fn, a, ctas, s) : launch_scores_as<T, 512, false>(fn, a, ctas, s);
+  return a.top > 0 ? launch_scores_as<T, 256, true>(fn, a, ctas, s) : launch_scores_as<T, 256, false>(fn, a, ctas, s);
 }
 
 template <typename T>
 int launch_gradient(const char* fn, const ScoreArgs& a, cudaStream_t s) {
-  const long long vectors = a.vocab * (long long)sizeof(T) / 16, span = kGradThreads * kGradSpan;
+  const long long vectors = a.vocab * (long long)sizeof(T) / 32, span = kGradThreads * kGradSpan;
   const long long runs = vectors <= span ? 1 : (vectors + span - 1) / span;
   if (a.batch * a.per * runs >= (1ll << 31)) return fail(SPECKV_ENOSUPPORT, "%s: too many rows", fn);
   token_logprobs_backward_kernel<T><<<(unsigned)(a.batch * a.per * runs), kGradThreads, 0, s>>>(a, (int)runs);

@@ -220,11 +220,9 @@ constexpr float kWide = 1048576.f; // references to 2^20 take the fused product
 // y is one fused product x c - rc with rc = r c rounded; what that rounding left out is put back once
 // at the end. References whose product is so large that the rounding would matter before that
 // (a row of a mask's lowest value, say) take the difference first, vector by vector (wide).
-// best / at: the largest entry of the current run of vectors and the first entry of its vector.
 template <typename T> struct Running {
-  float r = -INFINITY, rc = 0.f, limit = -INFINITY, best = -INFINITY;
+  float r = -INFINITY, rc = 0.f, limit = -INFINITY;
   Two s = 0ull, t = 0ull;  // of the even and the odd entries
-  int at = -1;
   bool bad = false, wide = false;  // bad: NaN or +inf seen
 
   __device__ __forceinline__ void move(float top, float c, float wide_at) {
@@ -270,14 +268,7 @@ template <typename T> struct Running {
   __device__ __forceinline__ void add_wide(float x0, float x1, float c) {
     add(fmaxf((x0 - r) * c, kEmpty), fmaxf((x1 - r) * c, kEmpty));
   }
-  __device__ __forceinline__ void track(float top, int index) {
-    if (top > best || at < 0) {
-      best = top;
-      at = index;
-    }
-  }
-  __device__ __forceinline__ void vector(const Bytes32& v, float c, float wide_at) {
-    const float top = vector_top<T>(v);
+  __device__ __forceinline__ void vector(const Bytes32& v, float top, float c, float wide_at) {
     if (!(top <= limit)) {
       move(top, c, wide_at);
       if (wide) {
@@ -354,20 +345,6 @@ __device__ __forceinline__ unsigned long long remote_u64(const void* p, uint32_t
   return x;
 }
 
-// 32 keys of a warp, largest in lane 0 (bitonic sort).
-__device__ __forceinline__ unsigned long long sort_warp(unsigned long long key) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-    for (int step = size >> 1; step > 0; step >>= 1) {
-      const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, step);
-      const bool larger = ((lane & step) == 0) == ((lane & size) == 0);  // this lane keeps the larger key
-      if ((other > key) == larger) key = other;
-    }
-  return key;
-}
-
 __device__ __forceinline__ void write_skipped(const ScoreArgs& a, long long n) {
   if (threadIdx.x == 0) {
     if (a.logprobs != nullptr) a.logprobs[n] = 0.f;
@@ -389,19 +366,25 @@ template <typename T> __device__ __forceinline__ float widest(float c) {
 
 // A cluster of CTAs per row, an equal run of its vectors each (one CTA for many rows).
 //
-// One pass over the logits. The alternatives come out of it exactly, whatever the logits: each
-// thread keeps the largest entry of the first and of the second half of its vectors; of those
-// take the k first in the order (value, index). An entry of the top k lies in one of those k half
-// runs, else k of them would each hold an entry before it. So those runs alone are read again
-// (k / (2 THREADS) of the row, from L2), and the entries not below the k-th key are ranked.
+// One pass over the logits. For the alternatives each thread also keeps the largest entry of each
+// of kRuns runs of its vectors. A search over the threads' largest entries (a count over the CTA a
+// step) finds a threshold that at least k of them reach and few more; the runs that reach it, and
+// only those (about k kRuns' share of a thread each), are read again, and all their entries that
+// reach it are ranked by (value, index). Those are all of the row's: so if they are k or more, the
+// k first of them are the row's. If not (or if they are too many, or NaN is among the logits),
+// k scans of the row find them.
+constexpr int kRuns = 8, kRunList = 128;
+
 template <typename T, int THREADS, bool TOP>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel(ScoreArgs a) {
+__global__ void __launch_bounds__(THREADS, 1280 / THREADS) token_logprobs_kernel(ScoreArgs a) {
   constexpr int WARPS = THREADS / 32, N = 32 / sizeof(T), AHEAD = 2;
-  __shared__ float s_r[WARPS], s_s[WARPS], s_t[WARPS];
-  __shared__ float s_part[3];
-  __shared__ int s_bad, s_count;
-  __shared__ unsigned long long s_keys[TOP ? 2 * WARPS : 1][TOP ? 32 : 1], s_first[TOP ? SPECKV_MAX_TOP : 1],
-      s_list[TOP ? THREADS : 1], s_result[TOP ? SPECKV_MAX_TOP : 1], s_best;
+  // bits of the order that every logit of the type has alike
+  constexpr int SHIFT = sizeof(T) == 4 ? 0 : Word<T>::kLow == -65504.f ? 13 : 16;
+  __shared__ float s_r[WARPS], s_most[WARPS], s_s[WARPS], s_t[WARPS], s_part[3];
+  __shared__ int s_bad, s_count, s_runs;
+  __shared__ float s_run[TOP ? kRuns : 1][TOP ? THREADS : 1];
+  __shared__ int s_runlist[TOP ? kRunList : 1];
+  __shared__ unsigned long long s_list[TOP ? THREADS : 1], s_result[TOP ? SPECKV_MAX_TOP : 1], s_best;
   const uint32_t ctas = cluster_size(), rank = cluster_rank();
   const long long n = blockIdx.x / ctas;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, vocab = (int)a.vocab;
@@ -411,187 +394,193 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
     return;  // every CTA of the cluster returns here
   }
   const T* x = static_cast<const T*>(a.logits) + offset;
+  const float given = tid == 0 && token >= 0 ? load_f<T>(x[token]) : 0.f;
   const RowSplit row(x, vocab, sizeof(T));
   const int lo = (int)((long long)row.vectors * rank / ctas), hi = (int)((long long)row.vectors * (rank + 1) / ctas);
-  const int half = ((hi - lo + THREADS - 1) / THREADS + 1) / 2;  // vectors of a thread's first run
+  const int own = (hi - lo + THREADS - 1) / THREADS, run = max(1, (own + kRuns - 1) / kRuns);  // vectors of a thread, of a run
   const T* vectors = x + row.head;
   const float c = a.inv_t * kLog2e, wide_at = widest<T>(c);
-  if (tid == 0) s_bad = s_count = 0;
+  if (tid == 0) s_bad = s_count = s_runs = 0;
 
   Running<T> w;
-  float best0 = -INFINITY;
-  int at0 = -1;
+  float best = -INFINITY, most = -INFINITY;  // of the run, of the thread
+  int run_at = 0;                            // the run
   auto single = [&](int i) {
     const float v = load_f<T>(x[i]);
     w.single(v, c, wide_at);
-    if (TOP) w.track(v, i);
+    best = fmaxf(best, v);
   };
   if (rank == 0 && tid < row.head) single(tid);
   {
     Bytes32 next[AHEAD];
-    int i = lo + tid;
+    int i = lo + tid, end = run;
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u)
       if (i + u * THREADS < hi) next[u] = load_stream(vectors + (long long)(i + u * THREADS) * N);
-    int j = 0;
-    for (; lo + j * THREADS < hi; j += AHEAD, i += AHEAD * THREADS)
+    for (int j = 0; j < own; j += AHEAD, i += AHEAD * THREADS)
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) {
-        if (TOP && j + u == half) {
-          best0 = w.best;
-          at0 = w.at;
-          w.best = -INFINITY;
-          w.at = -1;
+        if (TOP && j + u == end && end < own) {
+          s_run[run_at++][tid] = best;
+          most = fmaxf(most, best);
+          best = -INFINITY;
+          end += run;
         }
         if (i + u * THREADS < hi) {
           const Bytes32 v = next[u];
           if (i + (u + AHEAD) * THREADS < hi) next[u] = load_stream(vectors + (long long)(i + (u + AHEAD) * THREADS) * N);
-          w.vector(v, c, wide_at);
-          if (TOP) w.track(vector_top<T>(v), row.head + (i + u * THREADS) * N);
+          const float top = vector_top<T>(v);
+          if (TOP) best = fmaxf(best, top);
+          w.vector(v, top, c, wide_at);
         }
       }
-    if (TOP && j <= half) {  // the second run has no vectors
-      best0 = w.best;
-      at0 = w.at;
-      w.best = -INFINITY;
-      w.at = -1;
-    }
   }
   if (rank == ctas - 1 && tid < row.tail) single(row.head + row.vectors * N + tid);
+  if (TOP) {
+    s_run[run_at][tid] = best;
+    most = fmaxf(most, best);
+  }
 
-  // sums of the CTA
-  float r = w.r, s, t;
+  // sums of the CTA, by its largest reference
+  float s, t, r = w.r, peak = most;
   w.finish(c, s, t);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) {
-    const float r2 = __shfl_xor_sync(0xffffffffu, r, off), s2 = __shfl_xor_sync(0xffffffffu, s, off),
-                t2 = __shfl_xor_sync(0xffffffffu, t, off);
-    join_sums(r, s, t, r2, s2, t2, c);
+    r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, off));
+    if (TOP) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, off));
   }
   if (lane == 0) {
     s_r[warp] = r;
-    s_s[warp] = s;
-    s_t[warp] = t;
-  }
-  unsigned long long key = 0;
-  if (TOP) {
-    if (at0 >= 0) key = (unsigned long long)order_key(best0) << 32 | (0xffffffffu - (uint32_t)at0);
-    s_keys[warp][lane] = sort_warp(key);
-    key = w.at >= 0 ? (unsigned long long)order_key(w.best) << 32 | (0xffffffffu - (uint32_t)w.at) : 0ull;
-    s_keys[WARPS + warp][lane] = sort_warp(key);
+    s_most[warp] = peak;
   }
   __syncthreads();
   if (w.bad) s_bad = 1;
-  if (warp == 0) {
-    // the joins of the warps' sums, in one order
-    r = lane < WARPS ? s_r[lane] : -INFINITY;
-    s = lane < WARPS ? s_s[lane] : 0.f;
-    t = lane < WARPS ? s_t[lane] : 0.f;
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-      const float r2 = __shfl_xor_sync(0xffffffffu, r, off), s2 = __shfl_xor_sync(0xffffffffu, s, off),
-                  t2 = __shfl_xor_sync(0xffffffffu, t, off);
-      join_sums(r, s, t, r2, s2, t2, c);
-    }
-    if (lane == 0) {
-      s_part[0] = r;
-      s_part[1] = s;
-      s_part[2] = t;
-    }
-    if (TOP) {  // the k first of the runs' keys: the sorted lists, merged
-      int head = 0;
-      key = lane < 2 * WARPS ? s_keys[lane][0] : 0ull;
-      for (int j = 0; j < a.top; ++j) {
-        const uint32_t high = (uint32_t)(key >> 32), most = __reduce_max_sync(0xffffffffu, high);
-        const uint32_t low = high == most ? (uint32_t)key : 0u, least = __reduce_max_sync(0xffffffffu, low);
-        if (lane == 0) s_first[j] = (unsigned long long)most << 32 | least;
-        if (lane < 2 * WARPS && high == most && (uint32_t)key == least) {
-          ++head;
-          key = head < 32 ? s_keys[lane][head] : 0ull;
-        }
-      }
-    }
+  for (int v = 0; v < WARPS; ++v) {
+    r = fmaxf(r, s_r[v]);
+    if (TOP) peak = fmaxf(peak, s_most[v]);
   }
-  __syncthreads();
+  {
+    const float d = fmaxf((w.r - r) * c, kEmpty), f = exp2_fast(d);  // no entry above -inf: s = t = 0
+    t = f * fmaf(d, s, t);
+    s *= f;
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, off);
+    t += __shfl_xor_sync(0xffffffffu, t, off);
+  }
+  if (lane == 0) {
+    s_s[warp] = s;
+    s_t[warp] = t;
+  }
   if (TOP) {
     const int k = a.top;
-    // a thread's key names the vector of its largest entry: that entry is one of N
-    const unsigned long long threshold = s_first[k - 1] == 0ull ? 0ull : s_first[k - 1] - (N - 1);
-    auto keep = [&](unsigned long long e) {
-      if (e >= threshold) {
+    const uint32_t mine = order_key(most) >> SHIFT, first = order_key(peak) >> SHIFT;
+    // down from the largest entry in growing steps, then halving: k to k + 6 threads
+    uint32_t above = first + 1, level = first, step = 1u << (19 - SHIFT);
+    int reach = 0;
+    for (;;) {
+      level = first > step ? first - step : 0u;
+      reach = __syncthreads_count(mine >= level);
+      if (reach >= k || level == 0u) break;
+      above = level;
+      step *= 4u;
+      if (step >= (1u << 30)) step = 0xffffffffu;
+    }
+    while (reach > k + 6 && above - level > 1u) {
+      const uint32_t middle = level + (above - level) / 2;
+      const int count = __syncthreads_count(mine >= middle);
+      if (count >= k) {
+        level = middle;
+        reach = count;
+      } else {
+        above = middle;
+      }
+    }
+    if (mine >= level)
+      for (int i = 0; i <= run_at; ++i)
+        if (order_key(s_run[i][tid]) >> SHIFT >= level) {
+          const int place = atomicAdd(&s_runs, 1);
+          if (place < kRunList) s_runlist[place] = i << 16 | tid;
+        }
+    if (tid < SPECKV_MAX_TOP) s_result[tid] = 0ull;
+    __syncthreads();
+    const int runs = s_runs;
+    auto key_of = [](float v, int i) { return (unsigned long long)order_key(v) << 32 | (0xffffffffu - (uint32_t)i); };
+    auto keep = [&](float v, int i) {
+      if (order_key(v) >> SHIFT >= level) {
         const int place = atomicAdd(&s_count, 1);
-        if (place < THREADS) s_list[place] = e;
+        if (place < THREADS) s_list[place] = key_of(v, i);
       }
     };
-    auto offer = [&](int i) {
-      keep((unsigned long long)order_key(load_f<T>(x[i])) << 32 | (0xffffffffu - (uint32_t)i));
-    };
-    if (!s_bad) {
-      for (int j = warp; j < k; j += WARPS) {
-        if (s_first[j] == 0ull) continue;  // fewer threads than k hold entries
-        const int at = (int)(0xffffffffu - (uint32_t)s_first[j]);
-        const int after = at - row.head - row.vectors * N;
-        const int place = at < row.head ? 0 : (at - row.head) / N - lo;
-        const int owner = at < row.head ? at : after >= 0 ? after : place % THREADS;
-        const bool second = at >= row.head && (after >= 0 || place / THREADS >= half);
-        if (lane == 0) {
-          if (!second && rank == 0 && owner < row.head) offer(owner);
-          if (second && rank == ctas - 1 && owner < row.tail) offer(row.head + row.vectors * N + owner);
+    if (runs <= kRunList) {
+      for (int item = tid; item < runs * run; item += THREADS) {
+        const int entry = s_runlist[item / run], part = item % run, owner = entry & 0xffff, number = entry >> 16;
+        if (part == 0 && number == 0 && rank == 0 && owner < row.head) keep(load_f<T>(x[owner]), owner);
+        if (part == 0 && number == run_at && rank == ctas - 1 && owner < row.tail) {
+          const int i = row.head + row.vectors * N + owner;
+          keep(load_f<T>(x[i]), i);
         }
-        const int end = second ? hi : min(hi, lo + owner + half * THREADS);
-        for (int i = lo + owner + ((second ? half : 0) + lane) * THREADS; i < end; i += 32 * THREADS) {
+        const int i = lo + owner + (number * run + part) * THREADS;
+        if (i < hi) {
           const Bytes32 v = load_stream(vectors + (long long)i * N);
-          if (order_key(vector_top<T>(v)) >= (uint32_t)(threshold >> 32))
+          if (order_key(vector_top<T>(v)) >> SHIFT >= level)
 #pragma unroll
             for (int e = 0; e < N / 2; ++e) {
               float f0, f1;
               pair_values<T>(v, e, false, f0, f1);
-              keep((unsigned long long)order_key(f0) << 32 | (0xffffffffu - (uint32_t)(row.head + i * N + 2 * e)));
-              keep((unsigned long long)order_key(f1) << 32 | (0xffffffffu - (uint32_t)(row.head + i * N + 2 * e + 1)));
+              keep(f0, row.head + i * N + 2 * e);
+              keep(f1, row.head + i * N + 2 * e + 1);
             }
         }
       }
     }
-    if (tid < SPECKV_MAX_TOP) s_result[tid] = 0ull;
     __syncthreads();
-    if (!s_bad && s_count <= THREADS) {
-      if (tid < s_count) {
-        const unsigned long long own = s_list[tid];
+    const int count = s_count;
+    if (!s_bad && runs <= kRunList && count >= k && count <= THREADS) {
+      if (tid < count) {
+        const unsigned long long key = s_list[tid];
         int before = 0;
-        for (int i = 0; i < s_count; ++i) before += s_list[i] > own;
-        if (before < k) s_result[before] = own;
+        for (int i = 0; i < count; ++i) before += s_list[i] > key;
+        if (before < k) s_result[before] = key;
       }
     } else {
-      // NaN among the logits (its order is not the threads'), or more entries than the list
-      // holds at or above the threshold: k scans
       unsigned long long last = ~0ull;
       for (int j = 0; j < k; ++j) {
         __syncthreads();
         if (tid == 0) s_best = 0ull;
         __syncthreads();
-        unsigned long long mine = 0ull;
+        unsigned long long found = 0ull;
         auto scan = [&](int i) {
-          const unsigned long long e =
-              (unsigned long long)order_key(load_f<T>(x[i])) << 32 | (0xffffffffu - (uint32_t)i);
-          if (e < last && e > mine) mine = e;
+          const unsigned long long key = key_of(load_f<T>(x[i]), i);
+          if (key < last && key > found) found = key;
         };
         if (rank == 0 && tid < row.head) scan(tid);
         for (int i = lo * N + tid; i < hi * N; i += THREADS) scan(row.head + i);
         if (rank == ctas - 1 && tid < row.tail) scan(row.head + row.vectors * N + tid);
-        if (mine) atomicMax(&s_best, mine);
+        if (found) atomicMax(&s_best, found);
         __syncthreads();
         last = s_best;
         if (tid == 0) s_result[j] = last;
         if (last == 0ull) break;
       }
     }
-    __syncthreads();
   }
+  __syncthreads();
   bool bad = s_bad;
-  r = s_part[0];
-  s = s_part[1];
-  t = s_part[2];
+  s = t = 0.f;
+#pragma unroll
+  for (int v = 0; v < WARPS; ++v) {
+    s += s_s[v];
+    t += s_t[v];
+  }
   if (ctas > 1) {
+    if (tid == 0) {
+      s_part[0] = r;
+      s_part[1] = s;
+      s_part[2] = t;
+    }
     cluster_sync();
     if (rank == 0) {
       for (uint32_t o = 1; o < ctas; ++o) {
@@ -605,27 +594,27 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
     const bool empty = r == -INFINITY && !bad;
     auto logprob = [&](float v) { return bad ? NAN : empty ? -INFINITY : (v - r) * a.inv_t - log_s * kLn2; };
     if (tid == 0) {
-      if (a.logprobs != nullptr) a.logprobs[n] = logprob(load_f<T>(x[token]));
+      if (a.logprobs != nullptr) a.logprobs[n] = logprob(given);
       a.entropy[n] = bad ? NAN : empty ? 0.f : fmaxf(log_s - t / s, 0.f) * kLn2;
       a.stats[2 * n] = bad ? NAN : r;
       a.stats[2 * n + 1] = bad ? NAN : empty ? -INFINITY : log_s;
     }
     if (TOP) {
       const int k = a.top;
-      auto emit = [&](int place, unsigned long long e) {
+      auto emit = [&](int place, unsigned long long key) {
         const long long at = n * k + place;
-        a.top_ids[at] = 0xffffffffu - (uint32_t)e;
-        a.top_logprobs[at] = logprob(order_value((uint32_t)(e >> 32)));
+        a.top_ids[at] = 0xffffffffu - (uint32_t)key;
+        a.top_logprobs[at] = logprob(order_value((uint32_t)(key >> 32)));
       };
       if (ctas == 1) {
         if (tid < k) emit(tid, s_result[tid]);
       } else {
         // the CTAs' alternatives (at most 8 x 32), ranked
         for (int i = tid; i < (int)ctas * k; i += THREADS) {
-          const unsigned long long own = remote_u64(&s_result[i % k], i / k);
+          const unsigned long long key = remote_u64(&s_result[i % k], i / k);
           int before = 0;
-          for (int o = 0; o < (int)ctas * k; ++o) before += remote_u64(&s_result[o % k], o / k) > own;
-          if (own != 0ull && before < k) emit(before, own);
+          for (int o = 0; o < (int)ctas * k; ++o) before += remote_u64(&s_result[o % k], o / k) > key;
+          if (key != 0ull && before < k) emit(before, key);
         }
       }
     }

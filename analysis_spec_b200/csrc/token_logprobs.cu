@@ -125,9 +125,17 @@ __device__ __forceinline__ Bytes32 load_stream(const void* p) {
                : "l"(p));
   return r;
 }
+__device__ __forceinline__ Bytes32 from_pieces(const uint4& a, const uint4& b) {
+  return Bytes32{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+}
 __device__ __forceinline__ void store_stream(void* p, const Bytes32& v) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v.w[0]), "r"(v.w[1]),
                "r"(v.w[2]), "r"(v.w[3]), "r"(v.w[4]), "r"(v.w[5]), "r"(v.w[6]), "r"(v.w[7])
+               : "memory");
+}
+
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from)
                : "memory");
 }
 
@@ -137,6 +145,7 @@ template <typename T> struct Word;
 template <> struct Word<float> {
   static constexpr int N = 1;
   static constexpr float kLow = -INFINITY;  // the distance is cut instead
+  static constexpr uint32_t kNone = 0xff800000u;  // -inf
   static __device__ __forceinline__ uint32_t top(uint32_t x, uint32_t y) {
     return __float_as_uint(max_nan(__uint_as_float(x), __uint_as_float(y)));
   }
@@ -146,6 +155,7 @@ template <> struct Word<float> {
 template <> struct Word<__nv_bfloat16> {
   static constexpr int N = 2;
   static constexpr float kLow = -1e30f;
+  static constexpr uint32_t kNone = 0xff80ff80u;
   static __device__ __forceinline__ __nv_bfloat162 pair(uint32_t u) { return *reinterpret_cast<__nv_bfloat162*>(&u); }
   static __device__ __forceinline__ uint32_t bits(__nv_bfloat162 h) { return *reinterpret_cast<uint32_t*>(&h); }
   static __device__ __forceinline__ uint32_t top(uint32_t x, uint32_t y) { return bits(__hmax2_nan(pair(x), pair(y))); }
@@ -166,6 +176,7 @@ template <> struct Word<__nv_bfloat16> {
 template <> struct Word<__half> {
   static constexpr int N = 2;
   static constexpr float kLow = -65504.f;
+  static constexpr uint32_t kNone = 0xfc00fc00u;
   static __device__ __forceinline__ __half2 pair(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
   static __device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
   static __device__ __forceinline__ uint32_t top(uint32_t x, uint32_t y) { return bits(__hmax2_nan(pair(x), pair(y))); }
@@ -200,14 +211,15 @@ template <typename T> __device__ __forceinline__ float vector_top(const Bytes32&
                            W::top(W::top(v.w[4], v.w[5]), W::top(v.w[6], v.w[7]))));
 }
 
-// A row as single entries up to the first 32-byte boundary, 32-byte vectors, and single entries.
-struct RowSplit {
-  int head, vectors, tail;  // entries, vectors, entries
+// A row as single entries up to the first boundary of BYTES, whole pieces of that size, and
+// single entries.
+template <int BYTES> struct RowSplit {
+  int head, pieces, tail;  // entries, pieces, entries
   __device__ __forceinline__ RowSplit(const void* row, int vocab, int size) {
-    const int n = 32 / size;
-    head = min(vocab, (int)((32 - (reinterpret_cast<uintptr_t>(row) & 31)) & 31) / size);
-    vectors = (vocab - head) / n;
-    tail = vocab - head - vectors * n;
+    const int n = BYTES / size;
+    head = min(vocab, (int)((BYTES - (reinterpret_cast<uintptr_t>(row) & (BYTES - 1))) & (BYTES - 1)) / size);
+    pieces = (vocab - head) / n;
+    tail = vocab - head - pieces * n;
   }
 };
 
@@ -364,7 +376,8 @@ template <typename T> __device__ __forceinline__ float widest(float c) {
   return fminf(kWide, -Word<T>::kLow * c + kEmpty - kSlack);
 }
 
-// A cluster of CTAs per row, an equal run of its vectors each (one CTA for many rows).
+// A cluster of CTAs per row, an equal run of its vectors each (one CTA for many rows). A vector is two
+// 16-byte pieces half a warp's kilobyte apart, so that each copy of a warp is one run of memory.
 //
 // One pass over the logits. For the alternatives each thread also keeps the largest entry of each
 // of kRuns runs of its vectors. A search over the threads' largest entries (a count over the CTA a
@@ -376,10 +389,11 @@ template <typename T> __device__ __forceinline__ float widest(float c) {
 constexpr int kRuns = 8, kRunList = 128;
 
 template <typename T, int THREADS, bool TOP>
-__global__ void __launch_bounds__(THREADS, 1280 / THREADS) token_logprobs_kernel(ScoreArgs a) {
-  constexpr int WARPS = THREADS / 32, N = 32 / sizeof(T), AHEAD = 2;
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel(ScoreArgs a) {
+  constexpr int WARPS = THREADS / 32, P = 16 / sizeof(T), AHEAD = 4;  // P: entries of a piece
   // bits of the order that every logit of the type has alike
   constexpr int SHIFT = sizeof(T) == 4 ? 0 : Word<T>::kLow == -65504.f ? 13 : 16;
+  __shared__ uint4 s_ring[AHEAD][2][THREADS];
   __shared__ float s_r[WARPS], s_most[WARPS], s_s[WARPS], s_t[WARPS], s_part[3];
   __shared__ int s_bad, s_count, s_runs;
   __shared__ float s_run[TOP ? kRuns : 1][TOP ? THREADS : 1];
@@ -395,10 +409,15 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) token_logprobs_kernel
   }
   const T* x = static_cast<const T*>(a.logits) + offset;
   const float given = tid == 0 && token >= 0 ? load_f<T>(x[token]) : 0.f;
-  const RowSplit row(x, vocab, sizeof(T));
-  const int lo = (int)((long long)row.vectors * rank / ctas), hi = (int)((long long)row.vectors * (rank + 1) / ctas);
+  const RowSplit<16> row(x, vocab, sizeof(T));
+  const int blocks = (row.pieces + 63) / 64;  // 32 vectors each, the last one perhaps in part
+  const int lo = 32 * (int)((long long)blocks * rank / ctas), hi = 32 * (int)((long long)blocks * (rank + 1) / ctas);
   const int own = (hi - lo + THREADS - 1) / THREADS, run = max(1, (own + kRuns - 1) / kRuns);  // vectors of a thread, of a run
-  const T* vectors = x + row.head;
+  const T* pieces = x + row.head;
+  auto no_second = [](Bytes32& v) {
+    v.w[4] = v.w[5] = v.w[6] = v.w[7] = Word<T>::kNone;
+  };
+  auto piece_of = [](int i, int h) { return (i >> 5) * 64 + h * 32 + (i & 31); };
   const float c = a.inv_t * kLog2e, wide_at = widest<T>(c);
   if (tid == 0) s_bad = s_count = s_runs = 0;
 
@@ -412,11 +431,19 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) token_logprobs_kernel
   };
   if (rank == 0 && tid < row.head) single(tid);
   {
-    Bytes32 next[AHEAD];
+    // Each thread's vectors pass through its own slots of shared memory, AHEAD of them under way: no
+    // registers wait for memory, and no thread waits for another.
+    auto fetch = [&](int u, int i) {
+      if (i < hi) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (piece_of(i, h) < row.pieces) copy_async(&s_ring[u][h][tid], pieces + (long long)piece_of(i, h) * P);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
     int i = lo + tid, end = run;
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u)
-      if (i + u * THREADS < hi) next[u] = load_stream(vectors + (long long)(i + u * THREADS) * N);
+    for (int u = 0; u < AHEAD; ++u) fetch(u, i + u * THREADS);
     for (int j = 0; j < own; j += AHEAD, i += AHEAD * THREADS)
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) {
@@ -426,16 +453,19 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) token_logprobs_kernel
           best = -INFINITY;
           end += run;
         }
-        if (i + u * THREADS < hi) {
-          const Bytes32 v = next[u];
-          if (i + (u + AHEAD) * THREADS < hi) next[u] = load_stream(vectors + (long long)(i + (u + AHEAD) * THREADS) * N);
+        asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
+        const int at = i + u * THREADS;
+        if (at < hi && piece_of(at, 0) < row.pieces) {
+          Bytes32 v = from_pieces(s_ring[u][0][tid], s_ring[u][1][tid]);
+          if (piece_of(at, 1) >= row.pieces) no_second(v);
           const float top = vector_top<T>(v);
+          fetch(u, at + AHEAD * THREADS);
           if (TOP) best = fmaxf(best, top);
           w.vector(v, top, c, wide_at);
         }
       }
   }
-  if (rank == ctas - 1 && tid < row.tail) single(row.head + row.vectors * N + tid);
+  if (rank == ctas - 1 && tid < row.tail) single(row.head + row.pieces * P + tid);
   if (TOP) {
     s_run[run_at][tid] = best;
     most = fmaxf(most, best);
@@ -519,20 +549,26 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) token_logprobs_kernel
         const int entry = s_runlist[item / run], part = item % run, owner = entry & 0xffff, number = entry >> 16;
         if (part == 0 && number == 0 && rank == 0 && owner < row.head) keep(load_f<T>(x[owner]), owner);
         if (part == 0 && number == run_at && rank == ctas - 1 && owner < row.tail) {
-          const int i = row.head + row.vectors * N + owner;
+          const int i = row.head + row.pieces * P + owner;
           keep(load_f<T>(x[i]), i);
         }
         const int i = lo + owner + (number * run + part) * THREADS;
-        if (i < hi) {
-          const Bytes32 v = load_stream(vectors + (long long)i * N);
-          if (order_key(vector_top<T>(v)) >> SHIFT >= level)
+        if (i < hi && piece_of(i, 0) < row.pieces) {
 #pragma unroll
-            for (int e = 0; e < N / 2; ++e) {
-              float f0, f1;
-              pair_values<T>(v, e, false, f0, f1);
-              keep(f0, row.head + i * N + 2 * e);
-              keep(f1, row.head + i * N + 2 * e + 1);
+          for (int h = 0; h < 2; ++h) {
+            const int piece = piece_of(i, h);
+            if (piece < row.pieces) {
+              const uint4 raw = __ldg(reinterpret_cast<const uint4*>(pieces + (long long)piece * P));
+              const Bytes32 v{{raw.x, raw.y, raw.z, raw.w}};
+#pragma unroll
+              for (int e = 0; e < P / 2; ++e) {
+                float f0, f1;
+                pair_values<T>(v, e, false, f0, f1);
+                keep(f0, row.head + piece * P + 2 * e);
+                keep(f1, row.head + piece * P + 2 * e + 1);
+              }
             }
+          }
         }
       }
     }
@@ -557,8 +593,8 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) token_logprobs_kernel
           if (key < last && key > found) found = key;
         };
         if (rank == 0 && tid < row.head) scan(tid);
-        for (int i = lo * N + tid; i < hi * N; i += THREADS) scan(row.head + i);
-        if (rank == ctas - 1 && tid < row.tail) scan(row.head + row.vectors * N + tid);
+        for (int i = lo * 2 * P + tid; i < min(hi * 2, row.pieces) * P; i += THREADS) scan(row.head + i);
+        if (rank == ctas - 1 && tid < row.tail) scan(row.head + row.pieces * P + tid);
         if (found) atomicMax(&s_best, found);
         __syncthreads();
         last = s_best;
@@ -609,11 +645,14 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) token_logprobs_kernel
       if (ctas == 1) {
         if (tid < k) emit(tid, s_result[tid]);
       } else {
-        // the CTAs' alternatives (at most 8 x 32), ranked
-        for (int i = tid; i < (int)ctas * k; i += THREADS) {
-          const unsigned long long key = remote_u64(&s_result[i % k], i / k);
+        // the CTAs' alternatives, ranked
+        const int all = (int)ctas * k;
+        if (tid < all) s_list[tid] = remote_u64(&s_result[tid % k], tid / k);
+        __syncthreads();
+        if (tid < all) {
+          const unsigned long long key = s_list[tid];
           int before = 0;
-          for (int o = 0; o < (int)ctas * k; ++o) before += remote_u64(&s_result[o % k], o / k) > key;
+          for (int o = 0; o < all; ++o) before += s_list[o] > key;
           if (key != 0ull && before < k) emit(before, key);
         }
       }
@@ -634,15 +673,15 @@ __global__ void __launch_bounds__(kGradThreads) token_logprobs_backward_kernel(S
   const long long n = blockIdx.x / runs;
   const int part = (int)(blockIdx.x - n * runs), tid = threadIdx.x, vocab = (int)a.vocab;
   T* g = static_cast<T*>(a.grad) + n * a.vocab;
-  const RowSplit row(g, vocab, sizeof(T));
-  const int lo = part * kGradThreads * kGradSpan, hi = min(row.vectors, lo + kGradThreads * kGradSpan);
+  const RowSplit<32> row(g, vocab, sizeof(T));
+  const int lo = part * kGradThreads * kGradSpan, hi = min(row.pieces, lo + kGradThreads * kGradSpan);
   const int e_lo = part == 0 ? 0 : row.head + lo * N, e_hi = part == runs - 1 ? vocab : row.head + hi * N;
   long long offset = 0, token = -1;
   if (!score_row(a, n, offset, token) || a.stats[2 * n] == -INFINITY) {
     const Bytes32 zero{};
     for (int i = lo + tid; i < hi; i += kGradThreads) store_stream(g + row.head + (long long)i * N, zero);
     if (part == 0 && tid < row.head) g[tid] = store_f<T>(0.f);
-    if (part == runs - 1 && tid < row.tail) g[row.head + row.vectors * N + tid] = store_f<T>(0.f);
+    if (part == runs - 1 && tid < row.tail) g[row.head + row.pieces * N + tid] = store_f<T>(0.f);
     return;
   }
   const T* x = static_cast<const T*>(a.logits) + offset;
@@ -695,7 +734,7 @@ __global__ void __launch_bounds__(kGradThreads) token_logprobs_backward_kernel(S
   }
   if (part == 0 && tid < row.head) g[tid] = store_f<T>(slope(load_f<T>(x[tid])));
   if (part == runs - 1 && tid < row.tail) {
-    const int i = row.head + row.vectors * N + tid;
+    const int i = row.head + row.pieces * N + tid;
     g[i] = store_f<T>(slope(load_f<T>(x[i])));
   }
   // the entries that have a gradient of their own, each written once more, whole

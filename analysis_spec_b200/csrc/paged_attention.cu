@@ -502,31 +502,77 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? (NT == 1 ? 4 : 3) : D =
   if (threadIdx.x == 0) plan.joins[cta] = join;
 }
 
-// Joins the parts of the items that more than one share holds, in the order of the shares.
+// Joins the parts of the items that more than one share holds, in the order of the shares: CTA per
+// (share, query head of the item that begins in it); its warps take every fourth part each.
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(128) paged_attention_join_kernel(PagedArgs a, PlanArgs plan) {
-  constexpr int PART = 8 * NT * (D + 2);
+  constexpr int PART = 8 * NT * (D + 2), E = D / 32, BATCH = 4;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Join j = plan.joins[blockIdx.x];
-  if (j.count == 0) return;
-  const long long group = a.q_heads / a.kv_heads;
+  const int group = (int)(a.q_heads / a.kv_heads), head = blockIdx.y;
   const int hk = j.h / plan.chunks, h0 = (j.h - hk * plan.chunks) * 8 * NT;
-  const int heads = min((int)group - h0, 8 * NT);
-  const float* first = plan.parts + (long long)j.slot * PART;
-  const float* rest = plan.parts + (long long)2 * blockIdx.x * PART;  // part i >= 1: rest + 2 i PART
-  for (int i = threadIdx.x; i < heads * D; i += 128) {
-    const int head = i / D;
-    float top = -INFINITY;
-    for (int k = 0; k < j.count; ++k) top = fmaxf(top, (k == 0 ? first : rest + (long long)2 * k * PART)[8 * NT * D + head]);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, all = 0.f;
-    for (int k = 0; k < j.count; ++k) {
-      const float* p = k == 0 ? first : rest + (long long)2 * k * PART;
-      const float f = exp2f(p[8 * NT * D + head] - ref);
-      all = fmaf(p[8 * NT * (D + 1) + head], f, all);
-      sum = fmaf(p[i], f, sum);
+  if (j.count == 0 || h0 + head >= group) return;
+  __shared__ float s_top[4], s_all[4], s_sum[4][D];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // part 0 is at its own slot, part k >= 1 the first of share blockIdx.x + k
+  auto part = [&](int k) {
+    return plan.parts + (long long)(k == 0 ? j.slot : 2 * ((int)blockIdx.x + k)) * PART;
+  };
+  float top = -INFINITY, all = 0.f, sum[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) sum[e] = 0.f;
+  for (int k0 = warp; k0 < j.count; k0 += 4 * BATCH) {
+    float m[BATCH], l[BATCH], v[BATCH][E];
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int k = k0 + 4 * i;
+      m[i] = -INFINITY;
+      if (k < j.count) {
+        const float* p = part(k);
+        m[i] = p[8 * NT * D + head];
+        l[i] = p[8 * NT * (D + 1) + head];
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[i][e] = p[head * D + lane + 32 * e];
+      }
     }
-    static_cast<T*>(a.out)[(j.b * a.q_heads + hk * group + h0) * D + i] = store_f<T>(all == 0.f ? 0.f : sum / all);
+    float next = top;
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) next = fmaxf(next, m[i]);
+    const float ref = next == -INFINITY ? 0.f : next, keep = exp2f(top - ref);
+    all *= keep;
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum[e] *= keep;
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i)
+      if (k0 + 4 * i < j.count) {
+        const float f = exp2f(m[i] - ref);
+        all = fmaf(l[i], f, all);
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum[e] = fmaf(v[i][e], f, sum[e]);
+      }
+    top = next;
+  }
+  if (lane == 0) {
+    s_top[warp] = top;
+    s_all[warp] = all;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) s_sum[warp][lane + 32 * e] = sum[e];
+  __syncthreads();
+  top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+  const float ref = top == -INFINITY ? 0.f : top;
+  float f[4], total = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    f[w] = exp2f(s_top[w] - ref);
+    total = fmaf(s_all[w], f[w], total);
+  }
+  T* out = static_cast<T*>(a.out) + (j.b * a.q_heads + hk * group + h0 + head) * D;
+  for (int d = threadIdx.x; d < D; d += 128) {
+    float o = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) o = fmaf(s_sum[w][d], f[w], o);
+    out[d] = store_f<T>(total == 0.f ? 0.f : o / total);
   }
 }
 
@@ -569,7 +615,7 @@ int launch_mma(const PagedArgs& a, const PlanArgs& plan, int ctas, cudaStream_t 
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas);
+  cfg.gridDim = dim3(ctas, (unsigned)min((int)(a.q_heads / a.kv_heads), plan.heads));
   cfg.blockDim = dim3(128);
   cfg.stream = s;
   cfg.attrs = &attr;
@@ -595,7 +641,11 @@ int launch_paged(const PagedArgs& a, int32_t dtype, void* workspace, int64_t byt
   if constexpr (sizeof(T) == 2) {
     const int sms = sm_count();
     const int64_t group = a.q_heads / a.kv_heads;
-    const int nt = head_tiles(a.dim, group), ctas = sms * ctas_per_sm(a.dim, nt);
+    const int nt = head_tiles(a.dim, group);
+    // no more CTAs than shares of the longest lengths that the table can hold
+    const double most = (double)a.batch * a.kv_heads * ((group + 8 * nt - 1) / (8 * nt)) *
+                        ((a.table.width * a.table.page_size + kTile - 1) / kTile);
+    const int full = sms * ctas_per_sm(a.dim, nt), ctas = most < (double)full * kMinTiles ? (int)((most + kMinTiles - 1) / kMinTiles) : full;
     const int64_t need = workspace_bytes(a.q_heads, a.kv_heads, a.dim, dtype, sms);
     if (sms == 0) return fail(SPECKV_ECUDA, "speckv_paged_attention: no SM count");
     if (workspace == nullptr || bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)
@@ -603,7 +653,7 @@ int launch_paged(const PagedArgs& a, int32_t dtype, void* workspace, int64_t byt
                   (long long)bytes, (long long)need);
     PlanArgs plan;
     plan.joins = static_cast<Join*>(workspace);
-    plan.parts = reinterpret_cast<float*>(plan.joins + ctas);
+    plan.parts = reinterpret_cast<float*>(plan.joins + full);
     plan.heads = 8 * nt;
     plan.chunks = (int)((group + plan.heads - 1) / plan.heads);
     if (a.dim == 64) return nt == 1 ? launch_mma<T, 64, 1>(a, plan, ctas, s) : launch_mma<T, 64, 2>(a, plan, ctas, s);

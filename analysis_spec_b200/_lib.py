@@ -71,7 +71,7 @@ SIGNATURES = {
                             _i64, _i64, _i32, _i64, _i64, _i64, _i64, _i64, _i32, _p],
     'speckv_paged_attention': [_p, _p, _p, _pi64, _p, _i64, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _i64, _f32,
                                _i32, _p, _i64, _p],
-    'speckv_paged_attention_workspace': [_i64, _i64, _i64, _i32],  # returns bytes, not a status
+    'speckv_paged_attention_workspace': [_i64, _i64, _i64, _i64, _i64, _i64, _i32],  # returns bytes, not a status
     'speckv_token_logprobs': [_p, _i32, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _f32,
                               _i32, _p, _p, _p, _p, _p, _p],
     'speckv_token_logprobs_backward': [_p, _i32, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _f32, _i32, _p, _p,

@@ -182,7 +182,8 @@ Tensor paged_attention(const Tensor& query, const Tensor& key_pages, const Tenso
   Tensor out = given != nullptr ? *given : at::empty({batch, 1, q_heads, dim}, query.options());
   if (batch == 0) return out;
   // a workspace of this call alone: other streams and captured graphs have their own
-  const int64_t need = speckv_paged_attention_workspace(q_heads, kv_heads, dim, code);
+  const int64_t need = speckv_paged_attention_workspace(batch, q_heads, kv_heads, dim, page_table.size(1),
+                                                        key_pages.size(2), code);
   Tensor workspace;
   if (need > 0) workspace = at::empty({need}, query.options().dtype(at::kByte));
   const int64_t st[8] = {query.stride(0),       query.stride(1),       key_pages.stride(0),   key_pages.stride(1),

@@ -117,91 +117,155 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_scalar_kernel(App
   }
 }
 
-// 16 bytes of rows: N elements.
-template <typename T> struct Pack {
-  static constexpr int N = 16 / sizeof(T);
-  union {
-    uint4 raw;
-    T e[N];
-  };
+// 16 bytes of a row: their elements as pairs of fp32 numbers.
+template <typename T> struct Piece;
+template <> struct Piece<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void get(const uint4& r, float (&x)[4]) {
+    x[0] = __uint_as_float(r.x), x[1] = __uint_as_float(r.y), x[2] = __uint_as_float(r.z), x[3] = __uint_as_float(r.w);
+  }
+  static __device__ __forceinline__ uint4 put(const float (&x)[4]) {
+    return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+  }
+};
+template <> struct Piece<__nv_bfloat16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void get(const uint4& r, float (&x)[8]) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // a bf16 is the upper half of an fp32
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ uint32_t pair(float x, float y) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ uint4 put(const float (&x)[8]) {
+    return make_uint4(pair(x[0], x[1]), pair(x[2], x[3]), pair(x[4], x[5]), pair(x[6], x[7]));
+  }
+};
+template <> struct Piece<__half> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void get(const uint4& r, float (&x)[8]) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  }
+  static __device__ __forceinline__ uint32_t pair(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ uint4 put(const float (&x)[8]) {
+    return make_uint4(pair(x[0], x[1]), pair(x[2], x[3]), pair(x[4], x[5]), pair(x[6], x[7]));
+  }
 };
 
 // x' = x c - y s, y' = y c + x s of the pairs of two 16-byte pieces of a row: element i of one with
 // element i of the other, or neighbours within each.
-template <typename T, bool INTERLEAVED>
-__device__ __forceinline__ void rotate(Pack<T>& x, Pack<T>& y, const float (&c)[Pack<T>::N],
-                                       const float (&s)[Pack<T>::N]) {
-  constexpr int N = Pack<T>::N;
+template <typename T, bool INTERLEAVED, int N>
+__device__ __forceinline__ void rotate(uint4& px, uint4& py, const float (&c)[N], const float (&s)[N]) {
+  float x[N], y[N];
+  Piece<T>::get(px, x);
+  Piece<T>::get(py, y);
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    T& first = INTERLEAVED ? (i < N / 2 ? x.e[2 * i] : y.e[2 * i - N]) : x.e[i];
-    T& second = INTERLEAVED ? (i < N / 2 ? x.e[2 * i + 1] : y.e[2 * i - N + 1]) : y.e[i];
-    const float u = load_f<T>(first), v = load_f<T>(second);
-    first = store_f<T>(u * c[i] - v * s[i]);
-    second = store_f<T>(v * c[i] + u * s[i]);
+    float& first = INTERLEAVED ? (i < N / 2 ? x[2 * i] : y[2 * i - N]) : x[i];
+    float& second = INTERLEAVED ? (i < N / 2 ? x[2 * i + 1] : y[2 * i - N + 1]) : y[i];
+    const float u = first, v = second;
+    first = u * c[i] - v * s[i];
+    second = v * c[i] + u * s[i];
   }
+  px = Piece<T>::put(x);
+  py = Piece<T>::put(y);
 }
 
 // CTA per token. A thread keeps one slice of the token's cos / sin row in registers and turns that
 // pair of 16-byte pieces in kHeads heads at a time, all loaded before the first is stored; then the
 // pieces that are copied. Needs 16-byte aligned rows and rotation_dim / 2 a multiple of 16 bytes.
-constexpr int kHeads = 4;
+// A token's work is two dependent rounds of loads (where it goes; its page, angles and rows), so
+// the registers are held to 64: 8 CTAs of an SM run such rounds at once.
+constexpr int kHeads = 3;
 
 template <typename T, bool INTERLEAVED>
-__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(AppendArgs a) {
-  constexpr int N = Pack<T>::N;
+__global__ void __launch_bounds__(kAppendThreads, 8) paged_append_kernel(AppendArgs a) {
+  constexpr int N = Piece<T>::N;
   const uint32_t b = blockIdx.x / (uint32_t)a.rows, t = blockIdx.x - b * (uint32_t)a.rows;
-  const Place p = place_token(a, b, t);
   const int q_heads = a.query != nullptr ? (int)a.q_heads : 0, kv_heads = (int)a.kv_heads, dim = (int)a.dim;
+  const long long live = a.counts != nullptr ? a.counts[b] : a.rows, slot = a.starts[b] + t;
+  const long long position = a.positions != nullptr ? a.positions[b * a.pos_b + t * a.pos_t] : slot;
   const T* q = static_cast<const T*>(a.query) + b * a.qs[0] + t * a.qs[2];
   T* qo = static_cast<T*>(a.query_out) + b * a.os[0] + t * a.os[2];
-  if (p.page < 0) {  // padding: its queries are zeros
+  bool stored = t < live;
+  if (stored && (slot < 0 || slot >= a.table.width * a.table.page_size)) {
+    record_error(a.err, SPECKV_DERR_PAGE_TABLE, slot);
+    stored = false;
+  }
+  if (stored && a.cos != nullptr && (position < 0 || position >= a.rot_positions)) {
+    record_error(a.err, SPECKV_DERR_ROTATION_INDEX, position);
+    stored = false;
+  }
+  const uint32_t size = (uint32_t)a.table.page_size, index = stored ? (uint32_t)slot / size : 0u;
+  const long long page = stored ? a.table.entries[b * a.table.stride + index] : 0;  // checked below
+
+  const int half = a.rot / 2, slices = half / N;  // slices <= 128
+  const T* k = static_cast<const T*>(a.key) + b * a.ks[0] + t * a.ks[2];
+  const T* v = static_cast<const T*>(a.value) + b * a.vs[0] + t * a.vs[2];
+  const int slice = slices > 0 ? threadIdx.x % slices : 0, h0 = slices > 0 ? threadIdx.x / slices : 0;
+  const int step = slices > 0 ? kAppendThreads / slices : 1, heads = slices > 0 && h0 < step ? q_heads + kv_heads : 0;
+  const int x = INTERLEAVED ? 2 * slice * N : slice * N, y = INTERLEAVED ? x + N : x + half;
+  uint4 px[kHeads], py[kHeads];
+  auto load = [&](int h) {
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      const int hi = h + i * step;
+      if (hi < heads) {
+        const T* row = hi < q_heads ? q + hi * a.qs[1] : k + (hi - q_heads) * a.ks[1];
+        px[i] = *reinterpret_cast<const uint4*>(row + x);
+        py[i] = *reinterpret_cast<const uint4*>(row + y);
+      }
+    }
+  };
+  float c[N], s[N];
+  if (stored && heads > 0) {
+    load(h0);
+    const float4* cr = reinterpret_cast<const float4*>(a.cos + position * half + slice * N);
+    const float4* sr = reinterpret_cast<const float4*>(a.sin + position * half + slice * N);
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const float4 cc = __ldg(cr + i), ss = __ldg(sr + i);
+      c[4 * i] = cc.x, c[4 * i + 1] = cc.y, c[4 * i + 2] = cc.z, c[4 * i + 3] = cc.w;
+      s[4 * i] = ss.x, s[4 * i + 1] = ss.y, s[4 * i + 2] = ss.z, s[4 * i + 3] = ss.w;
+    }
+  }
+  if (stored && (page < 0 || page >= a.table.num_pages)) {
+    record_error(a.err, SPECKV_DERR_PAGE_TABLE, page);
+    stored = false;
+  }
+  if (!stored) {  // padding: its queries are zeros
     const int pieces = dim / N;
     for (int i = threadIdx.x; i < q_heads * pieces; i += kAppendThreads)
       *reinterpret_cast<uint4*>(qo + (i / pieces) * a.os[1] + (i % pieces) * N) = make_uint4(0, 0, 0, 0);
     return;
   }
-  const T* k = static_cast<const T*>(a.key) + b * a.ks[0] + t * a.ks[2];
-  const T* v = static_cast<const T*>(a.value) + b * a.vs[0] + t * a.vs[2];
-  T* kp = static_cast<T*>(a.key_pages) + p.page * a.kps[0] + p.row * a.kps[2];
-  T* vp = static_cast<T*>(a.value_pages) + p.page * a.vps[0] + p.row * a.vps[2];
-
-  const int half = a.rot / 2, slices = half / N;  // slices <= 128
-  if (slices > 0) {
-    const int slice = threadIdx.x % slices, h0 = threadIdx.x / slices, step = kAppendThreads / slices;
-    if (h0 < step) {
-      const int x = INTERLEAVED ? 2 * slice * N : slice * N, y = INTERLEAVED ? x + N : x + half;
-      float c[N], s[N];
-      const float4* cr = reinterpret_cast<const float4*>(a.cos + p.position * half + slice * N);
-      const float4* sr = reinterpret_cast<const float4*>(a.sin + p.position * half + slice * N);
+  const long long row = slot - (long long)index * size;
+  T* kp = static_cast<T*>(a.key_pages) + page * a.kps[0] + row * a.kps[2];
+  T* vp = static_cast<T*>(a.value_pages) + page * a.vps[0] + row * a.vps[2];
+  for (int h = h0; h < heads; h += kHeads * step) {
+    if (h != h0) load(h);
 #pragma unroll
-      for (int i = 0; i < N / 4; ++i) {
-        const float4 cc = __ldg(cr + i), ss = __ldg(sr + i);
-        c[4 * i] = cc.x, c[4 * i + 1] = cc.y, c[4 * i + 2] = cc.z, c[4 * i + 3] = cc.w;
-        s[4 * i] = ss.x, s[4 * i + 1] = ss.y, s[4 * i + 2] = ss.z, s[4 * i + 3] = ss.w;
-      }
-      const int heads = q_heads + kv_heads;
-      for (int h = h0; h < heads; h += kHeads * step) {
-        Pack<T> px[kHeads], py[kHeads];
-#pragma unroll
-        for (int i = 0; i < kHeads; ++i) {
-          const int hi = h + i * step;
-          if (hi < heads) {
-            const T* row = hi < q_heads ? q + hi * a.qs[1] : k + (hi - q_heads) * a.ks[1];
-            px[i].raw = *reinterpret_cast<const uint4*>(row + x);
-            py[i].raw = *reinterpret_cast<const uint4*>(row + y);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < kHeads; ++i) {
-          const int hi = h + i * step;
-          if (hi < heads) {
-            T* row = hi < q_heads ? qo + hi * a.os[1] : kp + (hi - q_heads) * a.kps[1];
-            rotate<T, INTERLEAVED>(px[i], py[i], c, s);
-            *reinterpret_cast<uint4*>(row + x) = px[i].raw;
-            *reinterpret_cast<uint4*>(row + y) = py[i].raw;
-          }
-        }
+    for (int i = 0; i < kHeads; ++i) {
+      const int hi = h + i * step;
+      if (hi < heads) {
+        T* to = hi < q_heads ? qo + hi * a.os[1] : kp + (hi - q_heads) * a.kps[1];
+        rotate<T, INTERLEAVED>(px[i], py[i], c, s);
+        *reinterpret_cast<uint4*>(to + x) = px[i];
+        *reinterpret_cast<uint4*>(to + y) = py[i];
       }
     }
   }

@@ -3,6 +3,7 @@
 //   out[b][0][hq][:] = sum_c softmax_c(scale q[b][hq] . k_c) v_c,   c < lengths[b]
 // with k_c / v_c the rows of KV head hq / g (g = q_heads / kv_heads) that the page table names.
 // A sequence of length 0 gives zeros. Scores, softmax statistics and output sums in fp32.
+#include "cluster.cuh"
 #include "paged.cuh"
 
 namespace speckv {
@@ -143,6 +144,8 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint3
 constexpr int kWarps = 4;
 constexpr int kTile = 16 * kWarps;   // keys of a tile: 16 a warp
 constexpr int kMinTiles = 2;         // a CTA's share is at least this many tiles
+constexpr int kCluster = 8;          // CTAs of a cluster at most
+constexpr int kClusterTiles = 8;     // tiles of a cluster's CTA at most
 constexpr float kSlack = 8.f;        // scores may pass the running reference by 2^8 before it moves
 
 // An item is (sequence, KV head, up to 8 NT of its query heads). All items' tiles, in order, are
@@ -156,7 +159,6 @@ struct Join {
 struct PlanArgs {
   float* parts;   // (2 * CTAs) x [8 NT][dim + 2]: sums, reference, total
   Join* joins;    // one per CTA
-  int heads;      // query heads of an item
   int chunks;     // items per (sequence, KV head)
 };
 
@@ -164,18 +166,271 @@ __device__ __forceinline__ long long tiles_of(const PagedArgs& a, long long b) {
   return (live_length(a, b) + kTile - 1) / kTile;
 }
 
+// Shared memory of a CTA: its warps' parts of an item.
+template <int D, int NT> struct Parts {
+  float o[kWarps][8][D + 4];
+  float m[kWarps][8 * NT], l[kWarps][8 * NT];
+};
+
+// One CTA's part of an item: tiles [t0, ...) of its keys up to position `end`. Calls
+// emit(head of the item, dim, sum, reference, total) for each of its heads and dims.
+template <typename T, int D, int NT, bool PAGE16, typename Emit>
+__device__ __forceinline__ void attend_part(const PagedArgs& a, Parts<D, NT>& sm, long long b, int hk, int h0, int heads,
+                                            int t0, long long end, Emit emit) {
+  constexpr int KC = D / 32;  // 16-byte chunks of a key row per lane
+  constexpr int VC = D / 64;  // 16-byte chunks of a value row per lane
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const long long group = a.q_heads / a.kv_heads;
+  const T* kbase = static_cast<const T*>(a.k) + hk * a.ks[1];
+  const T* vbase = static_cast<const T*>(a.v) + hk * a.vs[1];
+  const int64_t* table = a.table.entries + b * a.table.stride;
+  const uint32_t P = (uint32_t)a.table.page_size;
+
+  uint4 kreg[2][KC], vreg[4][VC];
+  uint32_t seen = 0;  // bit 0 / 1: key rows g and g + 8 of the block in kreg are live
+  long long pages = -1;
+  // block i of this warp: keys [16 (4 t0 + warp + 4 i), + 16)
+  const long long key0 = (long long)t0 * kTile + warp * 16;
+  const int count = key0 < end ? (int)((end - key0 + kTile - 1) / kTile) : 0;
+
+  // rows of block i: PAGE16: one page for all; else a page per row
+  long long page = -1;
+  uint32_t row = 0;
+  auto place = [&](int i) {
+    if (PAGE16) {
+      if ((i & 31) == 0) {
+        const long long key = key0 + (long long)(i + lane) * kTile;
+        pages = -1;
+        if (key < end) pages = a.table.page(b, (uint32_t)key / P, a.err);
+      }
+      page = __shfl_sync(0xffffffffu, pages, i & 31);
+      row = (uint32_t)(key0 + (long long)i * kTile) % P;
+    }
+  };
+  auto row_ptr = [&](const T* from, const long long* st, long long key) -> const T* {
+    if (key >= end) return nullptr;
+    const uint32_t index = (uint32_t)key / P;
+    const long long p = a.table.page(b, index, a.err);
+    return p < 0 ? nullptr : from + p * st[0] + (long long)((uint32_t)key - index * P) * st[2];
+  };
+  auto load_k = [&](int i) {
+    const long long key = key0 + (long long)i * kTile;
+    const T* p0;
+    const T* p1;
+    if (PAGE16) {
+      const int live = page < 0 ? 0 : (int)min(16ll, end - key);
+      p0 = kbase + page * a.ks[0] + (long long)(row + g) * a.ks[2];
+      p1 = g + 8 < live ? p0 + 8 * a.ks[2] : nullptr;
+      if (g >= live) p0 = nullptr;
+    } else {
+      p0 = row_ptr(kbase, a.ks, key + g);
+      p1 = row_ptr(kbase, a.ks, key + g + 8);
+    }
+    seen = (p0 != nullptr ? 1u : 0u) | (p1 != nullptr ? 2u : 0u);
+#pragma unroll
+    for (int j = 0; j < KC; ++j) {
+      kreg[0][j] = kreg[1][j] = make_uint4(0, 0, 0, 0);
+      if (p0 != nullptr) kreg[0][j] = load_stream(p0 + (t + 4 * j) * 8);
+      if (p1 != nullptr) kreg[1][j] = load_stream(p1 + (t + 4 * j) * 8);
+    }
+  };
+  auto load_v = [&](int i) {
+    const long long key = key0 + (long long)i * kTile;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int k = 2 * t + (x & 1) + (x >> 1) * 8;  // keys 2t, 2t + 1, 2t + 8, 2t + 9
+      const T* p;
+      if (PAGE16) {
+        const int live = page < 0 ? 0 : (int)min(16ll, end - key);
+        p = k < live ? vbase + page * a.vs[0] + (long long)(row + k) * a.vs[2] : nullptr;
+      } else {
+        p = row_ptr(vbase, a.vs, key + k);
+      }
+#pragma unroll
+      for (int c = 0; c < VC; ++c) {
+        vreg[x][c] = make_uint4(0, 0, 0, 0);  // rows that are not there may hold anything: 0 x NaN is NaN
+        if (p != nullptr) vreg[x][c] = load_stream(p + (g + 8 * c) * 8);
+      }
+    }
+  };
+
+  if (count > 0) {
+    place(0);
+    load_k(0);
+    load_v(0);
+  }
+  // queries as the second operand: lane (g, t) holds head g, the same dims as its key chunks
+  uint4 q[NT][KC];
+#pragma unroll
+  for (int u = 0; u < NT; ++u)
+#pragma unroll
+    for (int j = 0; j < KC; ++j) {
+      q[u][j] = make_uint4(0, 0, 0, 0);
+      if (u * 8 + g < heads) {
+        const T* p = static_cast<const T*>(a.q) + b * a.qs[0] + (hk * group + h0 + u * 8 + g) * a.qs[1] +
+                     (t + 4 * j) * 8;
+        q[u][j] = *reinterpret_cast<const uint4*>(p);
+      }
+    }
+  float o[NT][VC][4][4], m[NT][2], l[NT][2];
+#pragma unroll
+  for (int u = 0; u < NT; ++u) {
+#pragma unroll
+    for (int c = 0; c < VC; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[u][c][i][e] = 0.f;
+    m[u][0] = m[u][1] = -INFINITY;
+    l[u][0] = l[u][1] = 0.f;
+  }
+
+  for (int i = 0; i < count; ++i) {
+    // scores of 16 keys x 8 heads: rows keys g, g + 8, columns heads 2t, 2t + 1
+    float s[NT][4];
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      float s2[4] = {0.f, 0.f, 0.f, 0.f};
+      s[u][0] = s[u][1] = s[u][2] = s[u][3] = 0.f;
+#pragma unroll
+      for (int j = 0; j < KC; ++j) {
+        mma(s[u], kreg[0][j].x, kreg[1][j].x, kreg[0][j].y, kreg[1][j].y, q[u][j].x, q[u][j].y, T());
+        mma(s2, kreg[0][j].z, kreg[1][j].z, kreg[0][j].w, kreg[1][j].w, q[u][j].z, q[u][j].w, T());
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[u][e] = (s[u][e] + s2[e]) * a.scale_log2;
+        if (!(seen >> (e >> 1) & 1u)) s[u][e] = -INFINITY;
+      }
+    }
+    if (i + 1 < count) {
+      place(i + 1);
+      load_k(i + 1);
+    }
+    uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      float t0m = fmaxf(s[u][0], s[u][2]), t1m = fmaxf(s[u][1], s[u][3]);
+      // The reference need not be the maximum: any value within 2^8 of it keeps every weight and
+      // sum well inside fp32, and the sums are divided by the total at the end. So it moves only
+      // when a score passes it by more than that (the first block moves it from -inf).
+      if (__any_sync(0xffffffffu, t0m > m[u][0] + kSlack || t1m > m[u][1] + kSlack)) {
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) {
+          t0m = fmaxf(t0m, __shfl_xor_sync(0xffffffffu, t0m, off));
+          t1m = fmaxf(t1m, __shfl_xor_sync(0xffffffffu, t1m, off));
+        }
+        const float n0 = fmaxf(m[u][0], t0m), n1 = fmaxf(m[u][1], t1m);
+        const float f0 = n0 == -INFINITY ? 1.f : exp2f(m[u][0] - n0);
+        const float f1 = n1 == -INFINITY ? 1.f : exp2f(m[u][1] - n1);
+        m[u][0] = n0;
+        m[u][1] = n1;
+        l[u][0] *= f0;
+        l[u][1] *= f1;
+#pragma unroll
+        for (int c = 0; c < VC; ++c)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            o[u][c][x][0] *= f0;
+            o[u][c][x][1] *= f1;
+            o[u][c][x][2] *= f0;
+            o[u][c][x][3] *= f1;
+          }
+      }
+      const float r0 = m[u][0] == -INFINITY ? 0.f : m[u][0], r1 = m[u][1] == -INFINITY ? 0.f : m[u][1];
+      const float p0 = exp2f(s[u][0] - r0), p1 = exp2f(s[u][1] - r1), p2 = exp2f(s[u][2] - r0),
+                  p3 = exp2f(s[u][3] - r1);
+      l[u][0] += p0 + p2;
+      l[u][1] += p1 + p3;
+      // weights to (key pairs, heads) fragments, in two 16-bit parts: the tensor pipe has room
+      // for a second product, and one 8-bit weight alone would lose more than the output's rounding
+      split_pair(p0, p1, ph[u][0], pl[u][0], T());
+      split_pair(p2, p3, ph[u][1], pl[u][1], T());
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        ph[u][x] = transpose8(ph[u][x]);
+        pl[u][x] = transpose8(pl[u][x]);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < VC; ++c)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const uint32_t v0 = (&vreg[0][c].x)[x], v1 = (&vreg[1][c].x)[x];
+        const uint32_t v2 = (&vreg[2][c].x)[x], v3 = (&vreg[3][c].x)[x];
+        // pairs of keys of one dim: dims 2x (row g) and 2x + 1 (row g + 8) of the lane's chunk
+        const uint32_t a0 = __byte_perm(v0, v1, 0x5410), a1 = __byte_perm(v0, v1, 0x7632);
+        const uint32_t a2 = __byte_perm(v2, v3, 0x5410), a3 = __byte_perm(v2, v3, 0x7632);
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          mma(o[u][c][x], a0, a1, a2, a3, ph[u][0], ph[u][1], T());
+          mma(o[u][c][x], a0, a1, a2, a3, pl[u][0], pl[u][1], T());
+        }
+      }
+    if (i + 1 < count) load_v(i + 1);
+  }
+
+
+  // the warps' parts, joined
+#pragma unroll
+  for (int u = 0; u < NT; ++u)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) l[u][e] += __shfl_xor_sync(0xffffffffu, l[u][e], off);
+      if (g == 0) {
+        sm.m[warp][u * 8 + 2 * t + e] = m[u][e];
+        sm.l[warp][u * 8 + 2 * t + e] = l[u][e];
+      }
+    }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < NT; ++u) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int head = u * 8 + 2 * t + e;
+      float top = sm.m[0][head];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm.m[w][head]);
+      const float f = top == -INFINITY ? 1.f : exp2f(m[u][e] - top);
+#pragma unroll
+      for (int c = 0; c < VC; ++c) {
+        float* to = &sm.o[warp][2 * t + e][(g + 8 * c) * 8];
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          *reinterpret_cast<float2*>(to + 2 * x) = make_float2(o[u][c][x][e] * f, o[u][c][x][2 + e] * f);
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 8 * D; i += kWarps * 32) {
+      const int head = i / D, d = i - head * D;
+      if (u * 8 + head >= heads) break;
+      float top = sm.m[0][u * 8 + head];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm.m[w][u * 8 + head]);
+      const float ref = top == -INFINITY ? 0.f : top;
+      float sum = 0.f, all = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        sum += sm.o[w][head][d];
+        all = fmaf(sm.l[w][u * 8 + head], exp2f(sm.m[w][u * 8 + head] - ref), all);
+      }
+      emit(u * 8 + head, d, sum, top, all);
+    }
+    __syncthreads();
+  }
+}
+
+// CTAs per SM of the tensor-core kernels.
+template <int D, int NT> constexpr int resident() { return D == 64 ? (NT == 1 ? 4 : 3) : D == 128 ? (NT == 1 ? 3 : 2) : 2; }
+
 template <typename T, int D, int NT, bool PAGE16>
-__global__ void __launch_bounds__(kWarps * 32, D == 64 ? (NT == 1 ? 4 : 3) : D == 128 ? (NT == 1 ? 3 : 2) : 2)
-    paged_attention_mma_kernel(PagedArgs a, PlanArgs plan) {
-  constexpr int KC = D / 32;       // 16-byte chunks of a key row per lane
-  constexpr int VC = D / 64;       // 16-byte chunks of a value row per lane
-  constexpr int PAD = D + 4;
+__global__ void __launch_bounds__(kWarps * 32, resident<D, NT>()) paged_attention_mma_kernel(PagedArgs a, PlanArgs plan) {
   constexpr int PART = 8 * NT * (D + 2);
   asm volatile("griddepcontrol.launch_dependents;");
-  __shared__ float s_o[kWarps][8][PAD];
-  __shared__ float s_m[kWarps][8 * NT], s_l[kWarps][8 * NT];
+  __shared__ Parts<D, NT> sm;
   __shared__ long long s_scan[kWarps], s_find[2];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long group = a.q_heads / a.kv_heads, per_seq = a.kv_heads * plan.chunks;
   const int G = gridDim.x, cta = blockIdx.x;
 
@@ -243,207 +498,6 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? (NT == 1 ? 4 : 3) : D =
     const int heads = min((int)group - h0, 8 * NT);
     const long long end = min(n, (long long)t1 * kTile);
 
-    const T* kbase = static_cast<const T*>(a.k) + hk * a.ks[1];
-    const T* vbase = static_cast<const T*>(a.v) + hk * a.vs[1];
-    const int64_t* table = a.table.entries + b * a.table.stride;
-    const uint32_t P = (uint32_t)a.table.page_size;
-
-    uint4 kreg[2][KC], vreg[4][VC];
-    uint32_t seen = 0;  // bit 0 / 1: key rows g and g + 8 of the block in kreg are live
-    long long pages = -1;
-    // block i of this warp: keys [16 (4 t0 + warp + 4 i), + 16)
-    const long long key0 = (long long)t0 * kTile + warp * 16;
-    const int count = key0 < end ? (int)((end - key0 + kTile - 1) / kTile) : 0;
-
-    // rows of block i: PAGE16: one page for all; else a page per row
-    long long page = -1;
-    uint32_t row = 0;
-    auto place = [&](int i) {
-      if (PAGE16) {
-        if ((i & 31) == 0) {
-          const long long key = key0 + (long long)(i + lane) * kTile;
-          pages = -1;
-          if (key < end) pages = a.table.page(b, (uint32_t)key / P, a.err);
-        }
-        page = __shfl_sync(0xffffffffu, pages, i & 31);
-        row = (uint32_t)(key0 + (long long)i * kTile) % P;
-      }
-    };
-    auto row_ptr = [&](const T* from, const long long* st, long long key) -> const T* {
-      if (key >= end) return nullptr;
-      const uint32_t index = (uint32_t)key / P;
-      const long long p = a.table.page(b, index, a.err);
-      return p < 0 ? nullptr : from + p * st[0] + (long long)((uint32_t)key - index * P) * st[2];
-    };
-    auto load_k = [&](int i) {
-      const long long key = key0 + (long long)i * kTile;
-      const T* p0;
-      const T* p1;
-      if (PAGE16) {
-        const int live = page < 0 ? 0 : (int)min(16ll, end - key);
-        p0 = kbase + page * a.ks[0] + (long long)(row + g) * a.ks[2];
-        p1 = g + 8 < live ? p0 + 8 * a.ks[2] : nullptr;
-        if (g >= live) p0 = nullptr;
-      } else {
-        p0 = row_ptr(kbase, a.ks, key + g);
-        p1 = row_ptr(kbase, a.ks, key + g + 8);
-      }
-      seen = (p0 != nullptr ? 1u : 0u) | (p1 != nullptr ? 2u : 0u);
-#pragma unroll
-      for (int j = 0; j < KC; ++j) {
-        kreg[0][j] = kreg[1][j] = make_uint4(0, 0, 0, 0);
-        if (p0 != nullptr) kreg[0][j] = load_stream(p0 + (t + 4 * j) * 8);
-        if (p1 != nullptr) kreg[1][j] = load_stream(p1 + (t + 4 * j) * 8);
-      }
-    };
-    auto load_v = [&](int i) {
-      const long long key = key0 + (long long)i * kTile;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int k = 2 * t + (x & 1) + (x >> 1) * 8;  // keys 2t, 2t + 1, 2t + 8, 2t + 9
-        const T* p;
-        if (PAGE16) {
-          const int live = page < 0 ? 0 : (int)min(16ll, end - key);
-          p = k < live ? vbase + page * a.vs[0] + (long long)(row + k) * a.vs[2] : nullptr;
-        } else {
-          p = row_ptr(vbase, a.vs, key + k);
-        }
-#pragma unroll
-        for (int c = 0; c < VC; ++c) {
-          vreg[x][c] = make_uint4(0, 0, 0, 0);  // rows that are not there may hold anything: 0 x NaN is NaN
-          if (p != nullptr) vreg[x][c] = load_stream(p + (g + 8 * c) * 8);
-        }
-      }
-    };
-
-    if (count > 0) {
-      place(0);
-      load_k(0);
-      load_v(0);
-    }
-    // queries as the second operand: lane (g, t) holds head g, the same dims as its key chunks
-    uint4 q[NT][KC];
-#pragma unroll
-    for (int u = 0; u < NT; ++u)
-#pragma unroll
-      for (int j = 0; j < KC; ++j) {
-        q[u][j] = make_uint4(0, 0, 0, 0);
-        if (u * 8 + g < heads) {
-          const T* p = static_cast<const T*>(a.q) + b * a.qs[0] + (hk * group + h0 + u * 8 + g) * a.qs[1] +
-                       (t + 4 * j) * 8;
-          q[u][j] = *reinterpret_cast<const uint4*>(p);
-        }
-      }
-    float o[NT][VC][4][4], m[NT][2], l[NT][2];
-#pragma unroll
-    for (int u = 0; u < NT; ++u) {
-#pragma unroll
-      for (int c = 0; c < VC; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[u][c][i][e] = 0.f;
-      m[u][0] = m[u][1] = -INFINITY;
-      l[u][0] = l[u][1] = 0.f;
-    }
-
-    for (int i = 0; i < count; ++i) {
-      // scores of 16 keys x 8 heads: rows keys g, g + 8, columns heads 2t, 2t + 1
-      float s[NT][4];
-#pragma unroll
-      for (int u = 0; u < NT; ++u) {
-        float s2[4] = {0.f, 0.f, 0.f, 0.f};
-        s[u][0] = s[u][1] = s[u][2] = s[u][3] = 0.f;
-#pragma unroll
-        for (int j = 0; j < KC; ++j) {
-          mma(s[u], kreg[0][j].x, kreg[1][j].x, kreg[0][j].y, kreg[1][j].y, q[u][j].x, q[u][j].y, T());
-          mma(s2, kreg[0][j].z, kreg[1][j].z, kreg[0][j].w, kreg[1][j].w, q[u][j].z, q[u][j].w, T());
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[u][e] = (s[u][e] + s2[e]) * a.scale_log2;
-          if (!(seen >> (e >> 1) & 1u)) s[u][e] = -INFINITY;
-        }
-      }
-      if (i + 1 < count) {
-        place(i + 1);
-        load_k(i + 1);
-      }
-      uint32_t ph[NT][2], pl[NT][2];
-#pragma unroll
-      for (int u = 0; u < NT; ++u) {
-        float t0m = fmaxf(s[u][0], s[u][2]), t1m = fmaxf(s[u][1], s[u][3]);
-        // The reference need not be the maximum: any value within 2^8 of it keeps every weight and
-        // sum well inside fp32, and the sums are divided by the total at the end. So it moves only
-        // when a score passes it by more than that (the first block moves it from -inf).
-        if (__any_sync(0xffffffffu, t0m > m[u][0] + kSlack || t1m > m[u][1] + kSlack)) {
-#pragma unroll
-          for (int off = 4; off < 32; off <<= 1) {
-            t0m = fmaxf(t0m, __shfl_xor_sync(0xffffffffu, t0m, off));
-            t1m = fmaxf(t1m, __shfl_xor_sync(0xffffffffu, t1m, off));
-          }
-          const float n0 = fmaxf(m[u][0], t0m), n1 = fmaxf(m[u][1], t1m);
-          const float f0 = n0 == -INFINITY ? 1.f : exp2f(m[u][0] - n0);
-          const float f1 = n1 == -INFINITY ? 1.f : exp2f(m[u][1] - n1);
-          m[u][0] = n0;
-          m[u][1] = n1;
-          l[u][0] *= f0;
-          l[u][1] *= f1;
-#pragma unroll
-          for (int c = 0; c < VC; ++c)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              o[u][c][x][0] *= f0;
-              o[u][c][x][1] *= f1;
-              o[u][c][x][2] *= f0;
-              o[u][c][x][3] *= f1;
-            }
-        }
-        const float r0 = m[u][0] == -INFINITY ? 0.f : m[u][0], r1 = m[u][1] == -INFINITY ? 0.f : m[u][1];
-        const float p0 = exp2f(s[u][0] - r0), p1 = exp2f(s[u][1] - r1), p2 = exp2f(s[u][2] - r0),
-                    p3 = exp2f(s[u][3] - r1);
-        l[u][0] += p0 + p2;
-        l[u][1] += p1 + p3;
-        // weights to (key pairs, heads) fragments, in two 16-bit parts: the tensor pipe has room
-        // for a second product, and one 8-bit weight alone would lose more than the output's rounding
-        split_pair(p0, p1, ph[u][0], pl[u][0], T());
-        split_pair(p2, p3, ph[u][1], pl[u][1], T());
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          ph[u][x] = transpose8(ph[u][x]);
-          pl[u][x] = transpose8(pl[u][x]);
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < VC; ++c)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const uint32_t v0 = (&vreg[0][c].x)[x], v1 = (&vreg[1][c].x)[x];
-          const uint32_t v2 = (&vreg[2][c].x)[x], v3 = (&vreg[3][c].x)[x];
-          // pairs of keys of one dim: dims 2x (row g) and 2x + 1 (row g + 8) of the lane's chunk
-          const uint32_t a0 = __byte_perm(v0, v1, 0x5410), a1 = __byte_perm(v0, v1, 0x7632);
-          const uint32_t a2 = __byte_perm(v2, v3, 0x5410), a3 = __byte_perm(v2, v3, 0x7632);
-#pragma unroll
-          for (int u = 0; u < NT; ++u) {
-            mma(o[u][c][x], a0, a1, a2, a3, ph[u][0], ph[u][1], T());
-            mma(o[u][c][x], a0, a1, a2, a3, pl[u][0], pl[u][1], T());
-          }
-        }
-      if (i + 1 < count) load_v(i + 1);
-    }
-
-    // the warps' parts of the item
-#pragma unroll
-    for (int u = 0; u < NT; ++u)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-#pragma unroll
-        for (int off = 4; off < 32; off <<= 1) l[u][e] += __shfl_xor_sync(0xffffffffu, l[u][e], off);
-        if (g == 0) {
-          s_m[warp][u * 8 + 2 * t + e] = m[u][e];
-          s_l[warp][u * 8 + 2 * t + e] = l[u][e];
-        }
-      }
     const bool whole = t0 == 0 && t1 == nb;
     const int slot = 2 * cta + (first_segment ? 0 : 1);
     float* part = plan.parts + (long long)slot * PART;
@@ -451,55 +505,75 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? (NT == 1 ? 4 : 3) : D =
       const long long last = ((item + nb) * shares - 1) / total;  // the share that holds the item's last tile
       join = Join{(int)b, h, slot, (int)(last - cta) + 1};
     }
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < NT; ++u) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int head = u * 8 + 2 * t + e;
-        float top = s_m[0][head];
-#pragma unroll
-        for (int w = 1; w < kWarps; ++w) top = fmaxf(top, s_m[w][head]);
-        const float f = top == -INFINITY ? 1.f : exp2f(m[u][e] - top);
-#pragma unroll
-        for (int c = 0; c < VC; ++c) {
-          float* to = &s_o[warp][2 * t + e][(g + 8 * c) * 8];
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            *reinterpret_cast<float2*>(to + 2 * x) = make_float2(o[u][c][x][e] * f, o[u][c][x][2 + e] * f);
+    T* out = static_cast<T*>(a.out) + (b * a.q_heads + hk * group + h0) * D;
+    attend_part<T, D, NT, PAGE16>(a, sm, b, hk, h0, heads, t0, end, [&](int head, int d, float sum, float top, float all) {
+      if (whole) {
+        out[head * D + d] = store_f<T>(all == 0.f ? 0.f : sum / all);
+      } else {
+        part[head * D + d] = sum;
+        if (d == 0) {
+          part[8 * NT * D + head] = top;
+          part[8 * NT * (D + 1) + head] = all;
         }
       }
-      __syncthreads();
-      for (int i = threadIdx.x; i < 8 * D; i += kWarps * 32) {
-        const int head = i / D, d = i - head * D;
-        if (u * 8 + head >= heads) break;
-        float top = s_m[0][u * 8 + head];
-#pragma unroll
-        for (int w = 1; w < kWarps; ++w) top = fmaxf(top, s_m[w][u * 8 + head]);
-        const float ref = top == -INFINITY ? 0.f : top;
-        float sum = 0.f, all = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          sum += s_o[w][head][d];
-          all = fmaf(s_l[w][u * 8 + head], exp2f(s_m[w][u * 8 + head] - ref), all);
-        }
-        if (whole) {
-          static_cast<T*>(a.out)[(b * a.q_heads + hk * group + h0 + u * 8 + head) * D + d] =
-              store_f<T>(all == 0.f ? 0.f : sum / all);
-        } else {
-          part[(u * 8 + head) * D + d] = sum;
-          if (d == 0) {
-            part[8 * NT * D + u * 8 + head] = top;
-            part[8 * NT * (D + 1) + u * 8 + head] = all;
-          }
-        }
-      }
-      __syncthreads();
-    }
+    });
     at = item + t1;
     first_segment = false;
   }
   if (threadIdx.x == 0) plan.joins[cta] = join;
+}
+
+// Few items: a cluster of CTAs each, an equal run of its tiles per CTA, joined through the
+// cluster's shared memory. One launch, no workspace.
+template <typename T, int D, int NT, bool PAGE16>
+__global__ void __launch_bounds__(kWarps * 32, resident<D, NT>())
+    paged_attention_cluster_kernel(PagedArgs a, PlanArgs plan) {
+  __shared__ Parts<D, NT> sm;
+  __shared__ float s_sum[8 * NT][D], s_top[8 * NT], s_all[8 * NT];
+  const uint32_t ctas = cluster_size(), rank = cluster_rank();
+  const long long group = a.q_heads / a.kv_heads, per_seq = a.kv_heads * plan.chunks;
+  const uint32_t index = blockIdx.x / ctas;
+  const long long b = index / (uint32_t)per_seq;
+  const int h = (int)(index - b * per_seq);
+  const int hk = h / plan.chunks, h0 = (h - hk * plan.chunks) * 8 * NT, heads = min((int)group - h0, 8 * NT);
+  const long long n = live_length(a, b), nb = (n + kTile - 1) / kTile;
+  const int t0 = (int)(nb * rank / ctas), t1 = (int)(nb * (rank + 1) / ctas);
+  attend_part<T, D, NT, PAGE16>(a, sm, b, hk, h0, heads, t0, min(n, (long long)t1 * kTile),
+                                [&](int head, int d, float sum, float top, float all) {
+                                  s_sum[head][d] = sum;
+                                  if (d == 0) {
+                                    s_top[head] = top;
+                                    s_all[head] = all;
+                                  }
+                                });
+  cluster_sync();
+  // each CTA joins its share of the outputs
+  T* out = static_cast<T*>(a.out) + (b * a.q_heads + hk * group + h0) * D;
+  for (int i = rank * kWarps * 32 + threadIdx.x; i < heads * D; i += ctas * kWarps * 32) {
+    const int head = i / D, d = i - head * D;
+    float top[kCluster], all[kCluster], sum[kCluster], ref = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < kCluster; ++r)
+      if (r < ctas) {
+        top[r] = remote_float(&s_top[head], r);
+        all[r] = remote_float(&s_all[head], r);
+        sum[r] = remote_float(&s_sum[head][d], r);
+      }
+#pragma unroll
+    for (int r = 0; r < kCluster; ++r)
+      if (r < ctas) ref = fmaxf(ref, top[r]);
+    if (ref == -INFINITY) ref = 0.f;
+    float o = 0.f, total = 0.f;
+#pragma unroll
+    for (int r = 0; r < kCluster; ++r)
+      if (r < ctas) {
+        const float f = exp2f(top[r] - ref);
+        total = fmaf(all[r], f, total);
+        o = fmaf(sum[r], f, o);
+      }
+    out[i] = store_f<T>(total == 0.f ? 0.f : o / total);
+  }
+  cluster_sync();  // the other CTAs' shared memory is read until here
 }
 
 // Joins the parts of the items that more than one share holds, in the order of the shares: CTA per
@@ -585,8 +659,10 @@ int sm_count() {
   return counts[dev];
 }
 
-// CTAs per SM the tensor-core kernel is compiled for.
-int ctas_per_sm(int64_t dim, int nt) { return dim == 64 ? (nt == 1 ? 4 : 3) : dim == 128 ? (nt == 1 ? 3 : 2) : 2; }
+int ctas_per_sm(int64_t dim, int nt) {
+  return dim == 64 ? (nt == 1 ? resident<64, 1>() : resident<64, 2>())
+                   : dim == 128 ? (nt == 1 ? resident<128, 1>() : resident<128, 2>()) : resident<256, 1>();
+}
 
 // Query heads of an item: the tensor instruction takes 8, two of them share the key and value
 // registers where those leave room (head dims to 128).
@@ -596,14 +672,36 @@ bool tensor_shape(int64_t dim, int32_t dtype) {
   return dtype != SPECKV_F32 && (dim == 64 || dim == 128 || dim == 256);
 }
 
-int64_t workspace_bytes(int64_t q_heads, int64_t kv_heads, int64_t dim, int32_t dtype, int sms) {
-  if (!tensor_shape(dim, dtype)) return 0;
-  const int nt = head_tiles(dim, q_heads / kv_heads), ctas = sms * ctas_per_sm(dim, nt);
-  return (int64_t)ctas * (2 * 8 * nt * (dim + 2) * sizeof(float) + sizeof(Join));
+// CTAs of a cluster per item, 0 for equal shares: clusters where they all run at once and the
+// longest sequence that the table can hold leaves each CTA few tiles.
+int cluster_ctas(long long items, long long tiles, int full) {
+  int ctas = 1;
+  while (ctas < kCluster && ctas < tiles && items * ctas * 2 <= full) ctas *= 2;
+  return items * ctas <= full && tiles <= (long long)ctas * kClusterTiles ? ctas : 0;
+}
+
+// How a tensor shape is launched, from sizes that the host knows.
+struct Launch {
+  int tiles8, chunks, full, cluster;  // NT; items per (sequence, KV head); CTAs resident; CTAs per item or 0
+  long long items, tiles;             // tiles of the longest sequence that the table can hold
+  int64_t workspace;
+};
+
+Launch plan_launch(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t positions, int sms) {
+  Launch l;
+  const int64_t group = q_heads / kv_heads;
+  l.tiles8 = head_tiles(dim, group);
+  l.chunks = (int)((group + 8 * l.tiles8 - 1) / (8 * l.tiles8));
+  l.full = sms * ctas_per_sm(dim, l.tiles8);
+  l.items = batch * kv_heads * l.chunks;
+  l.tiles = (positions + kTile - 1) / kTile;
+  l.cluster = cluster_ctas(l.items, l.tiles, l.full);
+  l.workspace = l.cluster > 0 ? 0 : (int64_t)l.full * (2 * 8 * l.tiles8 * (dim + 2) * sizeof(float) + sizeof(Join));
+  return l;
 }
 
 template <typename T, int D, int NT>
-int launch_mma(const PagedArgs& a, const PlanArgs& plan, int ctas, cudaStream_t s) {
+int launch_shares(const PagedArgs& a, const PlanArgs& plan, int ctas, cudaStream_t s) {
   if (a.table.page_size % 16 == 0)
     paged_attention_mma_kernel<T, D, NT, true><<<ctas, kWarps * 32, 0, s>>>(a, plan);
   else
@@ -615,7 +713,7 @@ int launch_mma(const PagedArgs& a, const PlanArgs& plan, int ctas, cudaStream_t 
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas, (unsigned)min((int)(a.q_heads / a.kv_heads), plan.heads));
+  cfg.gridDim = dim3(ctas, (unsigned)min((int)(a.q_heads / a.kv_heads), 8 * NT));
   cfg.blockDim = dim3(128);
   cfg.stream = s;
   cfg.attrs = &attr;
@@ -623,6 +721,37 @@ int launch_mma(const PagedArgs& a, const PlanArgs& plan, int ctas, cudaStream_t 
   const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<T, D, NT>, a, plan);
   if (e != cudaSuccess) return fail(SPECKV_ECUDA, "speckv_paged_attention: launch failed: %s", cudaGetErrorString(e));
   return SPECKV_OK;
+}
+
+template <typename T, int D, int NT>
+int launch_clusters(const PagedArgs& a, const PlanArgs& plan, int items, int ctas, cudaStream_t s) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ctas;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(items * ctas));
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = a.table.page_size % 16 == 0
+                            ? cudaLaunchKernelEx(&cfg, paged_attention_cluster_kernel<T, D, NT, true>, a, plan)
+                            : cudaLaunchKernelEx(&cfg, paged_attention_cluster_kernel<T, D, NT, false>, a, plan);
+  if (e != cudaSuccess) return fail(SPECKV_ECUDA, "speckv_paged_attention: launch failed: %s", cudaGetErrorString(e));
+  return SPECKV_OK;
+}
+
+template <typename T, int D, int NT>
+int launch_tensor(const PagedArgs& a, const Launch& l, void* workspace, cudaStream_t s) {
+  PlanArgs plan;
+  plan.chunks = l.chunks;
+  plan.joins = static_cast<Join*>(workspace);
+  plan.parts = reinterpret_cast<float*>(plan.joins + l.full);
+  if (l.cluster > 0) return launch_clusters<T, D, NT>(a, plan, (int)l.items, l.cluster, s);
+  // no more CTAs than shares of the longest sequences possible
+  const double most = (double)l.items * (double)l.tiles / kMinTiles;
+  return launch_shares<T, D, NT>(a, plan, most < l.full ? (int)most + 1 : l.full, s);
 }
 
 template <typename T>
@@ -640,26 +769,16 @@ int launch_paged(const PagedArgs& a, int32_t dtype, void* workspace, int64_t byt
   }
   if constexpr (sizeof(T) == 2) {
     const int sms = sm_count();
-    const int64_t group = a.q_heads / a.kv_heads;
-    const int nt = head_tiles(a.dim, group);
-    // no more CTAs than shares of the longest lengths that the table can hold
-    const double most = (double)a.batch * a.kv_heads * ((group + 8 * nt - 1) / (8 * nt)) *
-                        ((a.table.width * a.table.page_size + kTile - 1) / kTile);
-    const int full = sms * ctas_per_sm(a.dim, nt), ctas = most < (double)full * kMinTiles ? (int)((most + kMinTiles - 1) / kMinTiles) : full;
-    const int64_t need = workspace_bytes(a.q_heads, a.kv_heads, a.dim, dtype, sms);
     if (sms == 0) return fail(SPECKV_ECUDA, "speckv_paged_attention: no SM count");
-    if (workspace == nullptr || bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)
+    const Launch l = plan_launch(a.batch, a.q_heads, a.kv_heads, a.dim, a.table.width * a.table.page_size, sms);
+    if (l.workspace > 0 && (workspace == nullptr || bytes < l.workspace || reinterpret_cast<uintptr_t>(workspace) % 16))
       return fail(SPECKV_EINVAL, "speckv_paged_attention: workspace of %lld bytes, %lld needed (16-byte aligned)",
-                  (long long)bytes, (long long)need);
-    PlanArgs plan;
-    plan.joins = static_cast<Join*>(workspace);
-    plan.parts = reinterpret_cast<float*>(plan.joins + full);
-    plan.heads = 8 * nt;
-    plan.chunks = (int)((group + plan.heads - 1) / plan.heads);
-    if (a.dim == 64) return nt == 1 ? launch_mma<T, 64, 1>(a, plan, ctas, s) : launch_mma<T, 64, 2>(a, plan, ctas, s);
+                  (long long)bytes, (long long)l.workspace);
+    if (a.dim == 64)
+      return l.tiles8 == 1 ? launch_tensor<T, 64, 1>(a, l, workspace, s) : launch_tensor<T, 64, 2>(a, l, workspace, s);
     if (a.dim == 128)
-      return nt == 1 ? launch_mma<T, 128, 1>(a, plan, ctas, s) : launch_mma<T, 128, 2>(a, plan, ctas, s);
-    return launch_mma<T, 256, 1>(a, plan, ctas, s);
+      return l.tiles8 == 1 ? launch_tensor<T, 128, 1>(a, l, workspace, s) : launch_tensor<T, 128, 2>(a, l, workspace, s);
+    return launch_tensor<T, 256, 1>(a, l, workspace, s);
   }
   return SPECKV_OK;
 }
@@ -720,7 +839,10 @@ extern "C" int speckv_paged_attention(const void* query, const void* key_pages, 
   }
 }
 
-extern "C" int64_t speckv_paged_attention_workspace(int64_t q_heads, int64_t kv_heads, int64_t dim, int32_t dtype) {
-  if (q_heads < 1 || kv_heads < 1 || q_heads % kv_heads != 0) return 0;
-  return workspace_bytes(q_heads, kv_heads, dim, dtype, sm_count());
+extern "C" int64_t speckv_paged_attention_workspace(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim,
+                                                    int64_t table_pages, int64_t page_size, int32_t dtype) {
+  if (batch < 1 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads != 0 || table_pages < 1 || page_size < 1 ||
+      table_pages > (1ll << 31) / page_size || !tensor_shape(dim, dtype))
+    return 0;
+  return plan_launch(batch, q_heads, kv_heads, dim, table_pages * page_size, sm_count()).workspace;
 }

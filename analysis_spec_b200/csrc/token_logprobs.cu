@@ -9,6 +9,7 @@
 // Statistics in fp32 whatever the logits' type. A row whose token (or source row) is negative is
 // skipped: not read, zeros out, ids -1, gradient 0. A row of -inf alone has nothing to choose
 // from: logprob -inf, entropy 0, gradient 0. NaN or +inf in a row makes its numbers NaN.
+#include "cluster.cuh"
 #include "paged.cuh"
 
 namespace speckv {
@@ -327,36 +328,6 @@ __device__ __forceinline__ void join_sums(float& r, float& s, float& t, float r2
   r = to;
 }
 
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t n;
-  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
-  return n;
-}
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t n;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(n));
-  return n;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// Address of CTA `rank`'s copy of a shared variable.
-__device__ __forceinline__ uint32_t remote(const void* p, uint32_t rank) {
-  uint32_t local = (uint32_t)__cvta_generic_to_shared(p), at;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(local), "r"(rank));
-  return at;
-}
-__device__ __forceinline__ float remote_float(const void* p, uint32_t rank) {
-  float x;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(remote(p, rank)) : "memory");
-  return x;
-}
-__device__ __forceinline__ unsigned long long remote_u64(const void* p, uint32_t rank) {
-  unsigned long long x;
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(x) : "r"(remote(p, rank)) : "memory");
-  return x;
-}
-
 __device__ __forceinline__ void write_skipped(const ScoreArgs& a, long long n) {
   if (threadIdx.x == 0) {
     if (a.logprobs != nullptr) a.logprobs[n] = 0.f;
@@ -619,10 +590,22 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
     }
     cluster_sync();
     if (rank == 0) {
-      for (uint32_t o = 1; o < ctas; ++o) {
-        join_sums(r, s, t, remote_float(&s_part[0], o), remote_float(&s_part[1], o), remote_float(&s_part[2], o), c);
-        bad |= __float_as_int(remote_float(&s_bad, o)) != 0;
-      }
+      float r2[8], s2[8], t2[8];
+      int bad2[8];
+#pragma unroll
+      for (uint32_t o = 1; o < 8; ++o)
+        if (o < ctas) {
+          r2[o] = remote_float(&s_part[0], o);
+          s2[o] = remote_float(&s_part[1], o);
+          t2[o] = remote_float(&s_part[2], o);
+          bad2[o] = __float_as_int(remote_float(&s_bad, o));
+        }
+#pragma unroll
+      for (uint32_t o = 1; o < 8; ++o)
+        if (o < ctas) {
+          join_sums(r, s, t, r2[o], s2[o], t2[o], c);
+          bad |= bad2[o] != 0;
+        }
     }
   }
   if (rank == 0) {

@@ -585,7 +585,7 @@ int speckv_paged_append(const void* key, const void* value, const void* query, v
  * 256: 64, 128 and 256 in bf16 / fp16 with 16-byte aligned rows take the tensor-core kernel, which
  * cuts the live positions of all sequences into equal shares and joins what is cut, other views a
  * CUDA-core kernel. workspace (16-byte aligned, workspace_bytes at least
- * speckv_paged_attention_workspace of the same shape on the same device; it holds nothing between
+ * speckv_paged_attention_workspace of the same sizes on the same device; it holds nothing between
  * calls) may be shared by calls that cannot run at the same time. */
 int speckv_paged_attention(const void* query, const void* key_pages, const void* value_pages, const int64_t* strides,
                            const int64_t* page_table, int64_t table_stride, int64_t table_pages, int64_t num_pages,
@@ -593,9 +593,10 @@ int speckv_paged_attention(const void* query, const void* key_pages, const void*
                            int64_t kv_heads, int64_t dim, float scale, int32_t dtype, void* workspace,
                            int64_t workspace_bytes, void* stream);
 
-/* Workspace bytes of speckv_paged_attention on the current device, whatever the batch and lengths
- * (0 for a shape that needs none). */
-int64_t speckv_paged_attention_workspace(int64_t q_heads, int64_t kv_heads, int64_t dim, int32_t dtype);
+/* Workspace bytes of speckv_paged_attention on the current device, whatever the lengths (0 for a
+ * call that needs none: few sequences of short tables, and the CUDA-core kernel's shapes). */
+int64_t speckv_paged_attention_workspace(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim,
+                                         int64_t table_pages, int64_t page_size, int32_t dtype);
 
 /* ---- Log-probabilities of tokens ------------------------------------------ */
 

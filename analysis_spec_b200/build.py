@@ -84,7 +84,7 @@ def build_front(force=False, verbose=False):
            f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}', '-isystem', str(include), '-isystem',
            str(include / 'torch' / 'csrc' / 'api' / 'include'), '-isystem', str(Path(NVCC).parent.parent / 'include'),
            '-isystem', sysconfig.get_paths()['include'], str(src), '-o', str(FRONT.with_suffix('.so.tmp')),
-           f'-L{libdir}', '-lc10', '-lc10_cuda', '-ltorch_cpu', '-ltorch', '-ltorch_python', f'-L{HERE}',
+           f'-L{libdir}', '-lc10', '-lc10_cuda', '-ltorch_cuda', '-ltorch_cpu', '-ltorch', '-ltorch_python', f'-L{HERE}',
            f'-l:{LIB.name}', '-Wl,-rpath,$ORIGIN']
     h = hashlib.sha256(' '.join(cmd + [torch.__version__]).encode())
     for path in (src, INCLUDE / 'speckv.h'):

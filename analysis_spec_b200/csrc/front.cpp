@@ -6,6 +6,8 @@
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
+#include <ATen/cuda/EmptyTensor.h>
+
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -62,6 +64,10 @@ int one_device(const char* fn, std::initializer_list<const Tensor*> tensors) {
 const Tensor* get(const Maybe& t) { return t.has_value() && t->defined() ? &*t : nullptr; }
 const void* data(const Tensor* t) { return t != nullptr ? t->const_data_ptr() : nullptr; }
 const int64_t* data64(const Tensor* t) { return static_cast<const int64_t*>(data(t)); }
+// A new tensor on the GPU of `like`, without the dispatcher.
+Tensor empty_like_device(at::IntArrayRef sizes, at::ScalarType dtype, const Tensor& like) {
+  return at::Tensor(at::detail::empty_cuda(sizes, dtype, like.device(), std::nullopt));
+}
 void* stream_of(int dev) { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream(); }
 
 void check_pages(const char* fn, const Tensor& k, const Tensor& v, const Tensor& table, int64_t batch) {
@@ -128,7 +134,7 @@ Maybe paged_append(const Tensor& key, const Tensor& value, const Tensor& key_pag
   Tensor made;
   if (query != nullptr && out == nullptr) {
     // (batch, rows, heads, dim) in memory, as projections and the attention lay their rows out
-    made = at::empty({batch, rows, query->size(1), dim}, query->options()).transpose(1, 2);
+    made = empty_like_device({batch, rows, query->size(1), dim}, dtype, *query).transpose(1, 2);
     out = &made;
   }
   Maybe result;
@@ -179,13 +185,13 @@ Tensor paged_attention(const Tensor& query, const Tensor& key_pages, const Tenso
     value_error(fn, "out must be a contiguous (batch, 1, q_heads, head_dim) tensor of the query dtype");
   const int dev = one_device(fn, {&query, &key_pages, &value_pages, &page_table, &lengths, given});
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
-  Tensor out = given != nullptr ? *given : at::empty({batch, 1, q_heads, dim}, query.options());
+  Tensor out = given != nullptr ? *given : empty_like_device({batch, 1, q_heads, dim}, query.scalar_type(), query);
   if (batch == 0) return out;
   // a workspace of this call alone: other streams and captured graphs have their own
   const int64_t need = speckv_paged_attention_workspace(batch, q_heads, kv_heads, dim, page_table.size(1),
                                                         key_pages.size(2), code);
   Tensor workspace;
-  if (need > 0) workspace = at::empty({need}, query.options().dtype(at::kByte));
+  if (need > 0) workspace = empty_like_device({need}, at::kByte, query);
   const int64_t st[8] = {query.stride(0),       query.stride(1),       key_pages.stride(0),   key_pages.stride(1),
                          key_pages.stride(2),   value_pages.stride(0), value_pages.stride(1), value_pages.stride(2)};
   check_status("speckv_paged_attention",
@@ -253,30 +259,30 @@ struct Scores {
   Tensor logprobs, entropy, stats, top_logprobs, top_ids;  // undefined: not asked for
 };
 
-Scores forward_scores(const Tensor& logits, const Tensor* tokens, const Tensor* rows, int64_t top, double temperature) {
+Scores forward_scores(const Tensor& logits, const Tensor* tokens, const Tensor* rows, int64_t top, double temperature,
+                      bool gradient) {
   const char* fn = "token_logprobs";
   const Rows r = check_rows(fn, logits, tokens, rows, top, temperature);
   const int dev = one_device(fn, {&logits, tokens, rows});
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
   const at::IntArrayRef shape = rows != nullptr ? rows->sizes() : logits.sizes().slice(0, logits.dim() - 1);
-  const auto f32 = logits.options().dtype(at::kFloat).requires_grad(false);
   Scores s;
   c10::SmallVector<int64_t, 4> wide(shape.begin(), shape.end());
-  if (tokens != nullptr) s.logprobs = at::empty(shape, f32);
-  s.entropy = at::empty(shape, f32);
+  if (tokens != nullptr) s.logprobs = empty_like_device(shape, at::kFloat, logits);
+  s.entropy = empty_like_device(shape, at::kFloat, logits);
   wide.push_back(2);
-  s.stats = at::empty(wide, f32);
+  if (gradient) s.stats = empty_like_device(wide, at::kFloat, logits);
   if (top > 0) {
     wide.back() = top;
-    s.top_logprobs = at::empty(wide, f32);
-    s.top_ids = at::empty(wide, f32.dtype(at::kLong));
+    s.top_logprobs = empty_like_device(wide, at::kFloat, logits);
+    s.top_ids = empty_like_device(wide, at::kLong, logits);
   }
   check_status("speckv_token_logprobs",
                speckv_token_logprobs(logits.const_data_ptr(), dtype_code(fn, logits.scalar_type()), r.logits[0],
                                      r.logits[1], data64(tokens), r.tokens[0], r.tokens[1], data64(rows), r.rows[0],
                                      r.rows[1], r.batch, r.per, r.source, logits.size(-1), (float)(1.0 / temperature),
                                      (int32_t)top, tokens != nullptr ? s.logprobs.mutable_data_ptr<float>() : nullptr,
-                                     s.entropy.mutable_data_ptr<float>(), s.stats.mutable_data_ptr<float>(),
+                                     s.entropy.mutable_data_ptr<float>(), gradient ? s.stats.mutable_data_ptr<float>() : nullptr,
                                      top > 0 ? s.top_logprobs.mutable_data_ptr<float>() : nullptr,
                                      top > 0 ? s.top_ids.mutable_data_ptr<int64_t>() : nullptr, stream_of(dev)));
   return s;
@@ -294,7 +300,7 @@ Tensor backward_scores(const Tensor& logits, const Tensor* tokens, const Tensor&
   for (Tensor* g : {&g_logprobs, &g_entropy, &g_top}) given[i++] = g->defined() ? g : nullptr;
   const int dev = one_device(fn, {&logits, tokens, &entropy, &stats, top_ids, given[0], given[1], given[2]});
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
-  Tensor grad = at::empty(logits.sizes(), logits.options().requires_grad(false));
+  Tensor grad = empty_like_device(logits.sizes(), logits.scalar_type(), logits);
   check_status("speckv_token_logprobs_backward",
                speckv_token_logprobs_backward(
                    logits.const_data_ptr(), dtype_code(fn, logits.scalar_type()), r.logits[0], r.logits[1],
@@ -310,7 +316,7 @@ Tensor backward_scores(const Tensor& logits, const Tensor* tokens, const Tensor&
 struct ScoreFunction : public torch::autograd::Function<ScoreFunction> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits,
                                                 const Maybe& tokens, int64_t top, double temperature) {
-    Scores s = forward_scores(logits, get(tokens), nullptr, top, temperature);
+    Scores s = forward_scores(logits, get(tokens), nullptr, top, temperature, true);
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["tokens"] = get(tokens) != nullptr;
     ctx->set_materialize_grads(false);
@@ -360,7 +366,7 @@ py::tuple token_logprobs(const Tensor& logits, const Maybe& tokens, const Maybe&
     return py::make_tuple(at ? item(out[0]) : py::none(), item(out[at]), top > 0 ? item(out[at + 1]) : py::none(),
                           top > 0 ? item(out[at + 2]) : py::none());
   }
-  const Scores s = forward_scores(logits, get(tokens), get(rows), top, temperature);
+  const Scores s = forward_scores(logits, get(tokens), get(rows), top, temperature, false);
   return py::make_tuple(item(s.logprobs), item(s.entropy), item(s.top_logprobs), item(s.top_ids));
 }
 

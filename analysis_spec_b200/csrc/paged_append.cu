@@ -58,7 +58,7 @@ __device__ __forceinline__ Place place_token(const AppendArgs& a, long long b, l
   return p;
 }
 
-constexpr int kAppendThreads = 128;
+constexpr int kAppendThreads = 64;
 
 // One CTA per token; elements one by one: any head dim, rotation width, stride and alignment.
 template <typename T>
@@ -189,11 +189,11 @@ __device__ __forceinline__ void rotate(uint4& px, uint4& py, const float (&c)[N]
 // pair of 16-byte pieces in kHeads heads at a time, all loaded before the first is stored; then the
 // pieces that are copied. Needs 16-byte aligned rows and rotation_dim / 2 a multiple of 16 bytes.
 // A token's work is two dependent rounds of loads (where it goes; its page, angles and rows), so
-// the registers are held to 64: 8 CTAs of an SM run such rounds at once.
+// the CTA is small and its registers are held to 64: 16 tokens of an SM are in such rounds at once.
 constexpr int kHeads = 3;
 
 template <typename T, bool INTERLEAVED>
-__global__ void __launch_bounds__(kAppendThreads, 8) paged_append_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, 16) paged_append_kernel(AppendArgs a) {
   constexpr int N = Piece<T>::N;
   const uint32_t b = blockIdx.x / (uint32_t)a.rows, t = blockIdx.x - b * (uint32_t)a.rows;
   const int q_heads = a.query != nullptr ? (int)a.q_heads : 0, kv_heads = (int)a.kv_heads, dim = (int)a.dim;
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(kAppendThreads, 8) paged_append_kernel(AppendA
   const uint32_t size = (uint32_t)a.table.page_size, index = stored ? (uint32_t)slot / size : 0u;
   const long long page = stored ? a.table.entries[b * a.table.stride + index] : 0;  // checked below
 
-  const int half = a.rot / 2, slices = half / N;  // slices <= 128
+  const int half = a.rot / 2, slices = half / N;  // slices <= 64
   const T* k = static_cast<const T*>(a.key) + b * a.ks[0] + t * a.ks[2];
   const T* v = static_cast<const T*>(a.value) + b * a.vs[0] + t * a.vs[2];
   const int slice = slices > 0 ? threadIdx.x % slices : 0, h0 = slices > 0 ? threadIdx.x / slices : 0;

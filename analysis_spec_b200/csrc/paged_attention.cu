@@ -95,13 +95,42 @@ __global__ void __launch_bounds__(kScalarWarps * 32) paged_attention_scalar_kern
   }
 }
 
-// ---- tensor-core kernel: head dims 64 / 128 / 256 in bf16 / fp16 -------------------------------
+// ---- tensor-core kernels: head dims 64 / 128 / 256 ------------------------------------------------
+//
+// Scores are K q^T (16 keys x 8 heads per matrix instruction), outputs V^T p^T (16 dims x 8
+// heads): the group's heads are the narrow side, so keys are never padded to 128 rows, as the
+// tcgen05 shapes would want. At 2 to 8 flops a byte the tensor pipe is a tenth busy either way; what
+// counts is the cache's bytes in flight, so every warp streams its own blocks of 16 keys and waits
+// for no other warp until an item ends.
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 __device__ __forceinline__ uint4 load_stream(const void* p) {
   uint4 r;
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
                : "l"(p));
+  return r;
+}
+
+// 16 bytes to shared memory; zeros when `live` is false (nothing is read then).
+__device__ __forceinline__ void copy_row(uint32_t to, const void* from, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
+}
+
+__device__ __forceinline__ void load_matrices(uint32_t at, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t load_word(uint32_t at) {
+  uint32_t r;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r) : "r"(at) : "memory");
   return r;
 }
 
@@ -118,6 +147,34 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
                "{%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+               "{%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// An fp32 number as two tf32 parts: hi is x rounded (off by 2^-11 of x at most), lo the rest, of
+// which the product takes 11 bits: x = hi + lo up to 2^-22 of x.
+__device__ __forceinline__ void split(uint32_t x, uint32_t& hi, uint32_t& lo) {
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(__uint_as_float(x)));
+  lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
+}
+// The same, not moved out of its loop: the parts of all queries would not fit the registers.
+__device__ __forceinline__ void split_here(uint32_t x, uint32_t& hi, uint32_t& lo) {
+  asm volatile("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(__uint_as_float(x)));
+  lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
+}
+// a b of fp32 operands: the three products above 2^-22.
+__device__ __forceinline__ void mma_fp32(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&bh)[2],
+                                         const uint32_t (&bl)[2]) {
+  uint32_t ah[4], al[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) split(a[i], ah[i], al[i]);
+  mma_tf32(c, al, bh[0], bh[1]);
+  mma_tf32(c, ah, bl[0], bl[1]);
+  mma_tf32(c, ah, bh[0], bh[1]);
 }
 
 // Transpose of an 8 x 8 matrix of 16-bit elements held as a matrix fragment.
@@ -141,12 +198,24 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint3
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
-constexpr int kWarps = 4;
-constexpr int kTile = 16 * kWarps;   // keys of a tile: 16 a warp
 constexpr int kMinTiles = 2;         // a CTA's share is at least this many tiles
 constexpr int kCluster = 8;          // CTAs of a cluster at most
-constexpr int kClusterTiles = 8;     // tiles of a cluster's CTA at most
+constexpr int kClusterTiles = 12;    // tiles of a cluster's CTA at most
 constexpr float kSlack = 8.f;        // scores may pass the running reference by 2^8 before it moves
+
+// Warps of a CTA, CTAs per SM (by registers in 16 bits, by the rings in fp32) and shared memory.
+template <typename T, int D, int NT> struct Shape {
+  static constexpr bool kHalf = sizeof(T) == 2;
+  static constexpr int kRow = D * (int)sizeof(T);      // bytes of a key row
+  static constexpr int kStages = 3;                    // fp32: blocks of K or V under way per warp
+  static constexpr int kWarps = kHalf || D == 256 ? 4 : 8;
+  static constexpr int kRing = kHalf ? 0 : kWarps * kStages * 16 * kRow;
+  static constexpr int kSums = kWarps * 8 * (D + 4) * 4;
+  static constexpr int kShared = kRing > kSums ? kRing : kSums;
+  static constexpr int kResident = !kHalf ? (D == 64 ? 2 : 1)
+                                   : D == 64 ? (NT == 1 ? 4 : 3) : D == 128 && NT == 1 ? 3 : 2;
+  static constexpr int kTile = 16 * kWarps;            // keys of a tile: a block a warp
+};
 
 // An item is (sequence, KV head, up to 8 NT of its query heads). All items' tiles, in order, are
 // cut into equal shares, one per CTA; a share that begins or ends inside an item leaves its part
@@ -162,49 +231,113 @@ struct PlanArgs {
   int chunks;     // items per (sequence, KV head)
 };
 
-__device__ __forceinline__ long long tiles_of(const PagedArgs& a, long long b) {
-  return (live_length(a, b) + kTile - 1) / kTile;
-}
-
-// Shared memory of a CTA: its warps' parts of an item.
-template <int D, int NT> struct Parts {
-  float o[kWarps][8][D + 4];
-  float m[kWarps][8 * NT], l[kWarps][8 * NT];
+// What a CTA's warps leave of an item, beside their sums.
+template <int W, int NT> struct Parts {
+  float m[W][8 * NT], l[W][8 * NT];
+  float top[8 * NT], all[8 * NT];  // of all warps
 };
 
-// One CTA's part of an item: tiles [t0, ...) of its keys up to position `end`. Calls
-// emit(head of the item, dim, sum, reference, total) for each of its heads and dims.
+// Joins the warps' parts of an item: own(u, e, f, to) writes the lane's sums of head 8 u + 2 t + e,
+// times f, to that head's row; emit(head of the item, dim, sum, reference, total) gets the outcome.
+template <int D, int NT, int W, typename Own, typename Emit>
+__device__ __forceinline__ void join_warps(unsigned char* shared, Parts<W, NT>& sm, float (&m)[NT][2], float (&l)[NT][2],
+                                           int heads, Own own, Emit emit) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int u = 0; u < NT; ++u)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) l[u][e] += __shfl_xor_sync(0xffffffffu, l[u][e], off);
+      if (g == 0) {
+        sm.m[warp][u * 8 + 2 * t + e] = m[u][e];
+        sm.l[warp][u * 8 + 2 * t + e] = l[u][e];
+      }
+    }
+  __syncthreads();  // the rings, over which the sums lie, are idle from here on
+  float(*sums)[8][D + 4] = reinterpret_cast<float(*)[8][D + 4]>(shared);  // [W]
+  if (threadIdx.x < 8 * NT) {
+    const int head = threadIdx.x;
+    float top = sm.m[0][head], all = 0.f;
+#pragma unroll
+    for (int w = 1; w < W; ++w) top = fmaxf(top, sm.m[w][head]);
+    const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < W; ++w) all = fmaf(sm.l[w][head], exp2f(sm.m[w][head] - ref), all);
+    sm.top[head] = top;
+    sm.all[head] = all;
+  }
+#pragma unroll
+  for (int u = 0; u < NT; ++u) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int head = u * 8 + 2 * t + e;
+      float top = sm.m[0][head];
+#pragma unroll
+      for (int w = 1; w < W; ++w) top = fmaxf(top, sm.m[w][head]);
+      const float f = top == -INFINITY ? 1.f : exp2f(m[u][e] - top);
+      own(u, e, f, sums[warp][2 * t + e]);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 8 * D; i += W * 32) {
+      const int head = i / D, d = i - head * D;
+      if (u * 8 + head >= heads) break;
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) sum += sums[w][head][d];
+      emit(u * 8 + head, d, sum, sm.top[u * 8 + head], sm.all[u * 8 + head]);
+    }
+    __syncthreads();
+  }
+}
+
+// 16-bit caches. Operands come straight from memory into registers: the dims of a product may be
+// taken in any order, so a lane's 16-byte chunks of its key rows are its fragments as they are, and
+// two keys' chunks of V give theirs by byte permutes. 8 KB a warp are under way, 12 warps on an SM.
+// (Copied ahead through shared memory instead, 8 warps, the same work took 6 to 16 % longer.)
+// One CTA's part of an item: tiles [t0, ...) of its keys up to position `end`.
 template <typename T, int D, int NT, bool PAGE16, typename Emit>
-__device__ __forceinline__ void attend_part(const PagedArgs& a, Parts<D, NT>& sm, long long b, int hk, int h0, int heads,
-                                            int t0, long long end, Emit emit) {
+__device__ __forceinline__ void attend_part16(const PagedArgs& a, unsigned char* shared,
+                                              Parts<Shape<T, D, NT>::kWarps, NT>& sm, long long b, int hk, int h0,
+                                              int heads, int t0, long long end, Emit emit) {
+  typedef Shape<T, D, NT> S;
   constexpr int KC = D / 32;  // 16-byte chunks of a key row per lane
   constexpr int VC = D / 64;  // 16-byte chunks of a value row per lane
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const long long group = a.q_heads / a.kv_heads;
   const T* kbase = static_cast<const T*>(a.k) + hk * a.ks[1];
   const T* vbase = static_cast<const T*>(a.v) + hk * a.vs[1];
-  const int64_t* table = a.table.entries + b * a.table.stride;
   const uint32_t P = (uint32_t)a.table.page_size;
 
   uint4 kreg[2][KC], vreg[4][VC];
-  uint32_t seen = 0;  // bit 0 / 1: key rows g and g + 8 of the block in kreg are live
-  long long pages = -1;
-  // block i of this warp: keys [16 (4 t0 + warp + 4 i), + 16)
-  const long long key0 = (long long)t0 * kTile + warp * 16;
-  const int count = key0 < end ? (int)((end - key0 + kTile - 1) / kTile) : 0;
+  // block i of this warp: keys [16 (W t0 + warp + W i), + 16)
+  const long long key0 = (long long)t0 * S::kTile + warp * 16;
+  const int count = key0 < end ? (int)((end - key0 + S::kTile - 1) / S::kTile) : 0;
+  // this lane's first row and chunk of a block: key rows g and g + 8, value rows 2t, 2t + 1, 2t + 8, 2t + 9
+  const T* klane = kbase + g * a.ks[2] + t * 8;
+  const T* vlane = vbase + 2 * t * a.vs[2] + g * 8;
 
-  // rows of block i: PAGE16: one page for all; else a page per row
-  long long page = -1;
-  uint32_t row = 0;
+  // PAGE16: a block lies in one page. Each lane finds the place of one block in 32.
+  long long k_places = -1, v_places = -1, k_at = -1, v_at = -1;  // element offsets; -1: no such block or page
+  int live = 0;  // keys of the block being loaded
+  uint32_t seen = 0;  // bit 0 / 1: key rows g and g + 8 of the block in kreg are live
   auto place = [&](int i) {
     if (PAGE16) {
       if ((i & 31) == 0) {
-        const long long key = key0 + (long long)(i + lane) * kTile;
-        pages = -1;
-        if (key < end) pages = a.table.page(b, (uint32_t)key / P, a.err);
+        const long long key = key0 + (long long)(i + lane) * S::kTile;
+        k_places = v_places = -1;
+        if (key < end) {
+          const uint32_t index = (uint32_t)key / P, row = (uint32_t)key - index * P;
+          const long long page = a.table.page(b, index, a.err);
+          if (page >= 0) {
+            k_places = page * a.ks[0] + row * a.ks[2];
+            v_places = page * a.vs[0] + row * a.vs[2];
+          }
+        }
       }
-      page = __shfl_sync(0xffffffffu, pages, i & 31);
-      row = (uint32_t)(key0 + (long long)i * kTile) % P;
+      k_at = __shfl_sync(0xffffffffu, k_places, i & 31);
+      v_at = __shfl_sync(0xffffffffu, v_places, i & 31);
+      live = k_at < 0 ? 0 : (int)min(16ll, end - key0 - (long long)i * S::kTile);
     }
   };
   auto row_ptr = [&](const T* from, const long long* st, long long key) -> const T* {
@@ -214,43 +347,50 @@ __device__ __forceinline__ void attend_part(const PagedArgs& a, Parts<D, NT>& sm
     return p < 0 ? nullptr : from + p * st[0] + (long long)((uint32_t)key - index * P) * st[2];
   };
   auto load_k = [&](int i) {
-    const long long key = key0 + (long long)i * kTile;
-    const T* p0;
-    const T* p1;
-    if (PAGE16) {
-      const int live = page < 0 ? 0 : (int)min(16ll, end - key);
-      p0 = kbase + page * a.ks[0] + (long long)(row + g) * a.ks[2];
-      p1 = g + 8 < live ? p0 + 8 * a.ks[2] : nullptr;
-      if (g >= live) p0 = nullptr;
-    } else {
-      p0 = row_ptr(kbase, a.ks, key + g);
-      p1 = row_ptr(kbase, a.ks, key + g + 8);
-    }
-    seen = (p0 != nullptr ? 1u : 0u) | (p1 != nullptr ? 2u : 0u);
+    if (PAGE16 && live == 16) {
+      const T* p = klane + k_at;
 #pragma unroll
-    for (int j = 0; j < KC; ++j) {
-      kreg[0][j] = kreg[1][j] = make_uint4(0, 0, 0, 0);
-      if (p0 != nullptr) kreg[0][j] = load_stream(p0 + (t + 4 * j) * 8);
-      if (p1 != nullptr) kreg[1][j] = load_stream(p1 + (t + 4 * j) * 8);
+      for (int j = 0; j < KC; ++j) {
+        kreg[0][j] = load_stream(p + 32 * j);
+        kreg[1][j] = load_stream(p + 8 * a.ks[2] + 32 * j);
+      }
+      seen = 3u;
+      return;
     }
+    const long long key = key0 + (long long)i * S::kTile;
+    const T* p[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      if (PAGE16)
+        p[x] = g + 8 * x < live ? klane + k_at + 8 * x * a.ks[2] : nullptr;
+      else
+        p[x] = row_ptr(kbase + t * 8, a.ks, key + g + 8 * x);
+#pragma unroll
+      for (int j = 0; j < KC; ++j) kreg[x][j] = p[x] != nullptr ? load_stream(p[x] + 32 * j) : make_uint4(0, 0, 0, 0);
+    }
+    seen = (p[0] != nullptr ? 1u : 0u) | (p[1] != nullptr ? 2u : 0u);
   };
   auto load_v = [&](int i) {
-    const long long key = key0 + (long long)i * kTile;
+    if (PAGE16 && live == 16) {
+      const T* p = vlane + v_at;
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int c = 0; c < VC; ++c) vreg[x][c] = load_stream(p + ((x & 1) + (x >> 1) * 8) * a.vs[2] + 64 * c);
+      return;
+    }
+    const long long key = key0 + (long long)i * S::kTile;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      const int k = 2 * t + (x & 1) + (x >> 1) * 8;  // keys 2t, 2t + 1, 2t + 8, 2t + 9
+      const int k = 2 * t + (x & 1) + (x >> 1) * 8;
       const T* p;
-      if (PAGE16) {
-        const int live = page < 0 ? 0 : (int)min(16ll, end - key);
-        p = k < live ? vbase + page * a.vs[0] + (long long)(row + k) * a.vs[2] : nullptr;
-      } else {
-        p = row_ptr(vbase, a.vs, key + k);
-      }
+      if (PAGE16)
+        p = k < live ? vlane + v_at + ((x & 1) + (x >> 1) * 8) * a.vs[2] : nullptr;
+      else
+        p = row_ptr(vbase + g * 8, a.vs, key + k);
+      // rows that are not there may hold anything: 0 x NaN is NaN
 #pragma unroll
-      for (int c = 0; c < VC; ++c) {
-        vreg[x][c] = make_uint4(0, 0, 0, 0);  // rows that are not there may hold anything: 0 x NaN is NaN
-        if (p != nullptr) vreg[x][c] = load_stream(p + (g + 8 * c) * 8);
-      }
+      for (int c = 0; c < VC; ++c) vreg[x][c] = p != nullptr ? load_stream(p + 64 * c) : make_uint4(0, 0, 0, 0);
     }
   };
 
@@ -338,8 +478,8 @@ __device__ __forceinline__ void attend_part(const PagedArgs& a, Parts<D, NT>& sm
           }
       }
       const float r0 = m[u][0] == -INFINITY ? 0.f : m[u][0], r1 = m[u][1] == -INFINITY ? 0.f : m[u][1];
-      const float p0 = exp2f(s[u][0] - r0), p1 = exp2f(s[u][1] - r1), p2 = exp2f(s[u][2] - r0),
-                  p3 = exp2f(s[u][3] - r1);
+      const float p0 = exp2_fast(s[u][0] - r0), p1 = exp2_fast(s[u][1] - r1), p2 = exp2_fast(s[u][2] - r0),
+                  p3 = exp2_fast(s[u][3] - r1);
       l[u][0] += p0 + p2;
       l[u][1] += p1 + p3;
       // weights to (key pairs, heads) fragments, in two 16-bit parts: the tensor pipe has room
@@ -370,66 +510,283 @@ __device__ __forceinline__ void attend_part(const PagedArgs& a, Parts<D, NT>& sm
     if (i + 1 < count) load_v(i + 1);
   }
 
+  join_warps<D, NT, S::kWarps>(shared, sm, m, l, heads, [&](int u, int e, float f, float* to) {
+#pragma unroll
+    for (int c = 0; c < VC; ++c)
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        *reinterpret_cast<float2*>(to + (g + 8 * c) * 8 + 2 * x) = make_float2(o[u][c][x][e] * f, o[u][c][x][2 + e] * f);
+  }, emit);
+}
 
-  // the warps' parts, joined
-#pragma unroll
-  for (int u = 0; u < NT; ++u)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-#pragma unroll
-      for (int off = 4; off < 32; off <<= 1) l[u][e] += __shfl_xor_sync(0xffffffffu, l[u][e], off);
-      if (g == 0) {
-        sm.m[warp][u * 8 + 2 * t + e] = m[u][e];
-        sm.l[warp][u * 8 + 2 * t + e] = l[u][e];
+// fp32 caches. Twice the bytes a key and six instructions a product: K and V rows are copied ahead
+// through a ring of shared memory per warp (blocks of K and of V in turn, 16 bytes a lane and copy),
+// which leaves the registers to the products. Products are three of tf32 parts.
+template <int D, int NT, bool PAGE16, typename Emit>
+__device__ __forceinline__ void attend_part32(const PagedArgs& a, unsigned char* shared,
+                                              Parts<Shape<float, D, NT>::kWarps, NT>& sm, long long b, int hk, int h0,
+                                              int heads, int t0, long long end, Emit emit) {
+  typedef Shape<float, D, NT> S;
+  constexpr int CHUNKS = S::kRow / 16, E = 4, BLOCK = 16 * S::kRow;
+  constexpr int STEPS = D / (2 * E);      // products of a score: 8 dims each
+  constexpr int ROWS = 32 / CHUNKS > 0 ? 32 / CHUNKS : 1;  // rows that one copy of a warp covers
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const long long group = a.q_heads / a.kv_heads;
+  const float* kbase = static_cast<const float*>(a.k) + hk * a.ks[1];
+  const float* vbase = static_cast<const float*>(a.v) + hk * a.vs[1];
+  const uint32_t P = (uint32_t)a.table.page_size;
+  const uint32_t mine = (uint32_t)__cvta_generic_to_shared(shared) + warp * S::kStages * BLOCK;
+  // Chunk c of row r lies at c ^ swizzle(r): the 8 rows of a matrix, and the 4 rows that a
+  // transposed operand takes, are in different banks.
+  auto swizzle = [](int r) { return ((r & 3) << 1) | ((r >> 2) & 1); };
+
+  // block i of this warp: keys [16 (W t0 + warp + W i), + 16)
+  const long long key0 = (long long)t0 * S::kTile + warp * 16;
+  const int count = key0 < end ? (int)((end - key0 + S::kTile - 1) / S::kTile) : 0;
+
+  // Each lane finds the place of one block in 32 (PAGE16: a block lies in one page) or of one row
+  // of a block, as element offsets; -1: no such block or row, or no page of the pools.
+  long long k_places = -1, v_places = -1;
+  bool missing = false;  // a page of this item is not one of the pools'
+  auto find = [&](long long key) {
+    k_places = v_places = -1;
+    bool bad = false;
+    if (key < end) {
+      const uint32_t index = (uint32_t)key / P, row = (uint32_t)key - index * P;
+      const long long page = a.table.page(b, index, a.err);
+      bad = page < 0;
+      if (!bad) {
+        k_places = page * a.ks[0] + row * a.ks[2];
+        v_places = page * a.vs[0] + row * a.vs[2];
       }
     }
-  __syncthreads();
+    missing = __any_sync(0xffffffffu, bad) || missing;
+  };
+  // piece 2 i: the keys of block i, piece 2 i + 1: its values
+  auto copy_piece = [&](int piece, int stage) {
+    const int i = piece >> 1;
+    const bool values = piece & 1;
+    const uint32_t to = mine + stage * BLOCK;
+    const long long key = key0 + (long long)i * S::kTile;
+    if (!values) {
+      if (PAGE16) {
+        if ((i & 31) == 0) find(key + (long long)lane * S::kTile);
+      } else {
+        find(lane < 16 ? key + lane : end);
+      }
+    }
+    const long long place = values ? v_places : k_places, block = __shfl_sync(0xffffffffu, place, i & 31);
+    const float* base = values ? vbase : kbase;
+    const long long stride = values ? a.vs[2] : a.ks[2];
+    const int rows = block < 0 ? 0 : (int)min(16ll, end - key);
+    const int r0 = lane / CHUNKS, chunk = lane % CHUNKS;
+#pragma unroll
+    for (int r = 0; r < 16; r += ROWS) {
+      const long long row = PAGE16 ? block + (r + r0) * stride : __shfl_sync(0xffffffffu, place, r + r0);
+      const bool live = PAGE16 ? r + r0 < rows : row >= 0;
+#pragma unroll
+      for (int c = chunk; c < CHUNKS; c += 32)
+        copy_row(to + (r + r0) * S::kRow + ((c ^ swizzle(r + r0)) << 4), live ? base + row + c * E : base, live);
+    }
+  };
+  // bits 0 and 1: whether keys g and g + 8 of block i count
+  auto counted = [&](int i) -> uint32_t {
+    uint32_t live = 0;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const long long key = key0 + (long long)i * S::kTile + g + 8 * x;
+      if (key < end) {
+        const long long page = a.table.entries[b * a.table.stride + (uint32_t)key / P];
+        if (page >= 0 && page < a.table.num_pages) live |= 1u << x;
+      }
+    }
+    return live;
+  };
+
+#pragma unroll
+  for (int i = 0; i < S::kStages; ++i) {
+    if (i < 2 * count) copy_piece(i, i);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  // queries as the second operand: head g, the dims of this lane's k
+  uint32_t q[NT][STEPS][2];
+#pragma unroll
+  for (int u = 0; u < NT; ++u) {
+    const bool there = u * 8 + g < heads;
+    const float* p = static_cast<const float*>(a.q) + b * a.qs[0] + (hk * group + h0 + (there ? u * 8 + g : 0)) * a.qs[1] +
+                 t;
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        q[u][i][x] = there ? *reinterpret_cast<const uint32_t*>(p + (2 * i + x) * E) : 0u;
+  }
+  float o[NT][D / 16][4], m[NT][2], l[NT][2];
 #pragma unroll
   for (int u = 0; u < NT; ++u) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int head = u * 8 + 2 * t + e;
-      float top = sm.m[0][head];
+    for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm.m[w][head]);
-      const float f = top == -INFINITY ? 1.f : exp2f(m[u][e] - top);
-#pragma unroll
-      for (int c = 0; c < VC; ++c) {
-        float* to = &sm.o[warp][2 * t + e][(g + 8 * c) * 8];
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-          *reinterpret_cast<float2*>(to + 2 * x) = make_float2(o[u][c][x][e] * f, o[u][c][x][2 + e] * f);
-      }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 8 * D; i += kWarps * 32) {
-      const int head = i / D, d = i - head * D;
-      if (u * 8 + head >= heads) break;
-      float top = sm.m[0][u * 8 + head];
-#pragma unroll
-      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm.m[w][u * 8 + head]);
-      const float ref = top == -INFINITY ? 0.f : top;
-      float sum = 0.f, all = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        sum += sm.o[w][head][d];
-        all = fmaf(sm.l[w][u * 8 + head], exp2f(sm.m[w][u * 8 + head] - ref), all);
-      }
-      emit(u * 8 + head, d, sum, top, all);
-    }
-    __syncthreads();
+      for (int e = 0; e < 4; ++e) o[u][i][e] = 0.f;
+    m[u][0] = m[u][1] = -INFINITY;
+    l[u][0] = l[u][1] = 0.f;
   }
+  const int k_lane = (lane & 15) * S::kRow, k_swizzle = swizzle(lane & 15), k_chunk = lane >> 4;
+  int stage = 0;
+  auto next_piece = [&](int piece) {  // the current one is read; its slot takes the piece kStages on
+    __syncwarp();
+    if (piece + S::kStages < 2 * count) copy_piece(piece + S::kStages, stage);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    stage = stage + 1 == S::kStages ? 0 : stage + 1;
+    asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
+    __syncwarp();  // the other lanes' copies too
+  };
+  asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
+  __syncwarp();
+
+  for (int i = 0; i < count; ++i) {
+    const uint32_t k_at = mine + stage * BLOCK;
+    // scores of 16 keys x 8 heads: rows keys g, g + 8, columns heads 2t, 2t + 1
+    float s[NT][4], s2[NT][4];
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[u][e] = s2[u][e] = 0.f;
+#pragma unroll
+    for (int j = 0; j < STEPS; ++j) {
+      uint32_t k[4];
+      load_matrices(k_at + k_lane + (((2 * j + k_chunk) ^ k_swizzle) << 4), k);
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        float(&to)[4] = j & 1 ? s2[u] : s[u];
+        uint32_t qh[2], ql[2];
+        split_here(q[u][j][0], qh[0], ql[0]);
+        split_here(q[u][j][1], qh[1], ql[1]);
+        mma_fp32(to, k, qh, ql);
+      }
+    }
+    // an infinite key has no parts (inf - inf): such a block's scores are summed term by term
+    bool lost = false;
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) lost |= s[u][e] + s2[u][e] != s[u][e] + s2[u][e];
+    if (__any_sync(0xffffffffu, lost)) {
+#pragma unroll
+      for (int u = 0; u < NT; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = g + 8 * (e >> 1), head = u * 8 + 2 * t + (e & 1);
+          s[u][e] = s2[u][e] = 0.f;
+          if (head < heads) {
+            const float* p = static_cast<const float*>(a.q) + b * a.qs[0] + (hk * group + h0 + head) * a.qs[1];
+            for (int d = 0; d < D; ++d)
+              s[u][e] = fmaf(p[d], __uint_as_float(load_word(k_at + row * S::kRow + (((d >> 2) ^ swizzle(row)) << 4) + (d & 3) * 4)),
+                             s[u][e]);
+          }
+        }
+    }
+    const bool part = missing || end - key0 - (long long)i * S::kTile < 16;
+    const uint32_t live = part ? counted(i) : 3u;
+    next_piece(2 * i);
+    const uint32_t v_at = mine + stage * BLOCK;
+    uint32_t ph[NT][2][2], pl[NT][2][2];  // weights as the second operand: keys t and t + 4 of each half, head g
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[u][e] = (s[u][e] + s2[u][e]) * a.scale_log2;
+      if (part)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (!(live >> (e >> 1) & 1u)) s[u][e] = -INFINITY;
+      float top0 = fmaxf(s[u][0], s[u][2]), top1 = fmaxf(s[u][1], s[u][3]);
+      // The reference need not be the maximum: any value within 2^8 of it keeps every weight and
+      // sum well inside fp32, and the sums are divided by the total at the end. So it moves only
+      // when a score passes it by more than that (the first block moves it from -inf).
+      if (__any_sync(0xffffffffu, top0 > m[u][0] + kSlack || top1 > m[u][1] + kSlack)) {
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) {
+          top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, off));
+          top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, off));
+        }
+        const float n0 = fmaxf(m[u][0], top0), n1 = fmaxf(m[u][1], top1);
+        const float f0 = n0 == -INFINITY ? 1.f : exp2f(m[u][0] - n0);
+        const float f1 = n1 == -INFINITY ? 1.f : exp2f(m[u][1] - n1);
+        m[u][0] = n0;
+        m[u][1] = n1;
+        l[u][0] *= f0;
+        l[u][1] *= f1;
+#pragma unroll
+        for (int x = 0; x < D / 16; ++x) {
+          o[u][x][0] *= f0;
+          o[u][x][1] *= f1;
+          o[u][x][2] *= f0;
+          o[u][x][3] *= f1;
+        }
+      }
+      const float r0 = m[u][0] == -INFINITY ? 0.f : m[u][0], r1 = m[u][1] == -INFINITY ? 0.f : m[u][1];
+      const float p[4] = {exp2_fast(s[u][0] - r0), exp2_fast(s[u][1] - r1), exp2_fast(s[u][2] - r0),
+                          exp2_fast(s[u][3] - r1)};
+      l[u][0] += p[0] + p[2];
+      l[u][1] += p[1] + p[3];
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const int from = (t + 4 * y) * 4 + (g >> 1);
+          const float even = __shfl_sync(0xffffffffu, p[2 * x], from), odd = __shfl_sync(0xffffffffu, p[2 * x + 1], from);
+          split(__float_as_uint(g & 1 ? odd : even), ph[u][x][y], pl[u][x][y]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        uint32_t v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // dims 16 j + g (+ 8), keys 8 x + t (+ 4)
+          const int row = 8 * x + t + 4 * (e >> 1);
+          v[e] = load_word(v_at + row * S::kRow + (((4 * j + (g >> 2) + 2 * (e & 1)) ^ swizzle(row)) << 4) + (g & 3) * 4);
+        }
+#pragma unroll
+        for (int u = 0; u < NT; ++u) mma_fp32(o[u][j], v, ph[u][x], pl[u][x]);
+      }
+    next_piece(2 * i + 1);
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+
+  join_warps<D, NT, S::kWarps>(shared, sm, m, l, heads, [&](int u, int e, float f, float* to) {
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) {
+      to[16 * j + g] = o[u][j][e] * f;
+      to[16 * j + g + 8] = o[u][j][2 + e] * f;
+    }
+  }, emit);
 }
 
-// CTAs per SM of the tensor-core kernels.
-template <int D, int NT> constexpr int resident() { return D == 64 ? (NT == 1 ? 4 : 3) : D == 128 ? (NT == 1 ? 3 : 2) : 2; }
+template <typename T, int D, int NT, bool PAGE16, typename Emit>
+__device__ __forceinline__ void attend_part(const PagedArgs& a, unsigned char* shared,
+                                            Parts<Shape<T, D, NT>::kWarps, NT>& sm, long long b, int hk, int h0, int heads,
+                                            int t0, long long end, Emit emit) {
+  if constexpr (sizeof(T) == 2)
+    attend_part16<T, D, NT, PAGE16>(a, shared, sm, b, hk, h0, heads, t0, end, emit);
+  else
+    attend_part32<D, NT, PAGE16>(a, shared, sm, b, hk, h0, heads, t0, end, emit);
+}
+
+__device__ __forceinline__ long long tiles_of(const PagedArgs& a, long long b, int tile) {
+  return (live_length(a, b) + tile - 1) / tile;
+}
 
 template <typename T, int D, int NT, bool PAGE16>
-__global__ void __launch_bounds__(kWarps * 32, resident<D, NT>()) paged_attention_mma_kernel(PagedArgs a, PlanArgs plan) {
+__global__ void __launch_bounds__(Shape<T, D, NT>::kWarps * 32, Shape<T, D, NT>::kResident)
+    paged_attention_share_kernel(PagedArgs a, PlanArgs plan) {
+  constexpr int W = Shape<T, D, NT>::kWarps, kTile = Shape<T, D, NT>::kTile;
   constexpr int PART = 8 * NT * (D + 2);
   asm volatile("griddepcontrol.launch_dependents;");
-  __shared__ Parts<D, NT> sm;
-  __shared__ long long s_scan[kWarps], s_find[2];
+  extern __shared__ __align__(128) unsigned char shared[];
+  __shared__ Parts<W, NT> sm;
+  __shared__ long long s_scan[W], s_find[2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long group = a.q_heads / a.kv_heads, per_seq = a.kv_heads * plan.chunks;
   const int G = gridDim.x, cta = blockIdx.x;
@@ -437,14 +794,14 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, NT>()) paged_attentio
   // sequences with nothing to see
   for (long long b = cta; b < a.batch; b += G)
     if (live_length(a, b) == 0)
-      for (long long i = threadIdx.x; i < a.q_heads * D; i += kWarps * 32)
+      for (long long i = threadIdx.x; i < a.q_heads * D; i += W * 32)
         static_cast<T*>(a.out)[b * a.q_heads * D + i] = store_f<T>(0.f);
 
   // tiles before each thread's run of sequences, and in all
-  const long long run = (a.batch + kWarps * 32 - 1) / (kWarps * 32);
+  const long long run = (a.batch + W * 32 - 1) / (W * 32);
   const long long b_lo = min(a.batch, (long long)threadIdx.x * run), b_hi = min(a.batch, b_lo + run);
   long long mine = 0;
-  for (long long b = b_lo; b < b_hi; ++b) mine += tiles_of(a, b);
+  for (long long b = b_lo; b < b_hi; ++b) mine += tiles_of(a, b, kTile);
   long long upto = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -456,7 +813,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, NT>()) paged_attentio
   __syncthreads();
   long long total = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
+  for (int w = 0; w < W; ++w) {
     if (w < warp) upto += s_scan[w];
     total += s_scan[w];
   }
@@ -472,7 +829,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, NT>()) paged_attentio
   if (mine > 0 && lo >= (upto - mine) * per_seq && lo < upto * per_seq) {
     long long before = (upto - mine) * per_seq, b = b_lo;
     for (; b + 1 < b_hi; ++b) {
-      const long long n = tiles_of(a, b) * per_seq;
+      const long long n = tiles_of(a, b, kTile) * per_seq;
       if (lo < before + n) break;
       before += n;
     }
@@ -506,7 +863,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, NT>()) paged_attentio
       join = Join{(int)b, h, slot, (int)(last - cta) + 1};
     }
     T* out = static_cast<T*>(a.out) + (b * a.q_heads + hk * group + h0) * D;
-    attend_part<T, D, NT, PAGE16>(a, sm, b, hk, h0, heads, t0, end, [&](int head, int d, float sum, float top, float all) {
+    attend_part<T, D, NT, PAGE16>(a, shared, sm, b, hk, h0, heads, t0, end, [&](int head, int d, float sum, float top, float all) {
       if (whole) {
         out[head * D + d] = store_f<T>(all == 0.f ? 0.f : sum / all);
       } else {
@@ -526,9 +883,11 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, NT>()) paged_attentio
 // Few items: a cluster of CTAs each, an equal run of its tiles per CTA, joined through the
 // cluster's shared memory. One launch, no workspace.
 template <typename T, int D, int NT, bool PAGE16>
-__global__ void __launch_bounds__(kWarps * 32, resident<D, NT>())
+__global__ void __launch_bounds__(Shape<T, D, NT>::kWarps * 32, Shape<T, D, NT>::kResident)
     paged_attention_cluster_kernel(PagedArgs a, PlanArgs plan) {
-  __shared__ Parts<D, NT> sm;
+  constexpr int W = Shape<T, D, NT>::kWarps, kTile = Shape<T, D, NT>::kTile;
+  extern __shared__ __align__(128) unsigned char shared[];
+  __shared__ Parts<W, NT> sm;
   __shared__ float s_sum[8 * NT][D], s_top[8 * NT], s_all[8 * NT];
   const uint32_t ctas = cluster_size(), rank = cluster_rank();
   const long long group = a.q_heads / a.kv_heads, per_seq = a.kv_heads * plan.chunks;
@@ -538,7 +897,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, NT>())
   const int hk = h / plan.chunks, h0 = (h - hk * plan.chunks) * 8 * NT, heads = min((int)group - h0, 8 * NT);
   const long long n = live_length(a, b), nb = (n + kTile - 1) / kTile;
   const int t0 = (int)(nb * rank / ctas), t1 = (int)(nb * (rank + 1) / ctas);
-  attend_part<T, D, NT, PAGE16>(a, sm, b, hk, h0, heads, t0, min(n, (long long)t1 * kTile),
+  attend_part<T, D, NT, PAGE16>(a, shared, sm, b, hk, h0, heads, t0, min(n, (long long)t1 * kTile),
                                 [&](int head, int d, float sum, float top, float all) {
                                   s_sum[head][d] = sum;
                                   if (d == 0) {
@@ -549,7 +908,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, NT>())
   cluster_sync();
   // each CTA joins its share of the outputs
   T* out = static_cast<T*>(a.out) + (b * a.q_heads + hk * group + h0) * D;
-  for (int i = rank * kWarps * 32 + threadIdx.x; i < heads * D; i += ctas * kWarps * 32) {
+  for (int i = rank * W * 32 + threadIdx.x; i < heads * D; i += ctas * W * 32) {
     const int head = i / D, d = i - head * D;
     float top[kCluster], all[kCluster], sum[kCluster], ref = -INFINITY;
 #pragma unroll
@@ -659,25 +1018,24 @@ int sm_count() {
   return counts[dev];
 }
 
-int ctas_per_sm(int64_t dim, int nt) {
-  return dim == 64 ? (nt == 1 ? resident<64, 1>() : resident<64, 2>())
-                   : dim == 128 ? (nt == 1 ? resident<128, 1>() : resident<128, 2>()) : resident<256, 1>();
+template <typename T> void shape_of(int64_t dim, int nt, int& resident, int& tile) {
+  if (dim == 64) resident = nt == 1 ? Shape<T, 64, 1>::kResident : Shape<T, 64, 2>::kResident, tile = Shape<T, 64, 1>::kTile;
+  else if (dim == 128) resident = nt == 1 ? Shape<T, 128, 1>::kResident : Shape<T, 128, 2>::kResident, tile = Shape<T, 128, 1>::kTile;
+  else resident = Shape<T, 256, 1>::kResident, tile = Shape<T, 256, 1>::kTile;
 }
 
 // Query heads of an item: the tensor instruction takes 8, two of them share the key and value
 // registers where those leave room (head dims to 128).
 int head_tiles(int64_t dim, int64_t group) { return group > 8 && dim <= 128 ? 2 : 1; }
 
-bool tensor_shape(int64_t dim, int32_t dtype) {
-  return dtype != SPECKV_F32 && (dim == 64 || dim == 128 || dim == 256);
-}
+bool tensor_shape(int64_t dim) { return dim == 64 || dim == 128 || dim == 256; }
 
 // CTAs of a cluster per item, 0 for equal shares: clusters where they all run at once and the
 // longest sequence that the table can hold leaves each CTA few tiles.
 int cluster_ctas(long long items, long long tiles, int full) {
-  int ctas = 1;
-  while (ctas < kCluster && ctas < tiles && items * ctas * 2 <= full) ctas *= 2;
-  return items * ctas <= full && tiles <= (long long)ctas * kClusterTiles ? ctas : 0;
+  if (items > full) return 0;
+  const long long ctas = min(min((long long)kCluster, full / items), tiles);
+  return tiles <= ctas * kClusterTiles ? (int)ctas : 0;
 }
 
 // How a tensor shape is launched, from sizes that the host knows.
@@ -687,27 +1045,46 @@ struct Launch {
   int64_t workspace;
 };
 
+template <typename T>
 Launch plan_launch(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t positions, int sms) {
   Launch l;
   const int64_t group = q_heads / kv_heads;
   l.tiles8 = head_tiles(dim, group);
+  int resident, tile;
+  shape_of<T>(dim, l.tiles8, resident, tile);
   l.chunks = (int)((group + 8 * l.tiles8 - 1) / (8 * l.tiles8));
-  l.full = sms * ctas_per_sm(dim, l.tiles8);
+  l.full = sms * resident;
   l.items = batch * kv_heads * l.chunks;
-  l.tiles = (positions + kTile - 1) / kTile;
+  l.tiles = (positions + tile - 1) / tile;
   l.cluster = cluster_ctas(l.items, l.tiles, l.full);
   l.workspace = l.cluster > 0 ? 0 : (int64_t)l.full * (2 * 8 * l.tiles8 * (dim + 2) * sizeof(float) + sizeof(Join));
   return l;
 }
 
-template <typename T, int D, int NT>
+// Lets `kernel` have its shared memory, once per device.
+template <typename K> cudaError_t allow_shared(K kernel, int bytes, bool (&done)[64]) {
+  if (bytes <= 32768) return cudaSuccess;  // within what every kernel has
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || dev < 0 || dev >= 64 || done[dev]) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done[dev] = true;
+  return e;
+}
+
+int launch_failed(cudaError_t e) {
+  return fail(SPECKV_ECUDA, "speckv_paged_attention: launch failed: %s", cudaGetErrorString(e));
+}
+
+template <typename T, int D, int NT, bool PAGE16>
 int launch_shares(const PagedArgs& a, const PlanArgs& plan, int ctas, cudaStream_t s) {
-  if (a.table.page_size % 16 == 0)
-    paged_attention_mma_kernel<T, D, NT, true><<<ctas, kWarps * 32, 0, s>>>(a, plan);
-  else
-    paged_attention_mma_kernel<T, D, NT, false><<<ctas, kWarps * 32, 0, s>>>(a, plan);
-  int st = check_launch("speckv_paged_attention");
-  if (st) return st;
+  typedef Shape<T, D, NT> S;
+  static bool done[64] = {false};
+  auto kernel = paged_attention_share_kernel<T, D, NT, PAGE16>;
+  cudaError_t e = allow_shared(kernel, S::kShared, done);
+  if (e != cudaSuccess) return launch_failed(e);
+  kernel<<<ctas, S::kWarps * 32, S::kShared, s>>>(a, plan);
+  if ((e = cudaGetLastError()) != cudaSuccess) return launch_failed(e);
   // starts while the first kernel ends (programmatic dependent launch), waits for it before it reads
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -718,28 +1095,30 @@ int launch_shares(const PagedArgs& a, const PlanArgs& plan, int ctas, cudaStream
   cfg.stream = s;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<T, D, NT>, a, plan);
-  if (e != cudaSuccess) return fail(SPECKV_ECUDA, "speckv_paged_attention: launch failed: %s", cudaGetErrorString(e));
-  return SPECKV_OK;
+  e = cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<T, D, NT>, a, plan);
+  return e == cudaSuccess ? SPECKV_OK : launch_failed(e);
 }
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, bool PAGE16>
 int launch_clusters(const PagedArgs& a, const PlanArgs& plan, int items, int ctas, cudaStream_t s) {
+  typedef Shape<T, D, NT> S;
+  static bool done[64] = {false};
+  auto kernel = paged_attention_cluster_kernel<T, D, NT, PAGE16>;
+  cudaError_t e = allow_shared(kernel, S::kShared, done);
+  if (e != cudaSuccess) return launch_failed(e);
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = ctas;
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(items * ctas));
-  cfg.blockDim = dim3(kWarps * 32);
+  cfg.blockDim = dim3(S::kWarps * 32);
+  cfg.dynamicSmemBytes = S::kShared;
   cfg.stream = s;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = a.table.page_size % 16 == 0
-                            ? cudaLaunchKernelEx(&cfg, paged_attention_cluster_kernel<T, D, NT, true>, a, plan)
-                            : cudaLaunchKernelEx(&cfg, paged_attention_cluster_kernel<T, D, NT, false>, a, plan);
-  if (e != cudaSuccess) return fail(SPECKV_ECUDA, "speckv_paged_attention: launch failed: %s", cudaGetErrorString(e));
-  return SPECKV_OK;
+  e = cudaLaunchKernelEx(&cfg, kernel, a, plan);
+  return e == cudaSuccess ? SPECKV_OK : launch_failed(e);
 }
 
 template <typename T, int D, int NT>
@@ -748,17 +1127,21 @@ int launch_tensor(const PagedArgs& a, const Launch& l, void* workspace, cudaStre
   plan.chunks = l.chunks;
   plan.joins = static_cast<Join*>(workspace);
   plan.parts = reinterpret_cast<float*>(plan.joins + l.full);
-  if (l.cluster > 0) return launch_clusters<T, D, NT>(a, plan, (int)l.items, l.cluster, s);
+  const bool page16 = a.table.page_size % 16 == 0;
+  if (l.cluster > 0)
+    return page16 ? launch_clusters<T, D, NT, true>(a, plan, (int)l.items, l.cluster, s)
+                  : launch_clusters<T, D, NT, false>(a, plan, (int)l.items, l.cluster, s);
   // no more CTAs than shares of the longest sequences possible
   const double most = (double)l.items * (double)l.tiles / kMinTiles;
-  return launch_shares<T, D, NT>(a, plan, most < l.full ? (int)most + 1 : l.full, s);
+  const int ctas = most < l.full ? (int)most + 1 : l.full;
+  return page16 ? launch_shares<T, D, NT, true>(a, plan, ctas, s) : launch_shares<T, D, NT, false>(a, plan, ctas, s);
 }
 
 template <typename T>
-int launch_paged(const PagedArgs& a, int32_t dtype, void* workspace, int64_t bytes, cudaStream_t s) {
+int launch_paged(const PagedArgs& a, void* workspace, int64_t bytes, cudaStream_t s) {
   // 16-byte loads need aligned rows; other views take the scalar kernel
   const size_t es = sizeof(T);
-  bool aligned = tensor_shape(a.dim, dtype);
+  bool aligned = tensor_shape(a.dim);
   const void* bases[4] = {a.q, a.k, a.v, a.out};
   for (const void* p : bases) aligned = aligned && reinterpret_cast<uintptr_t>(p) % 16 == 0;
   for (int i = 0; i < 3; ++i) aligned = aligned && a.ks[i] * es % 16 == 0 && a.vs[i] * es % 16 == 0;
@@ -767,20 +1150,17 @@ int launch_paged(const PagedArgs& a, int32_t dtype, void* workspace, int64_t byt
     paged_attention_scalar_kernel<T><<<(unsigned)(a.batch * a.q_heads), kScalarWarps * 32, 0, s>>>(a);
     return check_launch("speckv_paged_attention");
   }
-  if constexpr (sizeof(T) == 2) {
-    const int sms = sm_count();
-    if (sms == 0) return fail(SPECKV_ECUDA, "speckv_paged_attention: no SM count");
-    const Launch l = plan_launch(a.batch, a.q_heads, a.kv_heads, a.dim, a.table.width * a.table.page_size, sms);
-    if (l.workspace > 0 && (workspace == nullptr || bytes < l.workspace || reinterpret_cast<uintptr_t>(workspace) % 16))
-      return fail(SPECKV_EINVAL, "speckv_paged_attention: workspace of %lld bytes, %lld needed (16-byte aligned)",
-                  (long long)bytes, (long long)l.workspace);
-    if (a.dim == 64)
-      return l.tiles8 == 1 ? launch_tensor<T, 64, 1>(a, l, workspace, s) : launch_tensor<T, 64, 2>(a, l, workspace, s);
-    if (a.dim == 128)
-      return l.tiles8 == 1 ? launch_tensor<T, 128, 1>(a, l, workspace, s) : launch_tensor<T, 128, 2>(a, l, workspace, s);
-    return launch_tensor<T, 256, 1>(a, l, workspace, s);
-  }
-  return SPECKV_OK;
+  const int sms = sm_count();
+  if (sms == 0) return fail(SPECKV_ECUDA, "speckv_paged_attention: no SM count");
+  const Launch l = plan_launch<T>(a.batch, a.q_heads, a.kv_heads, a.dim, a.table.width * a.table.page_size, sms);
+  if (l.workspace > 0 && (workspace == nullptr || bytes < l.workspace || reinterpret_cast<uintptr_t>(workspace) % 16))
+    return fail(SPECKV_EINVAL, "speckv_paged_attention: workspace of %lld bytes, %lld needed (16-byte aligned)",
+                (long long)bytes, (long long)l.workspace);
+  if (a.dim == 64)
+    return l.tiles8 == 1 ? launch_tensor<T, 64, 1>(a, l, workspace, s) : launch_tensor<T, 64, 2>(a, l, workspace, s);
+  if (a.dim == 128)
+    return l.tiles8 == 1 ? launch_tensor<T, 128, 1>(a, l, workspace, s) : launch_tensor<T, 128, 2>(a, l, workspace, s);
+  return launch_tensor<T, 256, 1>(a, l, workspace, s);
 }
 
 }  // namespace
@@ -833,16 +1213,18 @@ extern "C" int speckv_paged_attention(const void* query, const void* key_pages, 
   if (a.err == nullptr) return fail(SPECKV_ECUDA, "%s: no error word on device", fn);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
-    case SPECKV_F32: return launch_paged<float>(a, dtype, workspace, workspace_bytes, s);
-    case SPECKV_BF16: return launch_paged<__nv_bfloat16>(a, dtype, workspace, workspace_bytes, s);
-    default: return launch_paged<__half>(a, dtype, workspace, workspace_bytes, s);
+    case SPECKV_F32: return launch_paged<float>(a, workspace, workspace_bytes, s);
+    case SPECKV_BF16: return launch_paged<__nv_bfloat16>(a, workspace, workspace_bytes, s);
+    default: return launch_paged<__half>(a, workspace, workspace_bytes, s);
   }
 }
 
 extern "C" int64_t speckv_paged_attention_workspace(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim,
                                                     int64_t table_pages, int64_t page_size, int32_t dtype) {
   if (batch < 1 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads != 0 || table_pages < 1 || page_size < 1 ||
-      table_pages > (1ll << 31) / page_size || !tensor_shape(dim, dtype))
+      table_pages > (1ll << 31) / page_size || !tensor_shape(dim))
     return 0;
-  return plan_launch(batch, q_heads, kv_heads, dim, table_pages * page_size, sm_count()).workspace;
+  const int64_t positions = table_pages * page_size;
+  return dtype == SPECKV_F32 ? plan_launch<float>(batch, q_heads, kv_heads, dim, positions, sm_count()).workspace
+                             : plan_launch<__half>(batch, q_heads, kv_heads, dim, positions, sm_count()).workspace;
 }

@@ -332,7 +332,7 @@ __device__ __forceinline__ void write_skipped(const ScoreArgs& a, long long n) {
   if (threadIdx.x == 0) {
     if (a.logprobs != nullptr) a.logprobs[n] = 0.f;
     a.entropy[n] = 0.f;
-    a.stats[2 * n] = a.stats[2 * n + 1] = 0.f;
+    if (a.stats != nullptr) a.stats[2 * n] = a.stats[2 * n + 1] = 0.f;
   }
   for (int j = threadIdx.x; j < a.top; j += blockDim.x) {
     a.top_logprobs[n * a.top + j] = 0.f;
@@ -615,8 +615,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
     if (tid == 0) {
       if (a.logprobs != nullptr) a.logprobs[n] = logprob(given);
       a.entropy[n] = bad ? NAN : empty ? 0.f : fmaxf(log_s - t / s, 0.f) * kLn2;
-      a.stats[2 * n] = bad ? NAN : r;
-      a.stats[2 * n + 1] = bad ? NAN : empty ? -INFINITY : log_s;
+      if (a.stats != nullptr) {
+        a.stats[2 * n] = bad ? NAN : r;
+        a.stats[2 * n + 1] = bad ? NAN : empty ? -INFINITY : log_s;
+      }
     }
     if (TOP) {
       const int k = a.top;
@@ -803,7 +805,7 @@ extern "C" int speckv_token_logprobs(const void* logits, int32_t dtype, int64_t 
   if (st || batch == 0 || per_batch == 0) return st;
   if (rows == nullptr && source_rows != per_batch)
     return fail(SPECKV_EINVAL, "%s: %lld rows of logits for %lld", fn, (long long)source_rows, (long long)per_batch);
-  if (logits == nullptr || entropy == nullptr || stats == nullptr || (tokens == nullptr) != (logprobs == nullptr) ||
+  if (logits == nullptr || entropy == nullptr || (tokens == nullptr) != (logprobs == nullptr) ||
       (top > 0 && (top_logprobs == nullptr || top_ids == nullptr)))
     return fail(SPECKV_EINVAL, "%s: null pointer", fn);
   st = check_current_device(fn, {logits, tokens, entropy});

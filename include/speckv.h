@@ -580,9 +580,10 @@ int speckv_paged_append(const void* key, const void* value, const void* query, v
 /* Attention of one new token per sequence over a paged cache:
  *   out[b][0][hq][:] = softmax_c(q[b][hq] . k_c * scale) v_c,   c < lengths[b]
  * with KV head hq / (q_heads / kv_heads). lengths is a device array of batch int64; a sequence of
- * length 0 (or less) gives zeros. out is contiguous (batch, 1, q_heads, dim). strides: 8 element
+ * length 0 (or less) gives zeros; an infinite value makes its output NaN. out is contiguous (batch, 1, q_heads, dim). strides: 8 element
  * strides, (b, h) of query and (page, head, position) of key_pages and value_pages. Head dims to
- * 256: 64, 128 and 256 in bf16 / fp16 with 16-byte aligned rows take the tensor-core kernel, which
+ * 256: 64, 128 and 256 with 16-byte aligned rows take the tensor-core kernels (fp32 in three tf32
+ * products, to 2^-22), which
  * cuts the live positions of all sequences into equal shares and joins what is cut, other views a
  * CUDA-core kernel. workspace (16-byte aligned, workspace_bytes at least
  * speckv_paged_attention_workspace of the same sizes on the same device; it holds nothing between
@@ -612,7 +613,7 @@ int64_t speckv_paged_attention_workspace(int64_t batch, int64_t q_heads, int64_t
  * whose token is >= vocab or whose source row is >= source_rows, which also sets device error
  * SPECKV_DERR_TOKEN_INDEX. A row of -inf alone: logprobs and top_logprobs -inf, entropy 0. A row
  * with a NaN or +inf: NaN. stats (2 fp32 a row: an entry r of the row and log2 sum_i
- * 2^((x_i - r) log2(e) inv_temperature)) is kept for the gradient. inv_temperature lies in
+ * 2^((x_i - r) log2(e) inv_temperature)), or NULL, is kept for the gradient. inv_temperature lies in
  * [1e-30, 1e30]. Without rows, source_rows == per_batch.
  * The numbers that the reference's sampler and GRPO loss take from the logits with log_softmax,
  * gather, argmax and topk (helper/opd_sampling.py:162-170, helper/fastgrpo_training.py). */

@@ -222,13 +222,14 @@ template <typename T, int D, int NT> struct Shape {
 // of that item in the workspace, and the CTA in whose share the item begins describes it for
 // the join.
 struct Join {
-  int b, h, slot, count;  // count 0: nothing to join; parts at `slot`, then slots 2 (c + 1), 2 (c + 2), ...
+  int b, h, slot, count;  // count 0: nothing to join; parts at `slot` of share slot / 2, then at slot 0 of each next share
 };
 
 struct PlanArgs {
   float* parts;   // (2 * CTAs) x [8 NT][dim + 2]: sums, reference, total
-  Join* joins;    // one per CTA
+  Join* joins;    // one per item where there are fewer items than CTAs (by_item), else one per CTA
   int chunks;     // items per (sequence, KV head)
+  int by_item;
 };
 
 // What a CTA's warps leave of an item, beside their sums.
@@ -793,9 +794,12 @@ __global__ void __launch_bounds__(Shape<T, D, NT>::kWarps * 32, Shape<T, D, NT>:
 
   // sequences with nothing to see
   for (long long b = cta; b < a.batch; b += G)
-    if (live_length(a, b) == 0)
+    if (live_length(a, b) == 0) {
+      if (plan.by_item)
+        for (long long i = threadIdx.x; i < per_seq; i += W * 32) plan.joins[b * per_seq + i] = Join{0, 0, 0, 0};
       for (long long i = threadIdx.x; i < a.q_heads * D; i += W * 32)
         static_cast<T*>(a.out)[b * a.q_heads * D + i] = store_f<T>(0.f);
+    }
 
   // tiles before each thread's run of sequences, and in all
   const long long run = (a.batch + W * 32 - 1) / (W * 32);
@@ -822,7 +826,7 @@ __global__ void __launch_bounds__(Shape<T, D, NT>::kWarps * 32, Shape<T, D, NT>:
   const long long lo = cta < shares ? cta * total / shares : total;
   const long long hi = cta < shares ? (cta + 1) * total / shares : total;
   if (lo >= hi) {
-    if (threadIdx.x == 0) plan.joins[cta] = Join{0, 0, 0, 0};
+    if (threadIdx.x == 0 && !plan.by_item) plan.joins[cta] = Join{0, 0, 0, 0};
     return;
   }
   // the sequence of tile `lo`
@@ -862,6 +866,7 @@ __global__ void __launch_bounds__(Shape<T, D, NT>::kWarps * 32, Shape<T, D, NT>:
       const long long last = ((item + nb) * shares - 1) / total;  // the share that holds the item's last tile
       join = Join{(int)b, h, slot, (int)(last - cta) + 1};
     }
+    if (t0 == 0 && plan.by_item && threadIdx.x == 0) plan.joins[b * per_seq + h] = t1 < nb ? join : Join{0, 0, 0, 0};
     T* out = static_cast<T*>(a.out) + (b * a.q_heads + hk * group + h0) * D;
     attend_part<T, D, NT, PAGE16>(a, shared, sm, b, hk, h0, heads, t0, end, [&](int head, int d, float sum, float top, float all) {
       if (whole) {
@@ -877,7 +882,7 @@ __global__ void __launch_bounds__(Shape<T, D, NT>::kWarps * 32, Shape<T, D, NT>:
     at = item + t1;
     first_segment = false;
   }
-  if (threadIdx.x == 0) plan.joins[cta] = join;
+  if (threadIdx.x == 0 && !plan.by_item) plan.joins[cta] = join;
 }
 
 // Few items: a cluster of CTAs each, an equal run of its tiles per CTA, joined through the
@@ -936,29 +941,28 @@ __global__ void __launch_bounds__(Shape<T, D, NT>::kWarps * 32, Shape<T, D, NT>:
 }
 
 // Joins the parts of the items that more than one share holds, in the order of the shares: CTA per
-// (share, query head of the item that begins in it); its warps take every fourth part each.
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(128) paged_attention_join_kernel(PagedArgs a, PlanArgs plan) {
+// (entry of the joins, query head of its item); its WARPS warps take every WARPS-th part each.
+template <typename T, int D, int NT, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) paged_attention_join_kernel(PagedArgs a, PlanArgs plan) {
   constexpr int PART = 8 * NT * (D + 2), E = D / 32, BATCH = 4;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Join j = plan.joins[blockIdx.x];
   const int group = (int)(a.q_heads / a.kv_heads), head = blockIdx.y;
   const int hk = j.h / plan.chunks, h0 = (j.h - hk * plan.chunks) * 8 * NT;
   if (j.count == 0 || h0 + head >= group) return;
-  __shared__ float s_top[4], s_all[4], s_sum[4][D];
+  __shared__ float s_top[WARPS], s_all[WARPS], s_sum[WARPS][D];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // part 0 is at its own slot, part k >= 1 the first of share blockIdx.x + k
   auto part = [&](int k) {
-    return plan.parts + (long long)(k == 0 ? j.slot : 2 * ((int)blockIdx.x + k)) * PART;
+    return plan.parts + (long long)(k == 0 ? j.slot : 2 * (j.slot / 2 + k)) * PART;
   };
   float top = -INFINITY, all = 0.f, sum[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) sum[e] = 0.f;
-  for (int k0 = warp; k0 < j.count; k0 += 4 * BATCH) {
+  for (int k0 = warp; k0 < j.count; k0 += WARPS * BATCH) {
     float m[BATCH], l[BATCH], v[BATCH][E];
 #pragma unroll
     for (int i = 0; i < BATCH; ++i) {
-      const int k = k0 + 4 * i;
+      const int k = k0 + WARPS * i;
       m[i] = -INFINITY;
       if (k < j.count) {
         const float* p = part(k);
@@ -977,7 +981,7 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(PagedArgs a, 
     for (int e = 0; e < E; ++e) sum[e] *= keep;
 #pragma unroll
     for (int i = 0; i < BATCH; ++i)
-      if (k0 + 4 * i < j.count) {
+      if (k0 + WARPS * i < j.count) {
         const float f = exp2f(m[i] - ref);
         all = fmaf(l[i], f, all);
 #pragma unroll
@@ -992,19 +996,21 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(PagedArgs a, 
 #pragma unroll
   for (int e = 0; e < E; ++e) s_sum[warp][lane + 32 * e] = sum[e];
   __syncthreads();
-  top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
-  const float ref = top == -INFINITY ? 0.f : top;
-  float f[4], total = 0.f;
+  top = s_top[0];
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 1; w < WARPS; ++w) top = fmaxf(top, s_top[w]);
+  const float ref = top == -INFINITY ? 0.f : top;
+  float f[WARPS], total = 0.f;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
     f[w] = exp2f(s_top[w] - ref);
     total = fmaf(s_all[w], f[w], total);
   }
   T* out = static_cast<T*>(a.out) + (j.b * a.q_heads + hk * group + h0 + head) * D;
-  for (int d = threadIdx.x; d < D; d += 128) {
+  for (int d = threadIdx.x; d < D; d += WARPS * 32) {
     float o = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) o = fmaf(s_sum[w][d], f[w], o);
+    for (int w = 0; w < WARPS; ++w) o = fmaf(s_sum[w][d], f[w], o);
     out[d] = store_f<T>(total == 0.f ? 0.f : o / total);
   }
 }
@@ -1090,12 +1096,15 @@ int launch_shares(const PagedArgs& a, const PlanArgs& plan, int ctas, cudaStream
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas, (unsigned)min((int)(a.q_heads / a.kv_heads), 8 * NT));
-  cfg.blockDim = dim3(128);
+  const int entries = plan.by_item ? (int)(a.batch * a.kv_heads * plan.chunks) : ctas;
+  const bool many = ctas > 16 * entries;  // parts of an item: 16 warps join them faster than 4
+  cfg.gridDim = dim3(entries, (unsigned)min((int)(a.q_heads / a.kv_heads), 8 * NT));
+  cfg.blockDim = dim3(many ? 512 : 128);
   cfg.stream = s;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<T, D, NT>, a, plan);
+  e = many ? cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<T, D, NT, 16>, a, plan)
+           : cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<T, D, NT, 4>, a, plan);
   return e == cudaSuccess ? SPECKV_OK : launch_failed(e);
 }
 
@@ -1125,6 +1134,7 @@ template <typename T, int D, int NT>
 int launch_tensor(const PagedArgs& a, const Launch& l, void* workspace, cudaStream_t s) {
   PlanArgs plan;
   plan.chunks = l.chunks;
+  plan.by_item = 0;
   plan.joins = static_cast<Join*>(workspace);
   plan.parts = reinterpret_cast<float*>(plan.joins + l.full);
   const bool page16 = a.table.page_size % 16 == 0;
@@ -1134,6 +1144,7 @@ int launch_tensor(const PagedArgs& a, const Launch& l, void* workspace, cudaStre
   // no more CTAs than shares of the longest sequences possible
   const double most = (double)l.items * (double)l.tiles / kMinTiles;
   const int ctas = most < l.full ? (int)most + 1 : l.full;
+  plan.by_item = l.items < ctas;
   return page16 ? launch_shares<T, D, NT, true>(a, plan, ctas, s) : launch_shares<T, D, NT, false>(a, plan, ctas, s);
 }
 

@@ -203,16 +203,17 @@ constexpr int kCluster = 8;          // CTAs of a cluster at most
 constexpr int kClusterTiles = 12;    // tiles of a cluster's CTA at most
 constexpr float kSlack = 8.f;        // scores may pass the running reference by 2^8 before it moves
 
-// Warps of a CTA, CTAs per SM (by registers in 16 bits, by the rings in fp32) and shared memory.
-template <typename T, int D, int NT> struct Shape {
+// Warps of a CTA, CTAs per SM (by registers in 16 bits, by the rings in fp32) and shared memory. WIDE:
+// 16 bits, twice the warps.
+template <typename T, int D, int NT, bool WIDE = false> struct Shape {
   static constexpr bool kHalf = sizeof(T) == 2;
   static constexpr int kRow = D * (int)sizeof(T);      // bytes of a key row
   static constexpr int kStages = 3;                    // fp32: blocks of K or V under way per warp
-  static constexpr int kWarps = kHalf || D == 256 ? 4 : 8;
+  static constexpr int kWarps = (kHalf && !WIDE) || (!kHalf && D == 256) ? 4 : 8;
   static constexpr int kRing = kHalf ? 0 : kWarps * kStages * 16 * kRow;
   static constexpr int kSums = kWarps * 8 * (D + 4) * 4;
   static constexpr int kShared = kRing > kSums ? kRing : kSums;
-  static constexpr int kResident = !kHalf ? (D == 64 ? 2 : 1)
+  static constexpr int kResident = WIDE ? 1 : !kHalf ? (D == 64 ? 2 : 1)
                                    : D == 64 ? (NT == 1 ? 4 : 3) : D == 128 && NT == 1 ? 3 : 2;
   static constexpr int kTile = 16 * kWarps;            // keys of a tile: a block a warp
 };
@@ -297,11 +298,11 @@ __device__ __forceinline__ void join_warps(unsigned char* shared, Parts<W, NT>& 
 // two keys' chunks of V give theirs by byte permutes. 8 KB a warp are under way, 12 warps on an SM.
 // (Copied ahead through shared memory instead, 8 warps, the same work took 6 to 16 % longer.)
 // One CTA's part of an item: tiles [t0, ...) of its keys up to position `end`.
-template <typename T, int D, int NT, bool PAGE16, typename Emit>
+template <typename T, int D, int NT, bool PAGE16, bool WIDE, typename Emit>
 __device__ __forceinline__ void attend_part16(const PagedArgs& a, unsigned char* shared,
-                                              Parts<Shape<T, D, NT>::kWarps, NT>& sm, long long b, int hk, int h0,
+                                              Parts<Shape<T, D, NT, WIDE>::kWarps, NT>& sm, long long b, int hk, int h0,
                                               int heads, int t0, long long end, Emit emit) {
-  typedef Shape<T, D, NT> S;
+  typedef Shape<T, D, NT, WIDE> S;
   constexpr int KC = D / 32;  // 16-byte chunks of a key row per lane
   constexpr int VC = D / 64;  // 16-byte chunks of a value row per lane
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -765,12 +766,12 @@ __device__ __forceinline__ void attend_part32(const PagedArgs& a, unsigned char*
   }, emit);
 }
 
-template <typename T, int D, int NT, bool PAGE16, typename Emit>
+template <typename T, int D, int NT, bool PAGE16, bool WIDE, typename Emit>
 __device__ __forceinline__ void attend_part(const PagedArgs& a, unsigned char* shared,
-                                            Parts<Shape<T, D, NT>::kWarps, NT>& sm, long long b, int hk, int h0, int heads,
+                                            Parts<Shape<T, D, NT, WIDE>::kWarps, NT>& sm, long long b, int hk, int h0, int heads,
                                             int t0, long long end, Emit emit) {
   if constexpr (sizeof(T) == 2)
-    attend_part16<T, D, NT, PAGE16>(a, shared, sm, b, hk, h0, heads, t0, end, emit);
+    attend_part16<T, D, NT, PAGE16, WIDE>(a, shared, sm, b, hk, h0, heads, t0, end, emit);
   else
     attend_part32<D, NT, PAGE16>(a, shared, sm, b, hk, h0, heads, t0, end, emit);
 }
@@ -868,7 +869,7 @@ __global__ void __launch_bounds__(Shape<T, D, NT>::kWarps * 32, Shape<T, D, NT>:
     }
     if (t0 == 0 && plan.by_item && threadIdx.x == 0) plan.joins[b * per_seq + h] = t1 < nb ? join : Join{0, 0, 0, 0};
     T* out = static_cast<T*>(a.out) + (b * a.q_heads + hk * group + h0) * D;
-    attend_part<T, D, NT, PAGE16>(a, shared, sm, b, hk, h0, heads, t0, end, [&](int head, int d, float sum, float top, float all) {
+    attend_part<T, D, NT, PAGE16, false>(a, shared, sm, b, hk, h0, heads, t0, end, [&](int head, int d, float sum, float top, float all) {
       if (whole) {
         out[head * D + d] = store_f<T>(all == 0.f ? 0.f : sum / all);
       } else {
@@ -886,11 +887,13 @@ __global__ void __launch_bounds__(Shape<T, D, NT>::kWarps * 32, Shape<T, D, NT>:
 }
 
 // Few items: a cluster of CTAs each, an equal run of its tiles per CTA, joined through the
-// cluster's shared memory. One launch, no workspace.
-template <typename T, int D, int NT, bool PAGE16>
-__global__ void __launch_bounds__(Shape<T, D, NT>::kWarps * 32, Shape<T, D, NT>::kResident)
+// cluster's shared memory. One launch, no workspace. Where each of
+// its CTAs has an SM to itself, eight warps share the work (WIDE): one warp per scheduler leaves
+// most of the issue slots empty.
+template <typename T, int D, int NT, bool PAGE16, bool WIDE>
+__global__ void __launch_bounds__(Shape<T, D, NT, WIDE>::kWarps * 32, Shape<T, D, NT, WIDE>::kResident)
     paged_attention_cluster_kernel(PagedArgs a, PlanArgs plan) {
-  constexpr int W = Shape<T, D, NT>::kWarps, kTile = Shape<T, D, NT>::kTile;
+  constexpr int W = Shape<T, D, NT, WIDE>::kWarps, kTile = Shape<T, D, NT, WIDE>::kTile;
   extern __shared__ __align__(128) unsigned char shared[];
   __shared__ Parts<W, NT> sm;
   __shared__ float s_sum[8 * NT][D], s_top[8 * NT], s_all[8 * NT];
@@ -902,7 +905,7 @@ __global__ void __launch_bounds__(Shape<T, D, NT>::kWarps * 32, Shape<T, D, NT>:
   const int hk = h / plan.chunks, h0 = (h - hk * plan.chunks) * 8 * NT, heads = min((int)group - h0, 8 * NT);
   const long long n = live_length(a, b), nb = (n + kTile - 1) / kTile;
   const int t0 = (int)(nb * rank / ctas), t1 = (int)(nb * (rank + 1) / ctas);
-  attend_part<T, D, NT, PAGE16>(a, shared, sm, b, hk, h0, heads, t0, min(n, (long long)t1 * kTile),
+  attend_part<T, D, NT, PAGE16, WIDE>(a, shared, sm, b, hk, h0, heads, t0, min(n, (long long)t1 * kTile),
                                 [&](int head, int d, float sum, float top, float all) {
                                   s_sum[head][d] = sum;
                                   if (d == 0) {
@@ -1046,7 +1049,7 @@ int cluster_ctas(long long items, long long tiles, int full) {
 
 // How a tensor shape is launched, from sizes that the host knows.
 struct Launch {
-  int tiles8, chunks, full, cluster;  // NT; items per (sequence, KV head); CTAs resident; CTAs per item or 0
+  int sms, tiles8, chunks, full, cluster;  // NT; items per (sequence, KV head); CTAs resident; CTAs per item or 0
   long long items, tiles;             // tiles of the longest sequence that the table can hold
   int64_t workspace;
 };
@@ -1054,6 +1057,7 @@ struct Launch {
 template <typename T>
 Launch plan_launch(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t positions, int sms) {
   Launch l;
+  l.sms = sms;
   const int64_t group = q_heads / kv_heads;
   l.tiles8 = head_tiles(dim, group);
   int resident, tile;
@@ -1108,11 +1112,11 @@ int launch_shares(const PagedArgs& a, const PlanArgs& plan, int ctas, cudaStream
   return e == cudaSuccess ? SPECKV_OK : launch_failed(e);
 }
 
-template <typename T, int D, int NT, bool PAGE16>
+template <typename T, int D, int NT, bool PAGE16, bool WIDE>
 int launch_clusters(const PagedArgs& a, const PlanArgs& plan, int items, int ctas, cudaStream_t s) {
-  typedef Shape<T, D, NT> S;
+  typedef Shape<T, D, NT, WIDE> S;
   static bool done[64] = {false};
-  auto kernel = paged_attention_cluster_kernel<T, D, NT, PAGE16>;
+  auto kernel = paged_attention_cluster_kernel<T, D, NT, PAGE16, WIDE>;
   cudaError_t e = allow_shared(kernel, S::kShared, done);
   if (e != cudaSuccess) return launch_failed(e);
   cudaLaunchAttribute attr;
@@ -1138,9 +1142,15 @@ int launch_tensor(const PagedArgs& a, const Launch& l, void* workspace, cudaStre
   plan.joins = static_cast<Join*>(workspace);
   plan.parts = reinterpret_cast<float*>(plan.joins + l.full);
   const bool page16 = a.table.page_size % 16 == 0;
+  // Wide CTAs have an SM each, and clusters of eight do not fill all of them: at 96 CTAs or fewer they
+  // all run at once (12.4 us instead of 15.3, 6 x 4000 keys of 16 / 2 heads), 128 took two turns (19.4, 15.8).
+  constexpr bool can = sizeof(T) == 2;
+  if (l.cluster > 0 && can && l.items * l.cluster * 3 <= l.sms * 2)
+    return page16 ? launch_clusters<T, D, NT, true, can>(a, plan, (int)l.items, l.cluster, s)
+                  : launch_clusters<T, D, NT, false, can>(a, plan, (int)l.items, l.cluster, s);
   if (l.cluster > 0)
-    return page16 ? launch_clusters<T, D, NT, true>(a, plan, (int)l.items, l.cluster, s)
-                  : launch_clusters<T, D, NT, false>(a, plan, (int)l.items, l.cluster, s);
+    return page16 ? launch_clusters<T, D, NT, true, false>(a, plan, (int)l.items, l.cluster, s)
+                  : launch_clusters<T, D, NT, false, false>(a, plan, (int)l.items, l.cluster, s);
   // no more CTAs than shares of the longest sequences possible
   const double most = (double)l.items * (double)l.tiles / kMinTiles;
   const int ctas = most < l.full ? (int)most + 1 : l.full;

@@ -29,6 +29,14 @@ __device__ __forceinline__ float remote_float(const void* p, uint32_t rank) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(remote(p, rank)) : "memory");
   return x;
 }
+__device__ __forceinline__ float4 remote_float4(const void* p, uint32_t rank) {
+  float4 x;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+               : "r"(remote(p, rank))
+               : "memory");
+  return x;
+}
 __device__ __forceinline__ unsigned long long remote_u64(const void* p, uint32_t rank) {
   unsigned long long x;
   asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(x) : "r"(remote(p, rank)) : "memory");

@@ -239,8 +239,16 @@ template <int W, int NT> struct Parts {
   float top[8 * NT], all[8 * NT];  // of all warps
 };
 
+// Four outputs: sums over their total, zeros where there is nothing to see.
+template <typename T> __device__ __forceinline__ void store_four(T* to, const float4& sum, float all) {
+  const float x[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) to[i] = store_f<T>(all == 0.f ? 0.f : x[i] / all);
+}
+
 // Joins the warps' parts of an item: own(u, e, f, to) writes the lane's sums of head 8 u + 2 t + e,
-// times f, to that head's row; emit(head of the item, dim, sum, reference, total) gets the outcome.
+// times f, to that head's row; emit(head of the item, dim, sums of four dims, reference, total) gets
+// the outcome.
 template <int D, int NT, int W, typename Own, typename Emit>
 __device__ __forceinline__ void join_warps(unsigned char* shared, Parts<W, NT>& sm, float (&m)[NT][2], float (&l)[NT][2],
                                            int heads, Own own, Emit emit) {
@@ -281,12 +289,15 @@ __device__ __forceinline__ void join_warps(unsigned char* shared, Parts<W, NT>& 
       own(u, e, f, sums[warp][2 * t + e]);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < 8 * D; i += W * 32) {
-      const int head = i / D, d = i - head * D;
+    for (int i = threadIdx.x; i < 2 * D; i += W * 32) {  // four dims each
+      const int head = 4 * i / D, d = 4 * i - head * D;
       if (u * 8 + head >= heads) break;
-      float sum = 0.f;
+      float4 sum = *reinterpret_cast<const float4*>(&sums[0][head][d]);
 #pragma unroll
-      for (int w = 0; w < W; ++w) sum += sums[w][head][d];
+      for (int w = 1; w < W; ++w) {
+        const float4 more = *reinterpret_cast<const float4*>(&sums[w][head][d]);
+        sum.x += more.x, sum.y += more.y, sum.z += more.z, sum.w += more.w;
+      }
       emit(u * 8 + head, d, sum, sm.top[u * 8 + head], sm.all[u * 8 + head]);
     }
     __syncthreads();
@@ -869,11 +880,11 @@ __global__ void __launch_bounds__(Shape<T, D, NT>::kWarps * 32, Shape<T, D, NT>:
     }
     if (t0 == 0 && plan.by_item && threadIdx.x == 0) plan.joins[b * per_seq + h] = t1 < nb ? join : Join{0, 0, 0, 0};
     T* out = static_cast<T*>(a.out) + (b * a.q_heads + hk * group + h0) * D;
-    attend_part<T, D, NT, PAGE16, false>(a, shared, sm, b, hk, h0, heads, t0, end, [&](int head, int d, float sum, float top, float all) {
+    attend_part<T, D, NT, PAGE16, false>(a, shared, sm, b, hk, h0, heads, t0, end, [&](int head, int d, const float4& sum, float top, float all) {
       if (whole) {
-        out[head * D + d] = store_f<T>(all == 0.f ? 0.f : sum / all);
+        store_four(out + head * D + d, sum, all);
       } else {
-        part[head * D + d] = sum;
+        *reinterpret_cast<float4*>(part + head * D + d) = sum;
         if (d == 0) {
           part[8 * NT * D + head] = top;
           part[8 * NT * (D + 1) + head] = all;
@@ -896,7 +907,8 @@ __global__ void __launch_bounds__(Shape<T, D, NT, WIDE>::kWarps * 32, Shape<T, D
   constexpr int W = Shape<T, D, NT, WIDE>::kWarps, kTile = Shape<T, D, NT, WIDE>::kTile;
   extern __shared__ __align__(128) unsigned char shared[];
   __shared__ Parts<W, NT> sm;
-  __shared__ float s_sum[8 * NT][D], s_top[8 * NT], s_all[8 * NT];
+  __shared__ __align__(16) float s_sum[8 * NT][D];
+  __shared__ float s_top[8 * NT], s_all[8 * NT];
   const uint32_t ctas = cluster_size(), rank = cluster_rank();
   const long long group = a.q_heads / a.kv_heads, per_seq = a.kv_heads * plan.chunks;
   const uint32_t index = blockIdx.x / ctas;
@@ -906,8 +918,8 @@ __global__ void __launch_bounds__(Shape<T, D, NT, WIDE>::kWarps * 32, Shape<T, D
   const long long n = live_length(a, b), nb = (n + kTile - 1) / kTile;
   const int t0 = (int)(nb * rank / ctas), t1 = (int)(nb * (rank + 1) / ctas);
   attend_part<T, D, NT, PAGE16, WIDE>(a, shared, sm, b, hk, h0, heads, t0, min(n, (long long)t1 * kTile),
-                                [&](int head, int d, float sum, float top, float all) {
-                                  s_sum[head][d] = sum;
+                                [&](int head, int d, const float4& sum, float top, float all) {
+                                  *reinterpret_cast<float4*>(&s_sum[head][d]) = sum;
                                   if (d == 0) {
                                     s_top[head] = top;
                                     s_all[head] = all;
@@ -916,29 +928,32 @@ __global__ void __launch_bounds__(Shape<T, D, NT, WIDE>::kWarps * 32, Shape<T, D
   cluster_sync();
   // each CTA joins its share of the outputs
   T* out = static_cast<T*>(a.out) + (b * a.q_heads + hk * group + h0) * D;
-  for (int i = rank * W * 32 + threadIdx.x; i < heads * D; i += ctas * W * 32) {
-    const int head = i / D, d = i - head * D;
-    float top[kCluster], all[kCluster], sum[kCluster], ref = -INFINITY;
+  for (int i = rank * W * 32 + threadIdx.x; i < heads * D / 4; i += ctas * W * 32) {
+    const int head = 4 * i / D, d = 4 * i - head * D;
+    float top[kCluster], all[kCluster], ref = -INFINITY;
+    float4 sum[kCluster];
 #pragma unroll
     for (int r = 0; r < kCluster; ++r)
       if (r < ctas) {
         top[r] = remote_float(&s_top[head], r);
         all[r] = remote_float(&s_all[head], r);
-        sum[r] = remote_float(&s_sum[head][d], r);
+        sum[r] = remote_float4(&s_sum[head][d], r);
       }
 #pragma unroll
     for (int r = 0; r < kCluster; ++r)
       if (r < ctas) ref = fmaxf(ref, top[r]);
     if (ref == -INFINITY) ref = 0.f;
-    float o = 0.f, total = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float total = 0.f;
 #pragma unroll
     for (int r = 0; r < kCluster; ++r)
       if (r < ctas) {
         const float f = exp2f(top[r] - ref);
         total = fmaf(all[r], f, total);
-        o = fmaf(sum[r], f, o);
+        o.x = fmaf(sum[r].x, f, o.x), o.y = fmaf(sum[r].y, f, o.y);
+        o.z = fmaf(sum[r].z, f, o.z), o.w = fmaf(sum[r].w, f, o.w);
       }
-    out[i] = store_f<T>(total == 0.f ? 0.f : o / total);
+    store_four(out + 4 * i, o, total);
   }
   cluster_sync();  // the other CTAs' shared memory is read until here
 }

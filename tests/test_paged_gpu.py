@@ -178,8 +178,9 @@ def test_append_reports_what_it_cannot_place(dim):
 def filled(batch, hkv, dim, page, lengths, dtype, g, scale=1.0, extra=2, slack=0):
     """Pools that hold NaN wherever no live position is, and the table (entries past the length: -7)."""
     per = max(1, max(-(-n // page) for n in lengths)) + slack
-    kp, vp = pools(batch * per + extra, hkv, page, dim, dtype, g)
-    order = torch.randperm(batch * per + extra, device='cuda', generator=g)
+    total = batch * (per - slack) + extra
+    kp, vp = pools(total, hkv, page, dim, dtype, g)
+    order = torch.randperm(total, device='cuda', generator=g)
     table = torch.full((batch, per), -7, dtype=torch.long, device='cuda')
     at = 0
     for b, n in enumerate(lengths):
@@ -222,15 +223,18 @@ def check_attention(out, q, kp, vp, table, lengths, scale, page, dtype):
     (40, 8, 128, 128, [4097]), (8, 8, 64, 32, [5, 90, 0, 31, 32, 257]), (12, 1, 128, 16, [100, 1500]),
     (16, 1, 64, 16, [77, 300]), (4, 2, 256, 16, [1, 19, 500]), (20, 1, 128, 32, [40, 333]), (32, 1, 256, 64, [130]),
     (6, 2, 128, 1, [50, 3]), (5, 1, 64, 3, [1, 100, 7]), (7, 7, 128, 24, [230, 24, 25]), (14, 2, 128, 8, [64, 9]),
+    (8, 1, 128, 32, list(range(1, 75, 2))), (4, 4, 64, 16, [700, 0, 90] * 5), (2, 2, 256, 8, [300] * 23),
     (6, 2, 40, 16, [19, 100]), (3, 1, 80, 5, [33, 0, 4]), (2, 2, 192, 16, [70]), (1, 1, 8, 2, [9])])
 def test_attention_over_pages(hq, hkv, dim, page, lengths, dtype):
-    g = gen(hq * 7 + page)
     batch = len(lengths)
-    kp, vp, table = filled(batch, hkv, dim, page, lengths, dtype, g)
-    q = randn(batch, 1, hq * dim, dtype=dtype, g=g).view(batch, 1, hq, dim).transpose(1, 2)
-    out = paged_attention(q, kp, vp, table, torch.tensor(lengths, device='cuda'))
-    check_attention(out, q, kp, vp, table, lengths, dim ** -0.5, page, dtype)
-    assert _ops.device_error() is None
+    # a table as wide as the lengths (a cluster per item), and one of 13000 positions (equal shares)
+    for slack in (0, -(-13000 // page)):
+        g = gen(hq * 7 + page)
+        kp, vp, table = filled(batch, hkv, dim, page, lengths, dtype, g, slack=slack)
+        q = randn(batch, 1, hq * dim, dtype=dtype, g=g).view(batch, 1, hq, dim).transpose(1, 2)
+        out = paged_attention(q, kp, vp, table, torch.tensor(lengths, device='cuda'))
+        check_attention(out, q, kp, vp, table, lengths, dim ** -0.5, page, dtype)
+        assert _ops.device_error() is None
 
 
 @pytest.mark.parametrize('hq,hkv,batch', [(8, 1, 1), (16, 2, 3), (4, 4, 40), (28, 4, 70)])
@@ -356,14 +360,18 @@ def test_pools_beyond_32_bit_offsets():
     assert _ops.device_error() is None
 
 
-def test_streams_and_graphs():
-    """A side stream, and two captured graphs of the same buffers replayed on two streams at once."""
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('slack', [0, 800])
+def test_streams_and_graphs(dtype, slack):
+    """A side stream, and two captured graphs of the same buffers replayed on two streams at once,
+    with a cluster per item and with equal shares and their join."""
     g = gen(10)
     lengths = [3000, 17, 900]
-    kp, vp, table = filled(3, 2, 128, 16, lengths, torch.bfloat16, g)
+    kp, vp, table = filled(3, 2, 128, 16, lengths, dtype, g, slack=slack)
     n = torch.tensor(lengths, device='cuda')
-    qs = [randn(3, 16, 1, 128, dtype=torch.bfloat16, g=g) for _ in range(2)]
+    qs = [randn(3, 16, 1, 128, dtype=dtype, g=g) for _ in range(2)]
     want = [paged_attention(q, kp, vp, table, n) for q in qs]
+    check_attention(want[0], qs[0], kp, vp, table, lengths, 128 ** -0.5, 16, dtype)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -389,7 +397,7 @@ def test_streams_and_graphs():
     n.copy_(torch.tensor([5, 1, 0]))  # lengths are read on the device at each replay
     graphs[0].replay()
     torch.cuda.synchronize()
-    check_attention(outs[0], qs[0], kp, vp, table, [5, 1, 0], 128 ** -0.5, 16, torch.bfloat16)
+    check_attention(outs[0], qs[0], kp, vp, table, [5, 1, 0], 128 ** -0.5, 16, dtype)
 
 
 def test_empty_calls():

@@ -670,13 +670,25 @@ __global__ void __launch_bounds__(kGradThreads) token_logprobs_backward_kernel(S
     return;
   }
   const T* x = static_cast<const T*>(a.logits) + offset;
-  const bool aligned = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(g)) & 31) == 0;
+  // The gradient's vectors are aligned; the logits' lie alike, or (a view such as logits[:, :-1]) only
+  // their words do, or not even those.
+  const uintptr_t apart = (reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(g)) & 31;
+  const bool in_words = (apart & 3) == 0;
   Bytes32 in[kGradSpan];
-  if (aligned) {
+  if (in_words) {
 #pragma unroll
-    for (int k = 0; k < kGradSpan; ++k)
-      if (lo + tid + k * kGradThreads < hi)
-        in[k] = load_stream(x + row.head + (long long)(lo + tid + k * kGradThreads) * N);
+    for (int k = 0; k < kGradSpan; ++k) {
+      const int i = lo + tid + k * kGradThreads;
+      if (i < hi) {
+        const T* from = x + row.head + (long long)i * N;
+        if (apart == 0) {
+          in[k] = load_stream(from);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) in[k].w[e] = __ldg(reinterpret_cast<const uint32_t*>(from) + e);
+        }
+      }
+    }
   }
   const float ga = a.g_logprobs != nullptr ? a.g_logprobs[n] : 0.f;
   const float gh = a.g_entropy != nullptr ? a.g_entropy[n] : 0.f;
@@ -689,7 +701,7 @@ __global__ void __launch_bounds__(kGradThreads) token_logprobs_backward_kernel(S
     const float y = fmaxf(fmaf(z - r, c, -log_s), kEmpty);  // -inf: weight 0, not 0 x inf
     return exp2_fast(y) * fmaf(v, y, u);
   };
-  if (aligned) {
+  if (in_words) {
 #pragma unroll
     for (int k = 0; k < kGradSpan; ++k) {
       const int i = lo + tid + k * kGradThreads;

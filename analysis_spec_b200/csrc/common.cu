@@ -73,6 +73,15 @@ int check_current_device(const char* fn, std::initializer_list<const void*> ptrs
   return SPECKV_OK;
 }
 
+int sm_count() {
+  static int counts[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  if (counts[dev] == 0 && cudaDeviceGetAttribute(&counts[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 0;
+  return counts[dev];
+}
+
 }  // namespace speckv
 
 extern "C" int speckv_version(void) { return 100; }

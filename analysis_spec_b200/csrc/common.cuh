@@ -20,6 +20,9 @@ int fail(int code, const char* fmt, ...);
 // Returns SPECKV_OK or SPECKV_ECUDA (with message) for the last launch.
 int check_launch(const char* what);
 
+// SMs of the current device; 0 when it cannot be found.
+int sm_count();
+
 // Device address of the library's error word on the current device.
 unsigned long long* device_error_word();
 

@@ -1033,15 +1033,6 @@ __global__ void __launch_bounds__(WARPS * 32) paged_attention_join_kernel(PagedA
   }
 }
 
-int sm_count() {
-  static int counts[64] = {0};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-  if (counts[dev] == 0 && cudaDeviceGetAttribute(&counts[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 0;
-  return counts[dev];
-}
-
 template <typename T> void shape_of(int64_t dim, int nt, int& resident, int& tile) {
   if (dim == 64) resident = nt == 1 ? Shape<T, 64, 1>::kResident : Shape<T, 64, 2>::kResident, tile = Shape<T, 64, 1>::kTile;
   else if (dim == 128) resident = nt == 1 ? Shape<T, 128, 1>::kResident : Shape<T, 128, 2>::kResident, tile = Shape<T, 128, 1>::kTile;

@@ -772,9 +772,18 @@ int launch_scores_as(const char* fn, const ScoreArgs& a, int ctas, cudaStream_t 
 template <typename T>
 int launch_scores(const char* fn, const ScoreArgs& a, cudaStream_t s) {
   const long long rows = a.batch * a.per, vectors = a.vocab * sizeof(T) / 32;
+  const int sms = sm_count();
+  if (sms == 0) return fail(SPECKV_ECUDA, "%s: no SM count", fn);
+  // A cluster per row while that makes no more than two CTAs an SM (four fit, but clusters do not pack:
+  // 148 x 151680 bf16 20.0 us, 28.7 with twice the CTAs) and leaves each thread a vector.
   int ctas = 1;
-  while (ctas < 8 && rows * ctas * 2 <= 592 && vectors / (ctas * 2) >= 256) ctas *= 2;
+  while (ctas < 8 && rows * ctas <= sms && vectors / (ctas * 2) >= 256) ctas *= 2;
   if (rows * ctas >= (1ll << 31)) return fail(SPECKV_ENOSUPPORT, "%s: too many rows", fn);
+  // What follows a row's last logit takes a CTA 2 to 6 us: at vocabularies to 128 K entries of 16 bits
+  // twice the CTAs of half the threads hide more of it (3904 x 32000 bf16, ten alternatives: 71 us
+  // instead of 86), longer rows want the wider CTA (900 x 151644 fp32: 109 us, 123 with 128 threads).
+  if (ctas == 1 && vectors <= 8192)
+    return a.top > 0 ? launch_scores_as<T, 128, true>(fn, a, 1, s) : launch_scores_as<T, 128, false>(fn, a, 1, s);
   return a.top > 0 ? launch_scores_as<T, 256, true>(fn, a, ctas, s) : launch_scores_as<T, 256, false>(fn, a, ctas, s);
 }
 

@@ -79,7 +79,7 @@ def some_logits(rows, vocab, dtype, g, banned=5):
 @pytest.mark.parametrize('rows,vocab,top,temperature', [
     (1, 1, 1, 1.0), (3, 2, 2, 1.0), (5, 7, 5, 0.5), (2, 97, 32, 1.0), (7, 1000, 10, 2.0), (4, 4099, 20, 0.7),
     (1, 32000, 10, 1.0), (40, 32000, 1, 1.3), (3, 151644, 10, 1.0), (300, 8192, 5, 1.0), (2, 151643, 32, 1.0),
-    (700, 513, 3, 1.0), (1, 300007, 4, 1.0), (33, 65536, 0, 1.0)])
+    (700, 513, 3, 1.0), (1, 300007, 4, 1.0), (33, 65536, 0, 1.0), (300, 151644, 10, 1.0), (100, 40000, 5, 1.0), (200, 65536, 7, 0.9)])
 def test_forward(rows, vocab, top, temperature, dtype):
     g = gen(rows + vocab)
     x = some_logits(rows, vocab, dtype, g)

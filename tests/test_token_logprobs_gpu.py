@@ -280,6 +280,32 @@ def test_gradient_against_the_formula(rows, vocab, top, temperature, dtype):
     assert _ops.device_error() is None
 
 
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('vocab,pitch', [(31, 33), (501, 501), (4099, 4100), (9001, 9015)])
+def test_gradient_of_views_at_any_offset(vocab, pitch, dtype):
+    """Logits whose entries lie 0 to 16 entries off the gradient's, words across each other included; the
+    entries around the view are NaN."""
+    g = gen(vocab)
+    tokens = torch.randint(0, vocab, (3,), device='cuda', generator=g)
+    ga, gh = (torch.randn(3, device='cuda', generator=g) for _ in range(2))
+    u = torch.finfo(dtype).eps / 2
+    small = 2.0 ** -25 if dtype == torch.float16 else 1e-38
+    for offset in (0, 1, 2, 3, 7, 8, 15, 16):
+        store = torch.full((3 * pitch + 32,), math.nan, dtype=dtype, device='cuda')
+        x = store[offset:offset + 3 * pitch].view(3, pitch)[:, :vocab]
+        x.copy_(some_logits(3, vocab, dtype, g))
+        leaf = x.detach().requires_grad_(True)
+        assert leaf.data_ptr() == x.data_ptr()
+        r = token_logprobs(leaf, tokens, temperature=0.9)
+        got, = torch.autograd.grad((r.logprobs, r.entropy), leaf, (ga, gh))
+        z = x.double() / 0.9
+        spread, e = bounds(z)
+        ref, size = reference_grad(x, tokens, None, 0.9, ga, gh, None)
+        tol = u * ref.abs() * 1.01 + size * ((1 + spread) * 3 * e)[:, None] + 2.0 ** -22 * (ref.abs() + size) + small
+        assert ((got.double() - ref).abs() <= tol).all(), (offset, (got.double() - ref).abs().max().item())
+    assert _ops.device_error() is None
+
+
 def test_gradient_against_differences():
     """Central differences of the kernel's own outputs in fp32: with a step of h the quotient is off by
     h^2 / 6 of a third derivative (at most 1 for log-probabilities, 1 + R for the entropy) and by the

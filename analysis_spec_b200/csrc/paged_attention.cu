@@ -36,7 +36,8 @@ __device__ __forceinline__ long long live_length(const PagedArgs& a, long long b
 constexpr int kScalarWarps = 8;
 constexpr int kScalarDims = 8;  // dims per lane: head dims to 256
 
-// CTA per (sequence, query head), a key per warp and step: any head dim to 256, stride, alignment.
+// CTA per (sequence, query head), a key per warp and step: any head dim to 256, stride, alignment. Reads
+// the cache once per query head and waits for each key: 30 times the time of the kernels below.
 template <typename T>
 __global__ void __launch_bounds__(kScalarWarps * 32) paged_attention_scalar_kernel(PagedArgs a) {
   const long long b = blockIdx.x / a.q_heads, hq = blockIdx.x % a.q_heads;
@@ -198,10 +199,25 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint3
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
+// 4 x 12000 keys, 16 q / 2 KV heads: 18.1 us at one tile and at two (half the parts), 20.3 at six.
 constexpr int kMinTiles = 2;         // a CTA's share is at least this many tiles
 constexpr int kCluster = 8;          // CTAs of a cluster at most
+// One launch beats two where the work is small (1 x 200 keys 8.2 us, 14.0 as shares) and still where a
+// CTA has 11 tiles (64 x 256..2048 23.7 us, 24.0); at 21 uneven lengths cost more (64 x 256..4000 37.9, 33.7).
 constexpr int kClusterTiles = 12;    // tiles of a cluster's CTA at most
-constexpr float kSlack = 8.f;        // scores may pass the running reference by 2^8 before it moves
+
+// Weights are 2^(score - reference). The reference need not be the maximum: any value near it keeps the
+// weights and sums well inside fp32, and the sums are divided by the total at the end. So it moves only
+// when a score passes it by more than kSlack, to kLow below that score. fp16 weights enter the
+// tensor cores in two parts above the type's smallest step, 2^-24: they are taken near the type's upper
+// end, 2^11 to 2^15, and what a weight loses is 2^-36 of the largest (2^-25 at a reference of the maximum:
+// 5000 keys of weight 2^-26 beside one of 1 came out 1.6 % low). bf16 and tf32 parts have fp32's range.
+template <typename T> struct Reference {
+  static constexpr float kLow = 0.f, kSlack = 8.f;
+};
+template <> struct Reference<__half> {
+  static constexpr float kLow = 11.f, kSlack = 15.f;
+};
 
 // Warps of a CTA, CTAs per SM (by registers in 16 bits, by the rings in fp32) and shared memory. WIDE:
 // 16 bits, twice the warps.
@@ -314,6 +330,7 @@ __device__ __forceinline__ void attend_part16(const PagedArgs& a, unsigned char*
                                               Parts<Shape<T, D, NT, WIDE>::kWarps, NT>& sm, long long b, int hk, int h0,
                                               int heads, int t0, long long end, Emit emit) {
   typedef Shape<T, D, NT, WIDE> S;
+  typedef Reference<T> R;
   constexpr int KC = D / 32;  // 16-byte chunks of a key row per lane
   constexpr int VC = D / 64;  // 16-byte chunks of a value row per lane
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -464,16 +481,13 @@ __device__ __forceinline__ void attend_part16(const PagedArgs& a, unsigned char*
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
       float t0m = fmaxf(s[u][0], s[u][2]), t1m = fmaxf(s[u][1], s[u][3]);
-      // The reference need not be the maximum: any value within 2^8 of it keeps every weight and
-      // sum well inside fp32, and the sums are divided by the total at the end. So it moves only
-      // when a score passes it by more than that (the first block moves it from -inf).
-      if (__any_sync(0xffffffffu, t0m > m[u][0] + kSlack || t1m > m[u][1] + kSlack)) {
+      if (__any_sync(0xffffffffu, t0m > m[u][0] + R::kSlack || t1m > m[u][1] + R::kSlack)) {  // the first block, from -inf
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) {
           t0m = fmaxf(t0m, __shfl_xor_sync(0xffffffffu, t0m, off));
           t1m = fmaxf(t1m, __shfl_xor_sync(0xffffffffu, t1m, off));
         }
-        const float n0 = fmaxf(m[u][0], t0m), n1 = fmaxf(m[u][1], t1m);
+        const float n0 = fmaxf(m[u][0], t0m - R::kLow), n1 = fmaxf(m[u][1], t1m - R::kLow);
         const float f0 = n0 == -INFINITY ? 1.f : exp2f(m[u][0] - n0);
         const float f1 = n1 == -INFINITY ? 1.f : exp2f(m[u][1] - n1);
         m[u][0] = n0;
@@ -496,7 +510,7 @@ __device__ __forceinline__ void attend_part16(const PagedArgs& a, unsigned char*
       l[u][0] += p0 + p2;
       l[u][1] += p1 + p3;
       // weights to (key pairs, heads) fragments, in two 16-bit parts: the tensor pipe has room
-      // for a second product, and one 8-bit weight alone would lose more than the output's rounding
+      // for a second product, and one of 8 bits alone would lose more than the output's rounding
       split_pair(p0, p1, ph[u][0], pl[u][0], T());
       split_pair(p2, p3, ph[u][1], pl[u][1], T());
 #pragma unroll
@@ -540,6 +554,7 @@ __device__ __forceinline__ void attend_part32(const PagedArgs& a, unsigned char*
                                               Parts<Shape<float, D, NT>::kWarps, NT>& sm, long long b, int hk, int h0,
                                               int heads, int t0, long long end, Emit emit) {
   typedef Shape<float, D, NT> S;
+  typedef Reference<float> R;
   constexpr int CHUNKS = S::kRow / 16, E = 4, BLOCK = 16 * S::kRow;
   constexpr int STEPS = D / (2 * E);      // products of a score: 8 dims each
   constexpr int ROWS = 32 / CHUNKS > 0 ? 32 / CHUNKS : 1;  // rows that one copy of a warp covers
@@ -713,16 +728,13 @@ __device__ __forceinline__ void attend_part32(const PagedArgs& a, unsigned char*
         for (int e = 0; e < 4; ++e)
           if (!(live >> (e >> 1) & 1u)) s[u][e] = -INFINITY;
       float top0 = fmaxf(s[u][0], s[u][2]), top1 = fmaxf(s[u][1], s[u][3]);
-      // The reference need not be the maximum: any value within 2^8 of it keeps every weight and
-      // sum well inside fp32, and the sums are divided by the total at the end. So it moves only
-      // when a score passes it by more than that (the first block moves it from -inf).
-      if (__any_sync(0xffffffffu, top0 > m[u][0] + kSlack || top1 > m[u][1] + kSlack)) {
+      if (__any_sync(0xffffffffu, top0 > m[u][0] + R::kSlack || top1 > m[u][1] + R::kSlack)) {
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) {
           top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, off));
           top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, off));
         }
-        const float n0 = fmaxf(m[u][0], top0), n1 = fmaxf(m[u][1], top1);
+        const float n0 = fmaxf(m[u][0], top0 - R::kLow), n1 = fmaxf(m[u][1], top1 - R::kLow);
         const float f0 = n0 == -INFINITY ? 1.f : exp2f(m[u][0] - n0);
         const float f1 = n1 == -INFINITY ? 1.f : exp2f(m[u][1] - n1);
         m[u][0] = n0;
@@ -791,6 +803,10 @@ __device__ __forceinline__ long long tiles_of(const PagedArgs& a, long long b, i
   return (live_length(a, b) + tile - 1) / tile;
 }
 
+// Equal shares of all sequences' tiles, one per resident CTA: no CTA waits for a longer sequence, and a
+// long cache is split as finely as the GPU is wide. Bound by memory: 256 sequences of 512 to 6144
+// positions (28 q / 4 KV heads x 128, fp16) 269 to 279 us, 2 of 100001 to 130000 (40 / 8, bf16) 145 to
+// 149 us, 0.97 of the copy bandwidth measured on this GPU; the first in fp32 693 us (0.78).
 template <typename T, int D, int NT, bool PAGE16>
 __global__ void __launch_bounds__(Shape<T, D, NT>::kWarps * 32, Shape<T, D, NT>::kResident)
     paged_attention_share_kernel(PagedArgs a, PlanArgs plan) {
@@ -898,9 +914,10 @@ __global__ void __launch_bounds__(Shape<T, D, NT>::kWarps * 32, Shape<T, D, NT>:
 }
 
 // Few items: a cluster of CTAs each, an equal run of its tiles per CTA, joined through the
-// cluster's shared memory. One launch, no workspace. Where each of
-// its CTAs has an SM to itself, eight warps share the work (WIDE): one warp per scheduler leaves
-// most of the issue slots empty.
+// cluster's shared memory. One launch, no workspace. Where each of its CTAs has an SM to itself, eight
+// warps share the work (WIDE): one warp per scheduler leaves most of the issue slots empty. Bound by latency: 64 sequences of 256 to 2048 positions (16 / 2 heads,
+// bf16) 23.7 us: a block of 16 keys a warp costs 1.3 us of dependent loads and products (11 of them in
+// the longest sequence's CTAs), the rest is launch, length, page and joins; one of 200 positions 8.2 us.
 template <typename T, int D, int NT, bool PAGE16, bool WIDE>
 __global__ void __launch_bounds__(Shape<T, D, NT, WIDE>::kWarps * 32, Shape<T, D, NT, WIDE>::kResident)
     paged_attention_cluster_kernel(PagedArgs a, PlanArgs plan) {
@@ -1040,7 +1057,8 @@ template <typename T> void shape_of(int64_t dim, int nt, int& resident, int& til
 }
 
 // Query heads of an item: the tensor instruction takes 8, two of them share the key and value
-// registers where those leave room (head dims to 128).
+// registers where those leave room (head dims to 128): 256 x 512..6144 with 32 q / 2 KV heads x 128
+// 177 us, 268 with every key read twice.
 int head_tiles(int64_t dim, int64_t group) { return group > 8 && dim <= 128 ? 2 : 1; }
 
 bool tensor_shape(int64_t dim) { return dim == 64 || dim == 128 || dim == 256; }
@@ -1107,7 +1125,9 @@ int launch_shares(const PagedArgs& a, const PlanArgs& plan, int ctas, cudaStream
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   const int entries = plan.by_item ? (int)(a.batch * a.kv_heads * plan.chunks) : ctas;
-  const bool many = ctas > 16 * entries;  // parts of an item: 16 warps join them faster than 4
+  // Few items of many parts: 16 warps join them faster (1 x 130000, 2 items, 32.5 us, 38.0 with 4),
+  // else 4 do (64 x 512..6144, 256 items, 78 us, 83 with 16).
+  const bool many = ctas > 16 * entries;
   cfg.gridDim = dim3(entries, (unsigned)min((int)(a.q_heads / a.kv_heads), 8 * NT));
   cfg.blockDim = dim3(many ? 512 : 128);
   cfg.stream = s;

@@ -263,6 +263,32 @@ def test_attention_peaked_flat_and_negative_scales(dtype, scale):
     check_attention(out, q, kp, vp, table, lengths, scale, 16, dtype)
 
 
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('n', [5000, 60000])
+@pytest.mark.parametrize('dim', [64, 128])
+def test_attention_sums_many_small_weights(dtype, n, dim):
+    """One key takes nearly all the weight and n - 1 have e^-18 of it each (2^-26, below fp16's smallest
+    step): only they have values. Scores are exact but for the factor scale log2(e), off by 2^-23 of
+    |s| = 26; the weights are summed in fp32 (n 2^-23 of the sum at most) and fp16 drops 2^-36 of the
+    largest weight of each."""
+    k = torch.zeros(n, dim, dtype=dtype, device='cuda')
+    k[1:, 0] = -18.0
+    v = torch.ones(n, dim, dtype=dtype, device='cuda')
+    v[0] = 0
+    pages = -(-n // 16)
+    kp, vp = torch.zeros(2, pages, 1, 16, dim, dtype=dtype, device='cuda')
+    kp.view(-1, dim)[:n], vp.view(-1, dim)[:n] = k, v
+    q = torch.zeros(1, 5, 1, dim, dtype=dtype, device='cuda')
+    q[..., 0] = 1
+    table = torch.arange(pages, device='cuda')[None]
+    out = paged_attention(q, kp, vp, table, torch.tensor([n], device='cuda'), 1.0).double()
+    mass = (n - 1) * math.exp(-18)
+    ref = mass / (1 + mass)
+    u = torch.finfo(dtype).eps / 2
+    assert ((out - ref).abs() <= ref * (u + 2.0 ** -16 + 26 * 2.0 ** -22 + n * 2.0 ** -23) + n * 2.0 ** -36).all(), (
+        out[0, 0, 0, 0].item(), ref)
+
+
 def test_attention_rising_scores_and_lowest_values():
     """Every key beats the ones before it (the running maximum moves each step); keys whose score is
     hugely negative; a key that holds -inf products (weight 0); one with NaN (its row is NaN)."""

@@ -33,7 +33,7 @@ def paged_append(key, value, key_pages, value_pages, page_table, starts, *, coun
     position). Queries of padding rows come back as zeros. ``query_out`` may be ``query`` itself.
     A page outside the pools, a position the table or the rotation does not hold: that token is
     treated as padding and reported by ``_ops.device_error``. No two live tokens of a call may
-    name the same slot.
+    name the same slot. Inference only: no gradient flows through it.
     """
     return _ops.paged_append(key, value, key_pages, value_pages, page_table, starts, counts, query, rotation,
                              positions, interleaved, query_out)
@@ -44,7 +44,8 @@ def paged_attention(query, key_pages, value_pages, page_table, lengths, scale=No
 
     ``query`` (batch, q_heads, 1, head_dim); pools and ``page_table`` as for ``paged_append``;
     ``lengths`` (batch,) int64. Query head h reads KV head h // (q_heads // kv_heads). A sequence
-    of length 0 gives zeros, an infinite value NaN. fp32 products are taken to 2^-22. Returns (batch, 1, q_heads, head_dim). Head dims to 256.
+    of length 0 gives zeros, an infinite value NaN. fp32 products are taken to 2^-22. Returns
+    (batch, 1, q_heads, head_dim). Head dims to 256. Inference only: no gradient flows through it.
     """
     return _ops.paged_attention(query, key_pages, value_pages, page_table, lengths,
                                 query.shape[-1] ** -0.5 if scale is None else scale, out)
@@ -215,7 +216,7 @@ class PagedKVCache(Cache):
                 raise ValueError('KV batch differs from live request count')
             if rows > 1 and any(self.lengths):
                 raise ValueError('after its prompt a paged cache takes one token per sequence at a time')
-            counts = self._prompts if rows > 1 and self._prompts is not None else [rows] * batch
+            counts = self._prompts if self._prompts is not None else [rows] * batch
             if len(counts) != batch or any(not 0 <= c <= rows for c in counts):
                 raise ValueError('prompt lengths do not match the prompt rows')
             self.begin(counts, device=key_states.device)

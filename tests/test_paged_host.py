@@ -209,3 +209,28 @@ def test_paged_update_refuses_multi_token_steps(monkeypatch):
     assert cache.lengths == [4, 2]
     with pytest.raises(ValueError, match='live request count'):
         cache.update(k[:1, :, :1], k[:1, :, :1], 0)
+
+
+def test_prompt_lengths_of_one_row(monkeypatch):
+    """Prompts whose batch is one row wide have lengths too: an empty one stays empty."""
+    calls = []
+    monkeypatch.setattr(_ops, 'paged_append', lambda *a: calls.append(a))
+    cache = PagedKVCache(8, 4, batch_capacity=2, max_length=16)
+    k = torch.zeros(2, 1, 1, 8)
+    cache.prompt_lengths([1, 0])
+    keys, _ = cache.update(k, k, 0)
+    assert cache.lengths == [1, 0] and keys._speckv_pages[1].tolist() == [1, 0] and calls[0][6].tolist() == [1, 0]
+    cache.update(k, k, 0)
+    assert cache.lengths == [2, 1]
+    cache.prompt_lengths([1])
+    with pytest.raises(ValueError, match='prompt lengths'):
+        cache.update(k, k, 0)
+
+
+def test_negative_strides_are_refused(lib):
+    with pytest.raises(_lib.SpecKVError, match='negative stride'):
+        _lib.call('speckv_paged_append', P, P, None, None, P, P, _lib.i64_array([0] * 17 + [-16]), P, 2, 2, 4, 16, P, None,
+                  None, 0, 0, None, None, 0, 0, 0, 1, 0, 2, 1, 128, _lib.BF16, None)
+    with pytest.raises(_lib.SpecKVError, match='negative stride'):
+        _lib.call('speckv_paged_attention', P, P, P, _lib.i64_array([0, 0, -1, 0, 0, 0, 0, 0]), P, 2, 2, 4, 16, P, P, 1, 2, 2,
+                  128, 1.0, _lib.BF16, None, 0, None)

@@ -104,4 +104,3 @@ def build_front(force=False, verbose=False):
 
 if __name__ == '__main__':
     print(build(force='--force' in sys.argv, verbose='-v' in sys.argv))
-

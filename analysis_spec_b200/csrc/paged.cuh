@@ -51,4 +51,10 @@ inline int check_pages(const char* fn, const int64_t* table, int64_t table_strid
   return SPECKV_OK;
 }
 
+inline int check_strides(const char* fn, const int64_t* strides, int n) {
+  for (int i = 0; i < n; ++i)
+    if (strides[i] < 0) return fail(SPECKV_EINVAL, "%s: negative stride %lld", fn, (long long)strides[i]);
+  return SPECKV_OK;
+}
+
 }  // namespace speckv

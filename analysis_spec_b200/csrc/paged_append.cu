@@ -350,6 +350,8 @@ extern "C" int speckv_paged_append(const void* key, const void* value, const voi
     return fail(SPECKV_ENOSUPPORT, "%s: 2^31 tokens or more", fn);
   if (!key || !value || !key_pages || !value_pages || !strides || !starts)
     return fail(SPECKV_EINVAL, "%s: null pointer", fn);
+  st = check_strides(fn, strides, 18);
+  if (st) return st;
   st = check_current_device(fn, {key, key_pages, page_table, query_out});
   if (st) return st;
   AppendArgs a;

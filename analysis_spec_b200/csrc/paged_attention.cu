@@ -1236,6 +1236,8 @@ extern "C" int speckv_paged_attention(const void* query, const void* key_pages, 
     return fail(SPECKV_ENOSUPPORT, "%s: more than 2^20 sequences or 1024 query heads", fn);
   if (!query || !key_pages || !value_pages || !strides || !lengths || !out)
     return fail(SPECKV_EINVAL, "%s: null pointer", fn);
+  st = check_strides(fn, strides, 8);
+  if (st) return st;
   st = check_current_device(fn, {query, key_pages, page_table, out});
   if (st) return st;
   PagedArgs a;

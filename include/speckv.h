@@ -565,7 +565,7 @@ int speckv_attention_test_hooks(int64_t wait_limit_ns, int32_t withhold_q_arriva
  * counts[b] are padding: nothing is read or stored for them and their query_out rows are zeros;
  * so are those of tokens refused with SPECKV_DERR_PAGE_TABLE or (position outside the tables)
  * SPECKV_DERR_ROTATION_INDEX. Two live tokens must not name one slot, and query_out must not
- * overlap key / value / query.
+ * overlap key or value, nor query unless it is query itself, strides included.
  * strides: 18 element strides, (b, h, t) of key, value, query and query_out, then (page, head,
  * position) of key_pages and value_pages. Replaces, for a paged cache, apply_rotary_pos_emb
  * followed by Cache.update (transformers models/qwen2/modeling_qwen2.py:215-225). */
@@ -580,14 +580,13 @@ int speckv_paged_append(const void* key, const void* value, const void* query, v
 /* Attention of one new token per sequence over a paged cache:
  *   out[b][0][hq][:] = softmax_c(q[b][hq] . k_c * scale) v_c,   c < lengths[b]
  * with KV head hq / (q_heads / kv_heads). lengths is a device array of batch int64; a sequence of
- * length 0 (or less) gives zeros; an infinite value makes its output NaN. out is contiguous (batch, 1, q_heads, dim). strides: 8 element
- * strides, (b, h) of query and (page, head, position) of key_pages and value_pages. Head dims to
- * 256: 64, 128 and 256 with 16-byte aligned rows take the tensor-core kernels (fp32 in three tf32
- * products, to 2^-22), which
- * cuts the live positions of all sequences into equal shares and joins what is cut, other views a
- * CUDA-core kernel. workspace (16-byte aligned, workspace_bytes at least
- * speckv_paged_attention_workspace of the same sizes on the same device; it holds nothing between
- * calls) may be shared by calls that cannot run at the same time. */
+ * length 0 (or less) gives zeros; an infinite value makes its output NaN. out is contiguous
+ * (batch, 1, q_heads, dim). strides: 8 element strides, (b, h) of query and (page, head, position)
+ * of key_pages and value_pages. Head dims to 256: 64, 128 and 256 with 16-byte aligned rows take
+ * the tensor-core kernels (fp32 in three tf32 products, to 2^-22), other views a CUDA-core kernel.
+ * workspace (16-byte aligned, workspace_bytes at least speckv_paged_attention_workspace of the
+ * same sizes on the same device; it holds nothing between calls) may be shared by calls that
+ * cannot run at the same time. */
 int speckv_paged_attention(const void* query, const void* key_pages, const void* value_pages, const int64_t* strides,
                            const int64_t* page_table, int64_t table_stride, int64_t table_pages, int64_t num_pages,
                            int64_t page_size, const int64_t* lengths, void* out, int64_t batch, int64_t q_heads,

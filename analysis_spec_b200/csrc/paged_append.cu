@@ -190,14 +190,15 @@ __device__ __forceinline__ void rotate(uint4& px, uint4& py, const float (&c)[N]
 // pair of 16-byte pieces in kHeads heads at a time, all loaded before the first is stored; then the
 // pieces that are copied. Needs 16-byte aligned rows and rotation_dim / 2 a multiple of 16 bytes.
 // A token's work is two dependent rounds of loads (where it goes; its page, angles and rows), so
-// the CTA is small and its registers are held to 64: 16 tokens of an SM are in such rounds at once.
+// the CTA is small and its registers are held to 64: 16 tokens of an SM (32 where a warp does for a
+// token) are in such rounds at once.
 // Memory bound where tokens are many: 8 prompts to 4001 tokens, 40 q / 8 KV heads x 128 in fp16,
 // 115 us (0.95 of the copy bandwidth measured on this GPU); latency bound below: 64 x 61 rows of 16 / 2
-// heads 12 us (0.54), one row each of 256 sequences 6.5 us, the cost of the host call.
+// heads 10.3 us (0.63), one row each of 256 sequences 6.6 us, the cost of the host call.
 constexpr int kHeads = 3;
 
-template <typename T, bool INTERLEAVED>
-__global__ void __launch_bounds__(kAppendThreads, 16) paged_append_kernel(AppendArgs a) {
+template <typename T, bool INTERLEAVED, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) paged_append_kernel(AppendArgs a) {
   constexpr int N = Piece<T>::N;
   const uint32_t b = blockIdx.x / (uint32_t)a.rows, t = blockIdx.x - b * (uint32_t)a.rows;
   const int q_heads = a.query != nullptr ? (int)a.q_heads : 0, kv_heads = (int)a.kv_heads, dim = (int)a.dim;
@@ -217,11 +218,11 @@ __global__ void __launch_bounds__(kAppendThreads, 16) paged_append_kernel(Append
   const uint32_t size = (uint32_t)a.table.page_size, index = stored ? (uint32_t)slot / size : 0u;
   const long long page = stored ? a.table.entries[b * a.table.stride + index] : 0;  // checked below
 
-  const int half = a.rot / 2, slices = half / N;  // slices <= 64
+  const int half = a.rot / 2, slices = half / N;  // slices <= THREADS
   const T* k = static_cast<const T*>(a.key) + b * a.ks[0] + t * a.ks[2];
   const T* v = static_cast<const T*>(a.value) + b * a.vs[0] + t * a.vs[2];
   const int slice = slices > 0 ? threadIdx.x % slices : 0, h0 = slices > 0 ? threadIdx.x / slices : 0;
-  const int step = slices > 0 ? kAppendThreads / slices : 1, heads = slices > 0 && h0 < step ? q_heads + kv_heads : 0;
+  const int step = slices > 0 ? THREADS / slices : 1, heads = slices > 0 && h0 < step ? q_heads + kv_heads : 0;
   const int x = INTERLEAVED ? 2 * slice * N : slice * N, y = INTERLEAVED ? x + N : x + half;
   uint4 px[kHeads], py[kHeads];
   auto load = [&](int h) {
@@ -253,7 +254,7 @@ __global__ void __launch_bounds__(kAppendThreads, 16) paged_append_kernel(Append
   }
   if (!stored) {  // padding: its queries are zeros
     const int pieces = dim / N;
-    for (int i = threadIdx.x; i < q_heads * pieces; i += kAppendThreads)
+    for (int i = threadIdx.x; i < q_heads * pieces; i += THREADS)
       *reinterpret_cast<uint4*>(qo + (i / pieces) * a.os[1] + (i % pieces) * N) = make_uint4(0, 0, 0, 0);
     return;
   }
@@ -276,7 +277,7 @@ __global__ void __launch_bounds__(kAppendThreads, 16) paged_append_kernel(Append
   // V, then what lies past the rotation in K and Q
   const int whole = dim / N, rest = (dim - a.rot) / N;
   const int v_items = kv_heads * whole, items = v_items + (rest > 0 ? (q_heads + kv_heads) * rest : 0);
-  for (int i = threadIdx.x; i < items; i += kAppendThreads) {
+  for (int i = threadIdx.x; i < items; i += THREADS) {
     const T* from;
     T* to;
     if (i < v_items) {
@@ -305,15 +306,28 @@ template <typename T> bool in_pieces(const AppendArgs& a) {
   return ok;
 }
 
+template <typename T, int THREADS> void launch_pieces(const AppendArgs& a, unsigned tokens, cudaStream_t s) {
+  if (a.interleaved)
+    paged_append_kernel<T, true, THREADS><<<tokens, THREADS, 0, s>>>(a);
+  else
+    paged_append_kernel<T, false, THREADS><<<tokens, THREADS, 0, s>>>(a);
+}
+
 template <typename T>
 int launch_append(const AppendArgs& a, cudaStream_t s) {
   const unsigned tokens = (unsigned)(a.batch * a.rows);
+  const int sms = sm_count();
+  if (sms == 0) return fail(SPECKV_ECUDA, "speckv_paged_append: no SM count");
+  // More tokens than CTAs of 64 run at once, and at most five pairs of pieces a lane: a warp does for a
+  // token, twice as many are under way (16 q / 2 KV heads x 128 bf16, 64 x 61 rows 12.0 -> 10.3 us, 8 x 4001
+  // 63.4 -> 57.5). With 28 / 4 heads, eight pairs a lane, it does not (64 x 61 rows 16.6 us, 17.4).
+  const int64_t slices = a.rot / 2 * (int64_t)sizeof(T) / 16, heads = a.kv_heads + (a.query != nullptr ? a.q_heads : 0);
   if (!in_pieces<T>(a))
     paged_append_scalar_kernel<T><<<tokens, kAppendThreads, 0, s>>>(a);
-  else if (a.interleaved)
-    paged_append_kernel<T, true><<<tokens, kAppendThreads, 0, s>>>(a);
+  else if (tokens > 16u * (unsigned)sms && slices > 0 && slices <= 32 && slices * heads <= 5 * 32)
+    launch_pieces<T, 32>(a, tokens, s);
   else
-    paged_append_kernel<T, false><<<tokens, kAppendThreads, 0, s>>>(a);
+    launch_pieces<T, kAppendThreads>(a, tokens, s);
   return check_launch("speckv_paged_append");
 }
 

@@ -110,6 +110,41 @@ def test_append_and_rotation(batch, rows, hq, hkv, dim, rot, page, past, dtype):
     run_append(batch, rows, hq, hkv, dim, rot, page, past, dtype, interleaved=True, ragged=rows > 1, placed=True, seed=1)
 
 
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('batch,rows,hq,hkv,dim,rot,page,past', [
+    (40, 61, 16, 2, 128, 128, 16, 100), (3, 901, 4, 1, 64, 32, 8, 7), (2, 1300, 1, 1, 256, 256, 64, 0),
+    (7, 400, 7, 3, 128, 96, 16, 20), (43, 61, 28, 4, 128, 128, 16, 9)])
+def test_append_of_many_tokens(batch, rows, hq, hkv, dim, rot, page, past, dtype):
+    """More tokens than the CTAs of 64 threads that run at once: a warp per token where heads are few."""
+    run_append(batch, rows, hq, hkv, dim, rot, page, past, dtype, interleaved=False, ragged=True, placed=False)
+    run_append(batch, rows, hq, hkv, dim, rot, page, past, dtype, interleaved=True, ragged=False, placed=True, seed=1,
+               query=batch != 3)
+
+
+def test_append_of_many_tokens_reports_bad_pages():
+    """Sequence 1's second page is none of the pools', sequence 2 starts past the table: their tokens
+    there are padding, every other one is stored."""
+    g = gen(11)
+    k, v = (randn(3, 2, 900, 128, dtype=torch.bfloat16, g=g) for _ in range(2))
+    q = randn(3, 8, 900, 128, dtype=torch.bfloat16, g=g)
+    kp, vp = pools(30, 2, 100, 128, torch.bfloat16, g)
+    table = torch.arange(27, device='cuda').view(3, 9).contiguous()
+    table[1, 1] = 30
+    starts = torch.tensor([0, 0, 500], device='cuda')
+    out = paged_append(k, v, kp, vp, table, starts, query=q, rotation=rotation_tables(900, 128))
+    kind, where = _ops.device_error()
+    assert kind == 'page table' and (where == 30 or 900 <= where < 1400)
+    live = torch.ones(3, 900, dtype=torch.bool, device='cuda')
+    live[1, 100:200] = False
+    live[2, 400:] = False
+    assert out.transpose(1, 2)[live].any(-1).all() and not out.transpose(1, 2)[~live].any()
+    want = torch.full_like(vp, math.nan)
+    for b in range(3):
+        slot = int(starts[b]) + torch.arange(900, device='cuda')[live[b]]
+        want[table[b][slot // 100], :, slot % 100] = v[b].transpose(0, 1)[live[b]]
+    assert torch.equal(vp.nan_to_num(9.0), want.nan_to_num(9.0)) and torch.equal(kp.isnan(), want.isnan())
+
+
 def test_append_without_rotation_or_query():
     run_append(3, 20, 4, 2, 128, 0, 16, 30, torch.bfloat16, False, True, False, query=False)
     run_append(3, 20, 4, 2, 128, 0, 16, 30, torch.bfloat16, False, False, False)

@@ -323,7 +323,7 @@ __device__ __forceinline__ void join_warps(unsigned char* shared, Parts<W, NT>& 
 // 16-bit caches. Operands come straight from memory into registers: the dims of a product may be
 // taken in any order, so a lane's 16-byte chunks of its key rows are its fragments as they are, and
 // two keys' chunks of V give theirs by byte permutes. 8 KB a warp are under way, 12 warps on an SM.
-// (Copied ahead through shared memory instead, 8 warps, the same work took 6 to 16 % longer.)
+// (Copied ahead through shared memory instead, 8 warps, 256 x 512..6144 took 293 us, 275 so.)
 // One CTA's part of an item: tiles [t0, ...) of its keys up to position `end`.
 template <typename T, int D, int NT, bool PAGE16, bool WIDE, typename Emit>
 __device__ __forceinline__ void attend_part16(const PagedArgs& a, unsigned char* shared,

@@ -36,7 +36,7 @@ __device__ __forceinline__ long long live_length(const PagedArgs& a, long long b
 constexpr int kScalarWarps = 8;
 constexpr int kScalarDims = 8;  // dims per lane: head dims to 256
 
-// CTA per (sequence, query head), a key per warp and step: any head dim to 256, stride, alignment. Reads
+// CTA per (sequence, query head), a key per warp and step: head dims and views off 16-byte boundaries. Reads
 // the cache once per query head and waits for each key: 30 times the time of the kernels below.
 template <typename T>
 __global__ void __launch_bounds__(kScalarWarps * 32) paged_attention_scalar_kernel(PagedArgs a) {
@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(kScalarWarps * 32) paged_attention_scalar_kern
   }
 }
 
-// ---- tensor-core kernels: head dims 64 / 128 / 256 ------------------------------------------------
+// ---- tensor-core kernels: head dims to 64 / 128 / 256 ----------------------------------------------
 //
 // Scores are K q^T (16 keys x 8 heads per matrix instruction), outputs V^T p^T (16 dims x 8
 // heads): the group's heads are the narrow side, so keys are never padded to 128 rows, as the
@@ -324,8 +324,11 @@ __device__ __forceinline__ void join_warps(unsigned char* shared, Parts<W, NT>& 
 // taken in any order, so a lane's 16-byte chunks of its key rows are its fragments as they are, and
 // two keys' chunks of V give theirs by byte permutes. 8 KB a warp are under way, 12 warps on an SM.
 // (Copied ahead through shared memory instead, 8 warps, 256 x 512..6144 took 293 us, 275 so.)
+// WHOLE: pages hold a multiple of 16 positions, so that a block lies in one, and the head dim is D. Else
+// each row is looked up by itself and cut to its dims (256 x 512..6144, 28 / 4 heads, fp16: pages of 24
+// positions 358 us, dim 96 349 us, 273 us where WHOLE holds).
 // One CTA's part of an item: tiles [t0, ...) of its keys up to position `end`.
-template <typename T, int D, int NT, bool PAGE16, bool WIDE, typename Emit>
+template <typename T, int D, int NT, bool WHOLE, bool WIDE, typename Emit>
 __device__ __forceinline__ void attend_part16(const PagedArgs& a, unsigned char* shared,
                                               Parts<Shape<T, D, NT, WIDE>::kWarps, NT>& sm, long long b, int hk, int h0,
                                               int heads, int t0, long long end, Emit emit) {
@@ -338,6 +341,7 @@ __device__ __forceinline__ void attend_part16(const PagedArgs& a, unsigned char*
   const T* kbase = static_cast<const T*>(a.k) + hk * a.ks[1];
   const T* vbase = static_cast<const T*>(a.v) + hk * a.vs[1];
   const uint32_t P = (uint32_t)a.table.page_size;
+  const int dim = WHOLE ? D : (int)a.dim;  // dims from there to D are zeros, not read
 
   uint4 kreg[2][KC], vreg[4][VC];
   // block i of this warp: keys [16 (W t0 + warp + W i), + 16)
@@ -347,12 +351,12 @@ __device__ __forceinline__ void attend_part16(const PagedArgs& a, unsigned char*
   const T* klane = kbase + g * a.ks[2] + t * 8;
   const T* vlane = vbase + 2 * t * a.vs[2] + g * 8;
 
-  // PAGE16: a block lies in one page. Each lane finds the place of one block in 32.
+  // A block lies in one page (WHOLE). Each lane finds the place of one block in 32.
   long long k_places = -1, v_places = -1, k_at = -1, v_at = -1;  // element offsets; -1: no such block or page
   int live = 0;  // keys of the block being loaded
   uint32_t seen = 0;  // bit 0 / 1: key rows g and g + 8 of the block in kreg are live
   auto place = [&](int i) {
-    if (PAGE16) {
+    if (WHOLE) {
       if ((i & 31) == 0) {
         const long long key = key0 + (long long)(i + lane) * S::kTile;
         k_places = v_places = -1;
@@ -377,7 +381,7 @@ __device__ __forceinline__ void attend_part16(const PagedArgs& a, unsigned char*
     return p < 0 ? nullptr : from + p * st[0] + (long long)((uint32_t)key - index * P) * st[2];
   };
   auto load_k = [&](int i) {
-    if (PAGE16 && live == 16) {
+    if (WHOLE && live == 16) {
       const T* p = klane + k_at;
 #pragma unroll
       for (int j = 0; j < KC; ++j) {
@@ -391,17 +395,18 @@ __device__ __forceinline__ void attend_part16(const PagedArgs& a, unsigned char*
     const T* p[2];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      if (PAGE16)
+      if (WHOLE)
         p[x] = g + 8 * x < live ? klane + k_at + 8 * x * a.ks[2] : nullptr;
       else
         p[x] = row_ptr(kbase + t * 8, a.ks, key + g + 8 * x);
 #pragma unroll
-      for (int j = 0; j < KC; ++j) kreg[x][j] = p[x] != nullptr ? load_stream(p[x] + 32 * j) : make_uint4(0, 0, 0, 0);
+      for (int j = 0; j < KC; ++j)
+        kreg[x][j] = p[x] != nullptr && (WHOLE || t * 8 + 32 * j < dim) ? load_stream(p[x] + 32 * j) : make_uint4(0, 0, 0, 0);
     }
     seen = (p[0] != nullptr ? 1u : 0u) | (p[1] != nullptr ? 2u : 0u);
   };
   auto load_v = [&](int i) {
-    if (PAGE16 && live == 16) {
+    if (WHOLE && live == 16) {
       const T* p = vlane + v_at;
 #pragma unroll
       for (int x = 0; x < 4; ++x)
@@ -414,13 +419,14 @@ __device__ __forceinline__ void attend_part16(const PagedArgs& a, unsigned char*
     for (int x = 0; x < 4; ++x) {
       const int k = 2 * t + (x & 1) + (x >> 1) * 8;
       const T* p;
-      if (PAGE16)
+      if (WHOLE)
         p = k < live ? vlane + v_at + ((x & 1) + (x >> 1) * 8) * a.vs[2] : nullptr;
       else
         p = row_ptr(vbase + g * 8, a.vs, key + k);
       // rows that are not there may hold anything: 0 x NaN is NaN
 #pragma unroll
-      for (int c = 0; c < VC; ++c) vreg[x][c] = p != nullptr ? load_stream(p + 64 * c) : make_uint4(0, 0, 0, 0);
+      for (int c = 0; c < VC; ++c)
+        vreg[x][c] = p != nullptr && (WHOLE || g * 8 + 64 * c < dim) ? load_stream(p + 64 * c) : make_uint4(0, 0, 0, 0);
     }
   };
 
@@ -436,7 +442,7 @@ __device__ __forceinline__ void attend_part16(const PagedArgs& a, unsigned char*
 #pragma unroll
     for (int j = 0; j < KC; ++j) {
       q[u][j] = make_uint4(0, 0, 0, 0);
-      if (u * 8 + g < heads) {
+      if (u * 8 + g < heads && (WHOLE || (t + 4 * j) * 8 < dim)) {
         const T* p = static_cast<const T*>(a.q) + b * a.qs[0] + (hk * group + h0 + u * 8 + g) * a.qs[1] +
                      (t + 4 * j) * 8;
         q[u][j] = *reinterpret_cast<const uint4*>(p);
@@ -549,7 +555,7 @@ __device__ __forceinline__ void attend_part16(const PagedArgs& a, unsigned char*
 // fp32 caches. Twice the bytes a key and six instructions a product: K and V rows are copied ahead
 // through a ring of shared memory per warp (blocks of K and of V in turn, 16 bytes a lane and copy),
 // which leaves the registers to the products. Products are three of tf32 parts.
-template <int D, int NT, bool PAGE16, typename Emit>
+template <int D, int NT, bool WHOLE, typename Emit>
 __device__ __forceinline__ void attend_part32(const PagedArgs& a, unsigned char* shared,
                                               Parts<Shape<float, D, NT>::kWarps, NT>& sm, long long b, int hk, int h0,
                                               int heads, int t0, long long end, Emit emit) {
@@ -563,6 +569,7 @@ __device__ __forceinline__ void attend_part32(const PagedArgs& a, unsigned char*
   const float* kbase = static_cast<const float*>(a.k) + hk * a.ks[1];
   const float* vbase = static_cast<const float*>(a.v) + hk * a.vs[1];
   const uint32_t P = (uint32_t)a.table.page_size;
+  const int dim = WHOLE ? D : (int)a.dim;  // dims from there to D are zeros, not read
   const uint32_t mine = (uint32_t)__cvta_generic_to_shared(shared) + warp * S::kStages * BLOCK;
   // Chunk c of row r lies at c ^ swizzle(r): the 8 rows of a matrix, and the 4 rows that a
   // transposed operand takes, are in different banks.
@@ -572,7 +579,7 @@ __device__ __forceinline__ void attend_part32(const PagedArgs& a, unsigned char*
   const long long key0 = (long long)t0 * S::kTile + warp * 16;
   const int count = key0 < end ? (int)((end - key0 + S::kTile - 1) / S::kTile) : 0;
 
-  // Each lane finds the place of one block in 32 (PAGE16: a block lies in one page) or of one row
+  // Each lane finds the place of one block in 32 (a block lies in one page where WHOLE) or of one row
   // of a block, as element offsets; -1: no such block or row, or no page of the pools.
   long long k_places = -1, v_places = -1;
   bool missing = false;  // a page of this item is not one of the pools'
@@ -597,7 +604,7 @@ __device__ __forceinline__ void attend_part32(const PagedArgs& a, unsigned char*
     const uint32_t to = mine + stage * BLOCK;
     const long long key = key0 + (long long)i * S::kTile;
     if (!values) {
-      if (PAGE16) {
+      if (WHOLE) {
         if ((i & 31) == 0) find(key + (long long)lane * S::kTile);
       } else {
         find(lane < 16 ? key + lane : end);
@@ -610,11 +617,13 @@ __device__ __forceinline__ void attend_part32(const PagedArgs& a, unsigned char*
     const int r0 = lane / CHUNKS, chunk = lane % CHUNKS;
 #pragma unroll
     for (int r = 0; r < 16; r += ROWS) {
-      const long long row = PAGE16 ? block + (r + r0) * stride : __shfl_sync(0xffffffffu, place, r + r0);
-      const bool live = PAGE16 ? r + r0 < rows : row >= 0;
+      const long long row = WHOLE ? block + (r + r0) * stride : __shfl_sync(0xffffffffu, place, r + r0);
+      const bool live = WHOLE ? r + r0 < rows : row >= 0;
 #pragma unroll
-      for (int c = chunk; c < CHUNKS; c += 32)
-        copy_row(to + (r + r0) * S::kRow + ((c ^ swizzle(r + r0)) << 4), live ? base + row + c * E : base, live);
+      for (int c = chunk; c < CHUNKS; c += 32) {
+        const bool there = live && (WHOLE || c * E < dim);
+        copy_row(to + (r + r0) * S::kRow + ((c ^ swizzle(r + r0)) << 4), there ? base + row + c * E : base, there);
+      }
     }
   };
   // bits 0 and 1: whether keys g and g + 8 of block i count
@@ -647,7 +656,7 @@ __device__ __forceinline__ void attend_part32(const PagedArgs& a, unsigned char*
     for (int i = 0; i < STEPS; ++i)
 #pragma unroll
       for (int x = 0; x < 2; ++x)
-        q[u][i][x] = there ? *reinterpret_cast<const uint32_t*>(p + (2 * i + x) * E) : 0u;
+        q[u][i][x] = there && (WHOLE || (2 * i + x) * E < dim) ? *reinterpret_cast<const uint32_t*>(p + (2 * i + x) * E) : 0u;
   }
   float o[NT][D / 16][4], m[NT][2], l[NT][2];
 #pragma unroll
@@ -708,7 +717,7 @@ __device__ __forceinline__ void attend_part32(const PagedArgs& a, unsigned char*
           s[u][e] = s2[u][e] = 0.f;
           if (head < heads) {
             const float* p = static_cast<const float*>(a.q) + b * a.qs[0] + (hk * group + h0 + head) * a.qs[1];
-            for (int d = 0; d < D; ++d)
+            for (int d = 0; d < dim; ++d)
               s[u][e] = fmaf(p[d], __uint_as_float(load_word(k_at + row * S::kRow + (((d >> 2) ^ swizzle(row)) << 4) + (d & 3) * 4)),
                              s[u][e]);
           }
@@ -789,14 +798,14 @@ __device__ __forceinline__ void attend_part32(const PagedArgs& a, unsigned char*
   }, emit);
 }
 
-template <typename T, int D, int NT, bool PAGE16, bool WIDE, typename Emit>
+template <typename T, int D, int NT, bool WHOLE, bool WIDE, typename Emit>
 __device__ __forceinline__ void attend_part(const PagedArgs& a, unsigned char* shared,
                                             Parts<Shape<T, D, NT, WIDE>::kWarps, NT>& sm, long long b, int hk, int h0, int heads,
                                             int t0, long long end, Emit emit) {
   if constexpr (sizeof(T) == 2)
-    attend_part16<T, D, NT, PAGE16, WIDE>(a, shared, sm, b, hk, h0, heads, t0, end, emit);
+    attend_part16<T, D, NT, WHOLE, WIDE>(a, shared, sm, b, hk, h0, heads, t0, end, emit);
   else
-    attend_part32<D, NT, PAGE16>(a, shared, sm, b, hk, h0, heads, t0, end, emit);
+    attend_part32<D, NT, WHOLE>(a, shared, sm, b, hk, h0, heads, t0, end, emit);
 }
 
 __device__ __forceinline__ long long tiles_of(const PagedArgs& a, long long b, int tile) {
@@ -807,7 +816,7 @@ __device__ __forceinline__ long long tiles_of(const PagedArgs& a, long long b, i
 // long cache is split as finely as the GPU is wide. Bound by memory: 256 sequences of 512 to 6144
 // positions (28 q / 4 KV heads x 128, fp16) 269 to 279 us, 2 of 100001 to 130000 (40 / 8, bf16) 145 to
 // 149 us, 0.97 of the copy bandwidth measured on this GPU; the first in fp32 693 us (0.78).
-template <typename T, int D, int NT, bool PAGE16>
+template <typename T, int D, int NT, bool WHOLE>
 __global__ void __launch_bounds__(Shape<T, D, NT>::kWarps * 32, Shape<T, D, NT>::kResident)
     paged_attention_share_kernel(PagedArgs a, PlanArgs plan) {
   constexpr int W = Shape<T, D, NT>::kWarps, kTile = Shape<T, D, NT>::kTile;
@@ -818,15 +827,15 @@ __global__ void __launch_bounds__(Shape<T, D, NT>::kWarps * 32, Shape<T, D, NT>:
   __shared__ long long s_scan[W], s_find[2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long group = a.q_heads / a.kv_heads, per_seq = a.kv_heads * plan.chunks;
-  const int G = gridDim.x, cta = blockIdx.x;
+  const int G = gridDim.x, cta = blockIdx.x, dim = WHOLE ? D : (int)a.dim;
 
   // sequences with nothing to see
   for (long long b = cta; b < a.batch; b += G)
     if (live_length(a, b) == 0) {
       if (plan.by_item)
         for (long long i = threadIdx.x; i < per_seq; i += W * 32) plan.joins[b * per_seq + i] = Join{0, 0, 0, 0};
-      for (long long i = threadIdx.x; i < a.q_heads * D; i += W * 32)
-        static_cast<T*>(a.out)[b * a.q_heads * D + i] = store_f<T>(0.f);
+      for (long long i = threadIdx.x; i < a.q_heads * dim; i += W * 32)
+        static_cast<T*>(a.out)[b * a.q_heads * dim + i] = store_f<T>(0.f);
     }
 
   // tiles before each thread's run of sequences, and in all
@@ -895,10 +904,10 @@ __global__ void __launch_bounds__(Shape<T, D, NT>::kWarps * 32, Shape<T, D, NT>:
       join = Join{(int)b, h, slot, (int)(last - cta) + 1};
     }
     if (t0 == 0 && plan.by_item && threadIdx.x == 0) plan.joins[b * per_seq + h] = t1 < nb ? join : Join{0, 0, 0, 0};
-    T* out = static_cast<T*>(a.out) + (b * a.q_heads + hk * group + h0) * D;
-    attend_part<T, D, NT, PAGE16, false>(a, shared, sm, b, hk, h0, heads, t0, end, [&](int head, int d, const float4& sum, float top, float all) {
+    T* out = static_cast<T*>(a.out) + (b * a.q_heads + hk * group + h0) * dim;
+    attend_part<T, D, NT, WHOLE, false>(a, shared, sm, b, hk, h0, heads, t0, end, [&](int head, int d, const float4& sum, float top, float all) {
       if (whole) {
-        store_four(out + head * D + d, sum, all);
+        if (WHOLE || d < dim) store_four(out + head * dim + d, sum, all);
       } else {
         *reinterpret_cast<float4*>(part + head * D + d) = sum;
         if (d == 0) {
@@ -918,7 +927,7 @@ __global__ void __launch_bounds__(Shape<T, D, NT>::kWarps * 32, Shape<T, D, NT>:
 // warps share the work (WIDE): one warp per scheduler leaves most of the issue slots empty. Bound by latency: 64 sequences of 256 to 2048 positions (16 / 2 heads,
 // bf16) 23.7 us: a block of 16 keys a warp costs 1.3 us of dependent loads and products (11 of them in
 // the longest sequence's CTAs), the rest is launch, length, page and joins; one of 200 positions 8.2 us.
-template <typename T, int D, int NT, bool PAGE16, bool WIDE>
+template <typename T, int D, int NT, bool WHOLE, bool WIDE>
 __global__ void __launch_bounds__(Shape<T, D, NT, WIDE>::kWarps * 32, Shape<T, D, NT, WIDE>::kResident)
     paged_attention_cluster_kernel(PagedArgs a, PlanArgs plan) {
   constexpr int W = Shape<T, D, NT, WIDE>::kWarps, kTile = Shape<T, D, NT, WIDE>::kTile;
@@ -934,7 +943,7 @@ __global__ void __launch_bounds__(Shape<T, D, NT, WIDE>::kWarps * 32, Shape<T, D
   const int hk = h / plan.chunks, h0 = (h - hk * plan.chunks) * 8 * NT, heads = min((int)group - h0, 8 * NT);
   const long long n = live_length(a, b), nb = (n + kTile - 1) / kTile;
   const int t0 = (int)(nb * rank / ctas), t1 = (int)(nb * (rank + 1) / ctas);
-  attend_part<T, D, NT, PAGE16, WIDE>(a, shared, sm, b, hk, h0, heads, t0, min(n, (long long)t1 * kTile),
+  attend_part<T, D, NT, WHOLE, WIDE>(a, shared, sm, b, hk, h0, heads, t0, min(n, (long long)t1 * kTile),
                                 [&](int head, int d, const float4& sum, float top, float all) {
                                   *reinterpret_cast<float4*>(&s_sum[head][d]) = sum;
                                   if (d == 0) {
@@ -944,7 +953,8 @@ __global__ void __launch_bounds__(Shape<T, D, NT, WIDE>::kWarps * 32, Shape<T, D
                                 });
   cluster_sync();
   // each CTA joins its share of the outputs
-  T* out = static_cast<T*>(a.out) + (b * a.q_heads + hk * group + h0) * D;
+  const int dim = WHOLE ? D : (int)a.dim;
+  T* out = static_cast<T*>(a.out) + (b * a.q_heads + hk * group + h0) * dim;
   for (int i = rank * W * 32 + threadIdx.x; i < heads * D / 4; i += ctas * W * 32) {
     const int head = 4 * i / D, d = 4 * i - head * D;
     float top[kCluster], all[kCluster], ref = -INFINITY;
@@ -970,7 +980,7 @@ __global__ void __launch_bounds__(Shape<T, D, NT, WIDE>::kWarps * 32, Shape<T, D
         o.x = fmaf(sum[r].x, f, o.x), o.y = fmaf(sum[r].y, f, o.y);
         o.z = fmaf(sum[r].z, f, o.z), o.w = fmaf(sum[r].w, f, o.w);
       }
-    store_four(out + 4 * i, o, total);
+    if (WHOLE || d < dim) store_four(out + head * dim + d, o, total);
   }
   cluster_sync();  // the other CTAs' shared memory is read until here
 }
@@ -1041,8 +1051,8 @@ __global__ void __launch_bounds__(WARPS * 32) paged_attention_join_kernel(PagedA
     f[w] = exp2f(s_top[w] - ref);
     total = fmaf(s_all[w], f[w], total);
   }
-  T* out = static_cast<T*>(a.out) + (j.b * a.q_heads + hk * group + h0 + head) * D;
-  for (int d = threadIdx.x; d < D; d += WARPS * 32) {
+  T* out = static_cast<T*>(a.out) + (j.b * a.q_heads + hk * group + h0 + head) * a.dim;
+  for (int d = threadIdx.x; d < a.dim; d += WARPS * 32) {
     float o = 0.f;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) o = fmaf(s_sum[w][d], f[w], o);
@@ -1061,7 +1071,12 @@ template <typename T> void shape_of(int64_t dim, int nt, int& resident, int& til
 // 177 us, 268 with every key read twice.
 int head_tiles(int64_t dim, int64_t group) { return group > 8 && dim <= 128 ? 2 : 1; }
 
-bool tensor_shape(int64_t dim) { return dim == 64 || dim == 128 || dim == 256; }
+// Head dim that the kernels are built for: rows of whole 16-byte pieces are read as the next one's, with
+// zeros behind them (64 x 256..2048, dim 96, bf16 32 us, 542 with the kernel for any dim); 0: none.
+template <typename T> int64_t built_dim(int64_t dim) {
+  if (dim > 256 || dim * sizeof(T) % 16 != 0) return 0;
+  return dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
+}
 
 // CTAs of a cluster per item, 0 for equal shares: clusters where they all run at once and the
 // longest sequence that the table can hold leaves each CTA few tiles.
@@ -1073,15 +1088,16 @@ int cluster_ctas(long long items, long long tiles, int full) {
 
 // How a tensor shape is launched, from sizes that the host knows.
 struct Launch {
-  int sms, tiles8, chunks, full, cluster;  // NT; items per (sequence, KV head); CTAs resident; CTAs per item or 0
+  int sms, tiles8, chunks, full, cluster;  // SMs; NT; items per (sequence, KV head); CTAs resident; CTAs per item or 0
   long long items, tiles;             // tiles of the longest sequence that the table can hold
-  int64_t workspace;
+  int64_t dim, workspace;             // dim: the kernels'
 };
 
 template <typename T>
-Launch plan_launch(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t positions, int sms) {
+Launch plan_launch(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t positions, int sms) {
   Launch l;
   l.sms = sms;
+  const int64_t dim = l.dim = built_dim<T>(head_dim);
   const int64_t group = q_heads / kv_heads;
   l.tiles8 = head_tiles(dim, group);
   int resident, tile;
@@ -1110,11 +1126,11 @@ int launch_failed(cudaError_t e) {
   return fail(SPECKV_ECUDA, "speckv_paged_attention: launch failed: %s", cudaGetErrorString(e));
 }
 
-template <typename T, int D, int NT, bool PAGE16>
+template <typename T, int D, int NT, bool WHOLE>
 int launch_shares(const PagedArgs& a, const PlanArgs& plan, int ctas, cudaStream_t s) {
   typedef Shape<T, D, NT> S;
   static bool done[64] = {false};
-  auto kernel = paged_attention_share_kernel<T, D, NT, PAGE16>;
+  auto kernel = paged_attention_share_kernel<T, D, NT, WHOLE>;
   cudaError_t e = allow_shared(kernel, S::kShared, done);
   if (e != cudaSuccess) return launch_failed(e);
   kernel<<<ctas, S::kWarps * 32, S::kShared, s>>>(a, plan);
@@ -1138,11 +1154,11 @@ int launch_shares(const PagedArgs& a, const PlanArgs& plan, int ctas, cudaStream
   return e == cudaSuccess ? SPECKV_OK : launch_failed(e);
 }
 
-template <typename T, int D, int NT, bool PAGE16, bool WIDE>
+template <typename T, int D, int NT, bool WHOLE, bool WIDE>
 int launch_clusters(const PagedArgs& a, const PlanArgs& plan, int items, int ctas, cudaStream_t s) {
   typedef Shape<T, D, NT, WIDE> S;
   static bool done[64] = {false};
-  auto kernel = paged_attention_cluster_kernel<T, D, NT, PAGE16, WIDE>;
+  auto kernel = paged_attention_cluster_kernel<T, D, NT, WHOLE, WIDE>;
   cudaError_t e = allow_shared(kernel, S::kShared, done);
   if (e != cudaSuccess) return launch_failed(e);
   cudaLaunchAttribute attr;
@@ -1167,28 +1183,28 @@ int launch_tensor(const PagedArgs& a, const Launch& l, void* workspace, cudaStre
   plan.by_item = 0;
   plan.joins = static_cast<Join*>(workspace);
   plan.parts = reinterpret_cast<float*>(plan.joins + l.full);
-  const bool page16 = a.table.page_size % 16 == 0;
+  const bool whole = a.table.page_size % 16 == 0 && a.dim == D;
   // Wide CTAs have an SM each, and clusters of eight do not fill all of them: at 96 CTAs or fewer they
   // all run at once (12.4 us instead of 15.3, 6 x 4000 keys of 16 / 2 heads), 128 took two turns (19.4, 15.8).
   constexpr bool can = sizeof(T) == 2;
   if (l.cluster > 0 && can && l.items * l.cluster * 3 <= l.sms * 2)
-    return page16 ? launch_clusters<T, D, NT, true, can>(a, plan, (int)l.items, l.cluster, s)
+    return whole ? launch_clusters<T, D, NT, true, can>(a, plan, (int)l.items, l.cluster, s)
                   : launch_clusters<T, D, NT, false, can>(a, plan, (int)l.items, l.cluster, s);
   if (l.cluster > 0)
-    return page16 ? launch_clusters<T, D, NT, true, false>(a, plan, (int)l.items, l.cluster, s)
+    return whole ? launch_clusters<T, D, NT, true, false>(a, plan, (int)l.items, l.cluster, s)
                   : launch_clusters<T, D, NT, false, false>(a, plan, (int)l.items, l.cluster, s);
   // no more CTAs than shares of the longest sequences possible
   const double most = (double)l.items * (double)l.tiles / kMinTiles;
   const int ctas = most < l.full ? (int)most + 1 : l.full;
   plan.by_item = l.items < ctas;
-  return page16 ? launch_shares<T, D, NT, true>(a, plan, ctas, s) : launch_shares<T, D, NT, false>(a, plan, ctas, s);
+  return whole ? launch_shares<T, D, NT, true>(a, plan, ctas, s) : launch_shares<T, D, NT, false>(a, plan, ctas, s);
 }
 
 template <typename T>
 int launch_paged(const PagedArgs& a, void* workspace, int64_t bytes, cudaStream_t s) {
   // 16-byte loads need aligned rows; other views take the scalar kernel
   const size_t es = sizeof(T);
-  bool aligned = tensor_shape(a.dim);
+  bool aligned = built_dim<T>(a.dim) > 0;
   const void* bases[4] = {a.q, a.k, a.v, a.out};
   for (const void* p : bases) aligned = aligned && reinterpret_cast<uintptr_t>(p) % 16 == 0;
   for (int i = 0; i < 3; ++i) aligned = aligned && a.ks[i] * es % 16 == 0 && a.vs[i] * es % 16 == 0;
@@ -1203,9 +1219,9 @@ int launch_paged(const PagedArgs& a, void* workspace, int64_t bytes, cudaStream_
   if (l.workspace > 0 && (workspace == nullptr || bytes < l.workspace || reinterpret_cast<uintptr_t>(workspace) % 16))
     return fail(SPECKV_EINVAL, "speckv_paged_attention: workspace of %lld bytes, %lld needed (16-byte aligned)",
                 (long long)bytes, (long long)l.workspace);
-  if (a.dim == 64)
+  if (l.dim == 64)
     return l.tiles8 == 1 ? launch_tensor<T, 64, 1>(a, l, workspace, s) : launch_tensor<T, 64, 2>(a, l, workspace, s);
-  if (a.dim == 128)
+  if (l.dim == 128)
     return l.tiles8 == 1 ? launch_tensor<T, 128, 1>(a, l, workspace, s) : launch_tensor<T, 128, 2>(a, l, workspace, s);
   return launch_tensor<T, 256, 1>(a, l, workspace, s);
 }
@@ -1271,7 +1287,7 @@ extern "C" int speckv_paged_attention(const void* query, const void* key_pages, 
 extern "C" int64_t speckv_paged_attention_workspace(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim,
                                                     int64_t table_pages, int64_t page_size, int32_t dtype) {
   if (batch < 1 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads != 0 || table_pages < 1 || page_size < 1 ||
-      table_pages > (1ll << 31) / page_size || !tensor_shape(dim))
+      table_pages > (1ll << 31) / page_size || (dtype == SPECKV_F32 ? built_dim<float>(dim) : built_dim<__half>(dim)) == 0)
     return 0;
   const int64_t positions = table_pages * page_size;
   return dtype == SPECKV_F32 ? plan_launch<float>(batch, q_heads, kv_heads, dim, positions, sm_count()).workspace

@@ -299,6 +299,37 @@ def test_attention_peaked_flat_and_negative_scales(dtype, scale):
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('dim', [4, 8, 24, 56, 72, 80, 96, 112, 120, 136, 160, 192, 248])
+def test_attention_head_dims_between(dim, dtype):
+    """Head dims that the kernels read as the next one they are built for, with zeros behind; pools whose
+    rows lie side by side, so that a row's end is the next one's beginning."""
+    lengths = [1, 0, 130, 47, 700]
+    for hq, hkv, page, slack in ((6, 2, 16, 0), (20, 2, 5, 0), (3, 3, 64, 400), (12, 1, 8, 2000)):
+        g = gen(dim + hq)
+        kp, vp, table = filled(5, hkv, dim, page, lengths, dtype, g, slack=slack)
+        q = randn(5, 1, hq * dim, dtype=dtype, g=g).view(5, 1, hq, dim).transpose(1, 2)
+        out = torch.full((6, 1, hq, dim), 7.0, dtype=dtype, device='cuda')
+        paged_attention(q, kp, vp, table, torch.tensor(lengths, device='cuda'), out=out[:5])
+        check_attention(out[:5], q, kp, vp, table, lengths, dim ** -0.5, page, dtype)
+        assert (out[5] == 7.0).all() and _ops.device_error() is None
+
+
+def test_attention_infinite_keys_of_a_dim_between():
+    """fp32 keys of -inf are summed term by term: over the row's own dims only."""
+    g = gen(12)
+    kp, vp, table = filled(1, 2, 80, 16, [90], torch.float32, g)
+    q = randn(1, 4, 1, 80, dtype=torch.float32, g=g).abs()
+    kp[table[0, 1], :, 3] = -math.inf
+    out = paged_attention(q, kp, vp, table, torch.tensor([90], device='cuda'))
+    keep = torch.arange(90, device='cuda') != 19
+    where, row = table[0][torch.arange(90, device='cuda')[keep] // 16], torch.arange(90, device='cuda')[keep] % 16
+    kp2, vp2 = (torch.zeros(6, 2, 16, 80, device='cuda') for _ in range(2))
+    slot = torch.arange(89, device='cuda')
+    kp2[slot // 16, :, slot % 16], vp2[slot // 16, :, slot % 16] = kp[where, :, row], vp[where, :, row]
+    check_attention(out, q, kp2, vp2, torch.arange(6, device='cuda')[None], [89], 80 ** -0.5, 16, torch.float32)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
 @pytest.mark.parametrize('n', [5000, 60000])
 @pytest.mark.parametrize('dim', [64, 128])
 def test_attention_sums_many_small_weights(dtype, n, dim):

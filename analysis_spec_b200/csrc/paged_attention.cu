@@ -202,7 +202,7 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint3
 // 4 x 12000 keys, 16 q / 2 KV heads: 18.1 us at one tile and at two (half the parts), 20.3 at six.
 constexpr int kMinTiles = 2;         // a CTA's share is at least this many tiles
 constexpr int kCluster = 8;          // CTAs of a cluster at most
-// One launch beats two where the work is small (1 x 200 keys 8.2 us, 14.0 as shares) and still where a
+// One launch beats two where the work is small (1 x 200 keys 8.3 us, 12.8 as shares) and still where a
 // CTA has 11 tiles (64 x 256..2048 23.7 us, 24.0); at 21 uneven lengths cost more (64 x 256..4000 37.9, 33.7).
 constexpr int kClusterTiles = 12;    // tiles of a cluster's CTA at most
 

@@ -922,11 +922,12 @@ __global__ void __launch_bounds__(Shape<T, D, NT>::kWarps * 32, Shape<T, D, NT>:
   if (threadIdx.x == 0 && !plan.by_item) plan.joins[cta] = join;
 }
 
-// Few items: a cluster of CTAs each, an equal run of its tiles per CTA, joined through the
-// cluster's shared memory. One launch, no workspace. Where each of its CTAs has an SM to itself, eight
-// warps share the work (WIDE): one warp per scheduler leaves most of the issue slots empty. Bound by latency: 64 sequences of 256 to 2048 positions (16 / 2 heads,
-// bf16) 23.7 us: a block of 16 keys a warp costs 1.3 us of dependent loads and products (11 of them in
-// the longest sequence's CTAs), the rest is launch, length, page and joins; one of 200 positions 8.2 us.
+// Few items: a cluster of CTAs each, an equal run of its tiles per CTA, joined through the cluster's
+// shared memory. One launch, no workspace. Where each of its CTAs has an SM to itself, eight warps share
+// the work (WIDE): one warp per scheduler leaves most of the issue slots empty. Bound by latency: 64
+// sequences of 256 to 2048 positions (16 / 2 heads, bf16) 23.7 us: a block of 16 keys a warp costs 1.3 us
+// of dependent loads and products (11 of them in the longest sequence's CTAs), the rest is launch,
+// length, page and joins; one of 200 positions 8.2 us a call, 6.3 in a captured graph.
 template <typename T, int D, int NT, bool WHOLE, bool WIDE>
 __global__ void __launch_bounds__(Shape<T, D, NT, WIDE>::kWarps * 32, Shape<T, D, NT, WIDE>::kResident)
     paged_attention_cluster_kernel(PagedArgs a, PlanArgs plan) {

@@ -234,7 +234,7 @@ constexpr float kWide = 1048576.f; // references to 2^20 take the fused product
 // at the end. References whose product is so large that the rounding would matter before that
 // (a row of a mask's lowest value, say) take the difference first, vector by vector (wide).
 template <typename T> struct Running {
-  float r = -INFINITY, rc = 0.f, limit = -INFINITY;
+  float r = -INFINITY, rc = 0.f, limit = NAN;  // a vector that is not below `limit` looks at the reference first
   Two s = 0ull, t = 0ull;  // of the even and the odd entries
   bool bad = false, wide = false;  // bad: NaN or +inf seen
 
@@ -293,6 +293,9 @@ template <typename T> struct Running {
         }
         return;
       }
+      // No entry above -inf yet: nothing to add. What stands for -inf has a finite distance from a reference
+      // that takes the fused product only; from none it would pass fp32's range at c above 3e8 (0 x inf).
+      if (r == -INFINITY) return;
     }
     add_vector(v, c);
   }

@@ -400,3 +400,32 @@ def test_rows_beyond_32_bit_offsets():
     assert r.top_ids[14999, 0] == 151640
     grad, = torch.autograd.grad(r.logprobs, x, torch.ones(15000, device='cuda'))
     assert grad[14999, 151640] > 0 and (grad[14999] != 0).all() and not grad[:14999].any()
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('temperature', [1e-29, 1e-20, 1e-9, 1e9, 1e29])
+@pytest.mark.parametrize('vocab', [7, 2500, 40000, 151644])
+def test_masked_rows_at_extreme_temperatures(dtype, temperature, vocab):
+    """Rows that leave five tokens, at the temperatures' ends: the equal largest share the weight (all of
+    the finite ones at high temperatures), whatever the threads that meet -inf alone would make of it."""
+    x = torch.full((2, vocab), -math.inf, dtype=dtype, device='cuda')
+    at = torch.linspace(1, vocab - 1, 5, device='cuda').long()
+    x[:, at] = 1.5
+    x[1, at[1]] = 0.5 if temperature < 1 else 1.25
+    tokens = torch.stack((at[0], at[4]))
+    r = token_logprobs(x, tokens, top=2, temperature=temperature)
+    check_forward(r, x, tokens, 2, temperature)
+    leaf = x.clone().requires_grad_(True)
+    r = token_logprobs(leaf, tokens, temperature=temperature)
+    gh = torch.tensor([1.0, -2.0], device='cuda')
+    # equal weights: the entropy's gradient -p (log p + H) / T is 0 but for the statistics' own error, 3 e p / T
+    grad, = torch.autograd.grad(r.entropy, leaf, gh)
+    spread, e = bounds(x.double() / temperature)
+    p = torch.softmax(x.double() / temperature, -1)
+    lp = torch.where(p > 0, p.log(), 0.0)
+    ref = -p * (lp - (p * lp).sum(-1, keepdim=True)) * gh[:, None] / temperature
+    size = p * (lp.abs() + 3) * gh.abs()[:, None] / temperature
+    tol = size * ((1 + spread) * 3 * e)[:, None] + torch.finfo(dtype).eps / 2 * ref.abs() + 2.0 ** -25
+    # 1 / T passes fp16's range, and so may a true value of ref +- tol: such ones round to infinity
+    got = grad.double().clamp(torch.finfo(dtype).min, torch.finfo(dtype).max)
+    assert ((got - ref).abs() <= tol).all()

@@ -246,7 +246,13 @@ template <typename T> struct Running {
     if (top > r) {
       const float to = top * c;
       const bool is_wide = !(fabsf(to) <= wide_at);
-      const float d = wide || is_wide ? (r - top) * c : rc - to;
+      // between the references the sums are by: r c itself where wide, else its rounding
+      float d = rc - to;
+      if (wide || is_wide) {
+        d = (r - top) * c;
+        if (!is_wide) d += fmaf(top, c, -to);
+        if (!wide) d -= fmaf(r, c, -rc);
+      }
       if (r == -INFINITY || d <= kEmpty) {
         s = t = 0ull;
       } else {

@@ -429,3 +429,20 @@ def test_masked_rows_at_extreme_temperatures(dtype, temperature, vocab):
     # 1 / T passes fp16's range, and so may a true value of ref +- tol: such ones round to infinity
     got = grad.double().clamp(torch.finfo(dtype).min, torch.finfo(dtype).max)
     assert ((got - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize('rows,vocab', [(300, 4096), (300, 70000), (2, 5000)])
+def test_references_that_pass_the_fused_products_border(rows, vocab):
+    """Scaled logits around +-2^20: a thread's reference changes between the form that takes the difference
+    first and the fused one, by steps of log2(e) / 16 whose rounding (2^-5 at most) differs each time."""
+    border = round(2.0 ** 20 * math.log(2.0) * 16) / 16
+    tokens = torch.arange(rows, device='cuda') % 7
+    half = torch.arange(vocab, device='cuda') * 2 >= vocab
+    one = torch.arange(vocab, device='cuda') == vocab - 9
+    j = torch.arange(rows, device='cuda')[:, None] % 24
+    # low entries first, below -2^20; then half of the row, up to 1.6 above them and past the border
+    x = torch.where(half, -border + (1 + j % 9) / 16, -border - (1 + j % 16) / 16).float()
+    check_forward(token_logprobs(x, tokens, top=1), x, tokens, 1, 1.0)
+    # ... and one entry past 2^20, far enough above the rest for a new reference (10 in powers of two)
+    x = torch.where(one, border + (1 + j % 9) / 16, border - 7.0 - (1 + j % 16) / 16).float()
+    check_forward(token_logprobs(x, tokens, top=1), x, tokens, 1, 1.0)

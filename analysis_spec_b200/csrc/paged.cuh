@@ -51,6 +51,15 @@ inline int check_pages(const char* fn, const int64_t* table, int64_t table_strid
   return SPECKV_OK;
 }
 
+// Strides of dimensions of one entry are never taken: they count as 0, so that an odd one does not cost a call
+// its aligned kernel (4000 keys of 8 q / 1 KV heads x 128 in bf16 with a head stride of 7: 12.5 us, 420 before).
+inline void drop_unused_strides(long long* strides, std::initializer_list<int64_t> sizes) {
+  for (const int64_t n : sizes) {
+    if (n == 1) *strides = 0;
+    ++strides;
+  }
+}
+
 inline int check_strides(const char* fn, const int64_t* strides, int n) {
   for (int i = 0; i < n; ++i)
     if (strides[i] < 0) return fail(SPECKV_EINVAL, "%s: negative stride %lld", fn, (long long)strides[i]);

@@ -383,6 +383,12 @@ extern "C" int speckv_paged_append(const void* key, const void* value, const voi
     a.kps[i] = strides[12 + i];
     a.vps[i] = strides[15 + i];
   }
+  drop_unused_strides(a.ks, {batch, kv_heads, rows});
+  drop_unused_strides(a.vs, {batch, kv_heads, rows});
+  drop_unused_strides(a.qs, {batch, q_heads, rows});
+  drop_unused_strides(a.os, {batch, q_heads, rows});
+  drop_unused_strides(a.kps, {num_pages, kv_heads, page_size});
+  drop_unused_strides(a.vps, {num_pages, kv_heads, page_size});
   a.table = {page_table, table_stride, table_pages, num_pages, page_size};
   a.starts = starts;
   a.counts = counts;

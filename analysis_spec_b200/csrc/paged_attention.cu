@@ -1268,6 +1268,9 @@ extern "C" int speckv_paged_attention(const void* query, const void* key_pages, 
     a.ks[i] = strides[2 + i];
     a.vs[i] = strides[5 + i];
   }
+  drop_unused_strides(a.qs, {batch, q_heads});
+  drop_unused_strides(a.ks, {num_pages, kv_heads, page_size});
+  drop_unused_strides(a.vs, {num_pages, kv_heads, page_size});
   a.table = {page_table, table_stride, table_pages, num_pages, page_size};
   a.lengths = lengths;
   a.batch = batch;

@@ -623,3 +623,30 @@ def test_transformers_model_decodes_through_pages():
         w, o = want[b], torch.stack(got[b])
         assert (o - w).abs().max() <= 0.06 * w.abs().max()  # two bf16 layers: some tens of roundings of 2^-8
     assert _ops.device_error() is None
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_strides_of_single_entries_do_not_count(dtype):
+    """A dimension of one entry may have any stride: the same kernels, the same bits."""
+    g = gen(13)
+
+    def odd(x, *dims):
+        return x.as_strided(x.shape, [7 if d in dims else s for d, s in enumerate(x.stride())])
+
+    for n, page in ((300, 16), (16, 16), (40, 1)):
+        kp, vp, table = filled(1, 1, 128, page, [n], dtype, g, extra=0)
+        dims = [1] + [0] * (kp.shape[0] == 1) + [2] * (page == 1)
+        q = randn(1, 1, 1, 128, dtype=dtype, g=g)
+        lengths = torch.tensor([n], device='cuda')
+        want = paged_attention(q, kp, vp, table, lengths)
+        assert torch.equal(paged_attention(odd(q, 0, 1, 2), odd(kp, *dims), odd(vp, *dims), table, lengths), want)
+        new = [randn(1, 1, 1, 128, dtype=dtype, g=g) for _ in range(3)]
+        starts = torch.tensor([n - 1], device='cuda')
+        made = []
+        for turn in (lambda x, *d: x, odd):
+            k2, v2 = kp.clone(), vp.clone()
+            out = paged_append(turn(new[0], 0, 1, 2), turn(new[1], 0, 1, 2), turn(k2, *dims), turn(v2, *dims), table,
+                               starts, query=turn(new[2], 0, 1, 2), rotation=rotation_tables(n, 128))
+            made.append((k2, v2, out))
+        assert all(torch.equal(x.nan_to_num(9.0), y.nan_to_num(9.0)) for x, y in zip(*made))
+    assert _ops.device_error() is None

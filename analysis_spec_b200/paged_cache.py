@@ -148,6 +148,7 @@ class PagedKVCache(Cache):
     def begin(self, counts=1, first=0, *, device=None):
         """Starts a forward over counts[i] new tokens (an int: the same for all) of sequence
         first + i: hands out the pages they need and fixes their positions."""
+        self._step = None  # a begin that raises leaves no forward behind
         live = len(self.lengths)
         if isinstance(counts, int):
             counts = [counts] * (live - first)
@@ -204,23 +205,33 @@ class PagedKVCache(Cache):
 
     # ---- transformers cache ------------------------------------------------------
     def prompt_lengths(self, lengths):
-        """Lengths of the right-padded prompts of the next forward (None: every row is live)."""
+        """Lengths of the right-padded prompts of the next forward (None: every row is live). They hold for
+        that forward alone, whether it succeeds or not; ``reset`` drops them too."""
         self._prompts = None if lengths is None else [int(n) for n in lengths]
 
-    def update(self, key_states, value_states, layer_idx, *args, **kwargs):
-        batch, rows = key_states.shape[0], key_states.shape[2]
-        if layer_idx == 0:
-            if not self.lengths:
-                self.admit(batch)
+    def _begin_update(self, batch, rows, device):
+        prompts, self._prompts, self._prompt_mask = self._prompts, None, {}
+        fresh = not self.lengths
+        if fresh:
+            self.admit(batch)
+        try:
             if batch != len(self.lengths):
                 raise ValueError('KV batch differs from live request count')
             if rows > 1 and any(self.lengths):
                 raise ValueError('after its prompt a paged cache takes one token per sequence at a time')
-            counts = self._prompts if self._prompts is not None else [rows] * batch
+            counts = prompts if prompts is not None else [rows] * batch
             if len(counts) != batch or any(not 0 <= c <= rows for c in counts):
                 raise ValueError('prompt lengths do not match the prompt rows')
-            self.begin(counts, device=key_states.device)
-            self._prompts, self._prompt_mask = None, {}
+            self.begin(counts, device=device)
+        except Exception:
+            if fresh:  # the sequences of a prompt that did not enter
+                self.release([True] * batch)
+            raise
+
+    def update(self, key_states, value_states, layer_idx, *args, **kwargs):
+        batch, rows = key_states.shape[0], key_states.shape[2]
+        if layer_idx == 0:
+            self._begin_update(batch, rows, key_states.device)
         self.append(key_states, value_states, layer_idx)
         if rows > 1:  # the prompt attends to itself: its own rows are all there is
             key_states._speckv_prompt = self._prompt_mask
@@ -246,7 +257,8 @@ class PagedKVCache(Cache):
         return bool(self.lengths)
 
     def reset(self):
-        """Drops every sequence; the pools stay."""
+        """Drops every sequence and the next forward's prompt lengths; the pools stay."""
+        self._prompts = None
         self.release([True] * len(self.lengths))
 
     def statistics(self):

@@ -234,3 +234,32 @@ def test_negative_strides_are_refused(lib):
     with pytest.raises(_lib.SpecKVError, match='negative stride'):
         _lib.call('speckv_paged_attention', P, P, P, _lib.i64_array([0, 0, -1, 0, 0, 0, 0, 0]), P, 2, 2, 4, 16, P, P, 1, 2, 2,
                   128, 1.0, _lib.BF16, None, 0, None)
+
+
+def test_prompt_lengths_hold_for_one_forward(monkeypatch):
+    """A forward that fails takes its prompt lengths and the sequences it admitted with it, and leaves none begun."""
+    monkeypatch.setattr(_ops, 'paged_append', lambda *a: None)
+    cache = PagedKVCache(16, 4, batch_capacity=3, max_length=24)
+    k = torch.zeros(3, 1, 20, 8)
+    cache.prompt_lengths([7, 20])
+    with pytest.raises(ValueError, match='prompt lengths'):
+        cache.update(k, k, 0)
+    assert cache.lengths == [] and cache.free_pages == 16
+    cache.update(k, k, 0)
+    assert cache.lengths == [20, 20, 20]
+    cache.reset()
+    cache.prompt_lengths([7, 25, 13])
+    with pytest.raises(ValueError, match='max_length'):  # fails in begin
+        cache.update(torch.zeros(3, 1, 30, 8), torch.zeros(3, 1, 30, 8), 0)
+    assert cache.lengths == [] and cache.free_pages == 16
+    cache.update(k[:2], k[:2], 0)  # a smaller batch, every row of it live
+    assert cache.lengths == [20, 20]
+    cache.prompt_lengths([7, 20, 13])
+    cache.reset()
+    cache.update(k, k, 0)
+    assert cache.lengths == [20, 20, 20]
+    with pytest.raises(RuntimeError, match='pages needed'):
+        cache.update(k[:, :, :1], k[:, :, :1], 0)
+    assert cache.lengths == [20, 20, 20]
+    with pytest.raises(RuntimeError, match='begin'):
+        cache.append(k[:, :, :1], k[:, :, :1], 0)

@@ -93,6 +93,7 @@ class PagedKVCache(Cache):
         self._table = None           # (batch_capacity, table_pages) int64 on the device
         self._device = None
         self._step = None            # (first, starts, counts, lengths) device views of the begun forward
+        self._rows = 0               # the most new tokens of a sequence in it
         self._prompts, self._prompt_mask = None, {}
 
     # ---- sequences -----------------------------------------------------------
@@ -174,7 +175,7 @@ class PagedKVCache(Cache):
         numbers = torch.tensor([self.lengths[first:first + len(counts)], counts, ends], dtype=torch.long)
         starts, counts_dev, lengths = self._pin(numbers).to(self._device, non_blocking=True).unbind(0)
         self.lengths[first:first + len(counts)] = ends
-        self._step = (first, starts, counts_dev, lengths)
+        self._step, self._rows = (first, starts, counts_dev, lengths), max(counts, default=0)
 
     def _layer_pools(self, layer, key):
         while len(self._pools) <= layer:
@@ -193,6 +194,8 @@ class PagedKVCache(Cache):
     def append(self, key, value, layer, *, query=None, rotation=None, positions=None, interleaved=False):
         """Stores the begun forward's K/V rows of `layer`; returns the rotated queries."""
         first, starts, counts, _ = self._begun(key.shape[0])
+        if key.shape[2] < self._rows:
+            raise ValueError(f'{key.shape[2]} rows for a forward begun over up to {self._rows} new tokens')
         k_pages, v_pages = self._layer_pools(layer, key)
         return _ops.paged_append(key, value, k_pages, v_pages, self.page_table(first, key.shape[0]), starts, counts,
                                  query, rotation, positions, interleaved)

@@ -263,3 +263,21 @@ def test_prompt_lengths_hold_for_one_forward(monkeypatch):
     assert cache.lengths == [20, 20, 20]
     with pytest.raises(RuntimeError, match='begin'):
         cache.append(k[:, :, :1], k[:, :, :1], 0)
+
+
+def test_append_needs_the_begun_rows(monkeypatch):
+    """Fewer rows than begun would leave positions that count as stored and hold nothing."""
+    calls = []
+    monkeypatch.setattr(_ops, 'paged_append', lambda *a: calls.append(a))
+    cache = PagedKVCache(16, 4, batch_capacity=2, max_length=24)
+    cache.admit(2)
+    cache.begin([2, 5], device='cpu')
+    k = torch.zeros(2, 1, 4, 8)
+    with pytest.raises(ValueError, match='4 rows for a forward begun over up to 5'):
+        cache.append(k, k, 0)
+    assert not calls
+    wide = torch.zeros(2, 1, 6, 8)  # padding behind the longest is the callers' choice
+    cache.append(wide, wide, 0)
+    cache.begin(1)
+    cache.append(k[:, :, :1], k[:, :, :1], 0)
+    assert len(calls) == 2

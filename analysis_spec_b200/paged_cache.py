@@ -67,7 +67,10 @@ class PagedKVCache(Cache):
     layer ``append`` and ``attend``. ``admit`` adds empty sequences at the end of the batch,
     ``release`` drops finished ones (the last sequences take their places, as
     ``swap_remove_plan`` has it) and hands their pages back. Sizes live on the host; the table
-    and lengths are copied to the device on the current stream.
+    and lengths are copied to the device on the current stream, into the same memory each time: the
+    ``append`` and ``attend`` calls of a step may be captured into a CUDA graph (every layer's pools made
+    before), and replayed after each ``begin`` over as many tokens of as many sequences from the same
+    first one. ``begin`` and ``release`` stay outside the capture.
 
     As a transformers cache: ``update`` begins a forward at layer 0. Prompts go through empty
     sequences, right-padded (``prompt_lengths`` says how long each is); afterwards one token per
@@ -91,8 +94,9 @@ class PagedKVCache(Cache):
         self._free = list(range(pages - 1, -1, -1))
         self._pools = []             # (key_pages, value_pages) per layer, created on first use
         self._table = None           # (batch_capacity, table_pages) int64 on the device
+        self._numbers = None         # (3 * batch_capacity,) int64 there: starts, counts, lengths of the begun forward
         self._device = None
-        self._step = None            # (first, starts, counts, lengths) device views of the begun forward
+        self._step = None            # (first, starts, counts, lengths) device views of it
         self._rows = 0               # the most new tokens of a sequence in it
         self._prompts, self._prompt_mask = None, {}
 
@@ -120,6 +124,7 @@ class PagedKVCache(Cache):
         from .opd_static_cache import swap_remove_plan
         if len(finished) != len(self.lengths):
             raise ValueError('one entry per live sequence required')
+        self._outside_capture('release')
         for i, done in enumerate(finished):
             if done:
                 self._free += reversed(self._held[i])
@@ -141,6 +146,11 @@ class PagedKVCache(Cache):
             self._table[rows[0]:rows[0] + len(rows)].copy_(self._pin(staged), non_blocking=True)
         else:
             self._table[torch.tensor(rows, device=self._device)] = staged.to(self._device)
+
+    def _outside_capture(self, what):
+        if self._device is not None and self._device.type == 'cuda' and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f'{what}() decides and copies on the host: call it before a captured graph is replayed, '
+                               'not inside its capture')
 
     def _pin(self, t):
         return t.pin_memory() if self._device.type == 'cuda' else t
@@ -164,16 +174,21 @@ class PagedKVCache(Cache):
             raise RuntimeError(f'{sum(wants)} pages needed, {len(self._free)} free')
         if self._device is None:
             self._device = torch.device(device if device is not None else 'cuda')
+        self._outside_capture('begin')
         if self._table is None:
             self._table = torch.zeros((self.batch_capacity, self.table_pages), dtype=torch.long, device=self._device)
+            self._numbers = torch.zeros(3 * self.batch_capacity, dtype=torch.long, device=self._device)
+            self._device = self._table.device
         for i, want in enumerate(wants):
             for _ in range(want):
                 self._held[first + i].append(self._free.pop())
         grown = [first + i for i, want in enumerate(wants) if want]
         if grown:
             self._upload_table(grown)
-        numbers = torch.tensor([self.lengths[first:first + len(counts)], counts, ends], dtype=torch.long)
-        starts, counts_dev, lengths = self._pin(numbers).to(self._device, non_blocking=True).unbind(0)
+        staged = torch.tensor([self.lengths[first:first + len(counts)], counts, ends], dtype=torch.long)
+        numbers = self._numbers[:staged.numel()].view(staged.shape)
+        numbers.copy_(self._pin(staged), non_blocking=True)
+        starts, counts_dev, lengths = numbers.unbind(0)
         self.lengths[first:first + len(counts)] = ends
         self._step, self._rows = (first, starts, counts_dev, lengths), max(counts, default=0)
 

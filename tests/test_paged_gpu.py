@@ -650,3 +650,66 @@ def test_strides_of_single_entries_do_not_count(dtype):
             made.append((k2, v2, out))
         assert all(torch.equal(x.nan_to_num(9.0), y.nan_to_num(9.0)) for x, y in zip(*made))
     assert _ops.device_error() is None
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_captured_step_of_a_cache(dtype):
+    """Two layers of a decode step captured once and replayed over steps that fill and open pages, with other
+    sequences admitted and released in between, beside the same steps as calls on a second cache."""
+    g = gen(14)
+    hq, hkv, dim, layers, batch = 8, 2, 128, 2, 3
+    tables = rotation_tables(160, dim)
+    caches = [PagedKVCache(60, 16, batch_capacity=5, max_length=160) for _ in range(2)]
+    new = [[randn(batch, h, 1, dim, dtype=dtype, g=g) for h in (hq, hkv, hkv)] for _ in range(layers)]
+
+    def layers_of(cache):
+        out = []
+        for layer, (q, k, v) in enumerate(new):
+            out.append(cache.attend(cache.append(k, v, layer, query=q, rotation=tables), layer))
+        return out
+
+    def prompt(counts, first):
+        for layer in range(layers):
+            k, v = (randn(len(counts), hkv, max(counts), dim, dtype=dtype, g=g) for _ in range(2))
+            for cache in caches:
+                if layer == 0:
+                    cache.begin(counts, first)
+                cache.append(k, v, layer, rotation=tables)
+
+    for cache in caches:
+        cache.admit(batch)
+    prompt([15, 1, 40], 0)
+    captured, eager = caches
+    for cache in caches:
+        cache.begin()
+    want = layers_of(eager)
+    layers_of(captured)  # as warm-up: stores the same rows as the capture's first replay
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = layers_of(captured)
+        with pytest.raises(RuntimeError, match='not inside its capture'):
+            captured.begin()
+    for step in range(24):
+        if step == 8:
+            for cache in caches:
+                cache.admit(2)
+            prompt([20, 33], batch)
+        if step == 16:
+            for cache in caches:
+                assert cache.release([False] * batch + [True] * 2) == [0, 1, 2]
+        if step:
+            for q, k, v in new:
+                for t in (q, k, v):
+                    t.copy_(randn(*t.shape, dtype=dtype, g=g))
+            for cache in caches:
+                cache.begin([1] * batch, 0)
+            want = layers_of(eager)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want)), step
+    assert captured.lengths == eager.lengths == [39, 25, 64]
+    kp, vp = captured._pools[1]
+    check_attention(got[1], paged_append(new[1][1], new[1][2], kp.clone(), vp.clone(), captured.page_table(),
+                                         torch.tensor([38, 24, 63], device='cuda'), query=new[1][0], rotation=tables),
+                    kp, vp, captured.page_table(), captured.lengths, dim ** -0.5, 16, dtype)
+    assert _ops.device_error() is None

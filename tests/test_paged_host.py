@@ -281,3 +281,28 @@ def test_append_needs_the_begun_rows(monkeypatch):
     cache.begin(1)
     cache.append(k[:, :, :1], k[:, :, :1], 0)
     assert len(calls) == 2
+
+
+def test_a_step_lies_in_the_same_memory_each_time(monkeypatch):
+    """Table, starts, counts and lengths keep their addresses, which a captured step has recorded; what
+    happens on the host is refused inside a capture, and changes nothing."""
+    cache = PagedKVCache(16, 4, batch_capacity=4, max_length=40)
+    cache.admit(2)
+    cache.begin([5, 9], device='cpu')
+    cache.begin()
+    step = cache._step
+    places = [t.data_ptr() for t in (*step[1:], cache.page_table())]
+    assert cache.admit(1) == 2
+    cache.begin([3], first=2)
+    assert cache.release([False, False, True]) == [0, 1]
+    for i in range(5):
+        cache.begin()
+        assert [t.data_ptr() for t in (*cache._step[1:], cache.page_table())] == places
+        assert [t.tolist() for t in step[1:]] == [[6 + i, 10 + i], [1, 1], [7 + i, 11 + i]]
+    cache._device = torch.device('cuda')  # as if the pools were on a GPU whose stream is being captured
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
+    before = cache.lengths[:], cache.free_pages
+    for refused in (cache.begin, lambda: cache.release([True, False])):
+        with pytest.raises(RuntimeError, match='not inside its capture'):
+            refused()
+    assert (cache.lengths, cache.free_pages) == before

@@ -279,6 +279,12 @@ class PagedKVCache(Cache):
         self._prompts = None
         self.release([True] * len(self.lengths))
 
+    def _unsupported(self, *args, **kwargs):
+        raise NotImplementedError('a paged cache admits and releases whole sequences (admit, release); its rows are '
+                                  'not cropped, reordered or repeated')
+
+    crop = reorder_cache = batch_repeat_interleave = batch_select_indices = _unsupported
+
     def statistics(self):
         return {'pages': self.pages, 'free_pages': len(self._free), 'sequences': len(self.lengths),
                 'kv_cache_bytes': sum(p.numel() * p.element_size() for pair in self._pools if pair for p in pair)}

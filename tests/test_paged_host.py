@@ -306,3 +306,16 @@ def test_a_step_lies_in_the_same_memory_each_time(monkeypatch):
         with pytest.raises(RuntimeError, match='not inside its capture'):
             refused()
     assert (cache.lengths, cache.free_pages) == before
+
+
+def test_cache_operations_on_rows_are_refused(monkeypatch):
+    """transformers' own forms of these pass over a cache without layer objects and change nothing."""
+    monkeypatch.setattr(_ops, 'paged_append', lambda *a: None)
+    cache = PagedKVCache(8, 4, batch_capacity=2, max_length=16)
+    k = torch.zeros(2, 1, 3, 8)
+    cache.update(k, k, 0)
+    for call in (lambda: cache.crop(2), lambda: cache.reorder_cache(torch.tensor([1, 0])),
+                 lambda: cache.batch_repeat_interleave(2), lambda: cache.batch_select_indices(torch.tensor([0]))):
+        with pytest.raises(NotImplementedError, match='admit, release'):
+            call()
+    assert cache.lengths == [3, 3]

@@ -777,10 +777,12 @@ def _front(name, *args):
     profile.calls += 1
     if not profile.enabled:
         return getattr(_lib.front(), name)(*args)
-    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
-    start.record()
-    out = getattr(_lib.front(), name)(*args)
-    end.record()
+    dev = _first_device(args)
+    with torch.cuda.device(dev if dev is not None else torch.cuda.current_device()):  # where the launch goes
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        out = getattr(_lib.front(), name)(*args)
+        end.record()
     profile.events.setdefault('speckv_' + name, []).append((start, end))
     return out
 

@@ -319,3 +319,40 @@ def test_cache_operations_on_rows_are_refused(monkeypatch):
         with pytest.raises(NotImplementedError, match='admit, release'):
             call()
     assert cache.lengths == [3, 3]
+
+
+def test_profile_events_go_to_the_operands_gpu(monkeypatch):
+    """The front end launches on its operands' GPU; events of the current one would time nothing."""
+    class Device:
+        now = 0
+
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, Device.now = Device.now, self.index
+
+        def __exit__(self, *error):
+            Device.now = self.before
+
+    class Event:
+        def __init__(self, enable_timing):
+            self.at = None
+
+        def record(self):
+            self.at = Device.now
+
+    class Front:
+        def paged_attention(self, *args):
+            return Device.now
+
+    monkeypatch.setattr(torch.cuda, 'device', Device)
+    monkeypatch.setattr(torch.cuda, 'Event', Event)
+    monkeypatch.setattr(torch.cuda, 'current_device', lambda: Device.now)
+    monkeypatch.setattr(_lib, 'front', Front)
+    monkeypatch.setattr(_ops, '_first_device', lambda values: 1)
+    monkeypatch.setattr(_lib.profile, 'enabled', True)
+    monkeypatch.setattr(_lib.profile, 'events', {})
+    monkeypatch.setattr(_lib.profile, 'calls', 0)
+    assert _ops._front('paged_attention', None) == 1 and Device.now == 0
+    assert [(s.at, e.at) for s, e in _lib.profile.events['speckv_paged_attention']] == [(1, 1)]

@@ -357,6 +357,8 @@ struct ScoreFunction : public torch::autograd::Function<ScoreFunction> {
 py::tuple token_logprobs(const Tensor& logits, const Maybe& tokens, const Maybe& rows, int64_t top,
                          double temperature) {
   auto item = [](const Tensor& t) -> py::object { return t.defined() ? py::cast(t) : py::none(); };
+  if (logits._fw_grad(0).defined())
+    value_error("token_logprobs", "no forward-mode derivative: the logits carry a tangent, which would be lost");
   if (logits.requires_grad() && at::GradMode::is_enabled()) {
     if (get(rows) != nullptr)
       value_error("token_logprobs", "rows selects verified rows of a rollout and carries no gradient; detach the "

@@ -30,6 +30,7 @@ def token_logprobs(logits, tokens=None, *, rows=None, top=0, temperature=1.0):
     b's logits for output (b, i) (negative: skipped); no gradient flows through it. A token outside
     the vocabulary or a row outside the logits is skipped and reported by ``_ops.device_error``.
     A row of -inf alone has log-probability -inf and entropy 0; NaN or +inf in a row makes its
-    numbers NaN. The outputs carry a gradient to ``logits`` (not twice differentiable).
+    numbers NaN. The outputs carry a gradient to ``logits`` (not twice differentiable;
+    forward-mode tangents are refused).
     """
     return TokenLogprobs(*_ops.token_logprobs(logits, tokens, rows, top, temperature))

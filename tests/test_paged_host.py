@@ -356,3 +356,14 @@ def test_profile_events_go_to_the_operands_gpu(monkeypatch):
     monkeypatch.setattr(_lib.profile, 'calls', 0)
     assert _ops._front('paged_attention', None) == 1 and Device.now == 0
     assert [(s.at, e.at) for s, e in _lib.profile.events['speckv_paged_attention']] == [(1, 1)]
+
+
+def test_tangents_are_refused():
+    from torch.autograd import forward_ad
+    x, t = torch.zeros(3, 7), torch.zeros(3, dtype=torch.long)
+    with forward_ad.dual_level():
+        for logits in (forward_ad.make_dual(x, x + 1), forward_ad.make_dual(x.requires_grad_(True), x + 1)):
+            with pytest.raises(ValueError, match='forward-mode'):
+                token_logprobs(logits, t)
+    with pytest.raises(RuntimeError, match='no CPU path'):
+        token_logprobs(x, t)

@@ -151,32 +151,32 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
 }
 
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
                "{%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// An fp32 number as two tf32 parts: hi is x rounded (off by 2^-11 of x at most), lo the rest, of
-// which the product takes 11 bits: x = hi + lo up to 2^-22 of x.
+// An fp32 number as two tf32 parts: hi is x rounded (off by 2^-11 of x at most), lo the rest, at most 12 bits,
+// of which the product takes 11: x = hi + lo up to 2^-23 of x. The rounding is two whole-number instructions:
+// cvt.rna, which shares a slower pipe, made 64 x 256..2048 49.9 us instead of 47.5. Numbers within 2^-12 of fp32's
+// largest round to infinity, and what is infinite has no rest (NaN).
 __device__ __forceinline__ void split(uint32_t x, uint32_t& hi, uint32_t& lo) {
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(__uint_as_float(x)));
+  hi = (x + 0x1000u) & 0xffffe000u;
   lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
 }
 // The same, not moved out of its loop: the parts of all queries would not fit the registers.
 __device__ __forceinline__ void split_here(uint32_t x, uint32_t& hi, uint32_t& lo) {
-  asm volatile("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(__uint_as_float(x)));
+  asm volatile("{\n\t.reg .u32 r;\n\tadd.u32 r, %1, 0x1000;\n\tand.b32 %0, r, 0xffffe000;\n\t}" : "=r"(hi) : "r"(x));
   lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
 }
-// a b of fp32 operands: the three products above 2^-22.
-__device__ __forceinline__ void mma_fp32(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&bh)[2],
-                                         const uint32_t (&bl)[2]) {
-  uint32_t ah[4], al[4];
+__device__ __forceinline__ void split4(const uint32_t (&x)[4], uint32_t (&hi)[4], uint32_t (&lo)[4]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) split(a[i], ah[i], al[i]);
-  mma_tf32(c, al, bh[0], bh[1]);
-  mma_tf32(c, ah, bl[0], bl[1]);
-  mma_tf32(c, ah, bh[0], bh[1]);
+  for (int i = 0; i < 4; ++i) split(x[i], hi[i], lo[i]);
 }
+// A product of fp32 operands is the three products above 2^-22: ah bh, and the small ones al bh + ah bl. The
+// matrix instructions cut their sums toward zero, about 2^-24 of what they hold each time: sums kept in them over a
+// sequence came out low by up to 2.5e-6. So sums of ah bh are kept there over a few instructions only and go on in
+// rounded fp32 additions; the small products are 2^-11 of them, and so is what is cut from theirs.
 
 // Transpose of an 8 x 8 matrix of 16-bit elements held as a matrix fragment.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
@@ -554,7 +554,8 @@ __device__ __forceinline__ void attend_part16(const PagedArgs& a, unsigned char*
 
 // fp32 caches. Twice the bytes a key and six instructions a product: K and V rows are copied ahead
 // through a ring of shared memory per warp (blocks of K and of V in turn, 16 bytes a lane and copy),
-// which leaves the registers to the products. Products are three of tf32 parts.
+// which leaves the registers to the products. Products are three of tf32 parts. Against 64 bits the outputs are
+// off by 1.9e-7 to 2.9e-7 (rms, normal inputs, 200 to 130000 keys), plain fp32 operations by 3.0e-7 to 9.3e-7.
 template <int D, int NT, bool WHOLE, typename Emit>
 __device__ __forceinline__ void attend_part32(const PagedArgs& a, unsigned char* shared,
                                               Parts<Shape<float, D, NT>::kWarps, NT>& sm, long long b, int hk, int h0,
@@ -563,6 +564,7 @@ __device__ __forceinline__ void attend_part32(const PagedArgs& a, unsigned char*
   typedef Reference<float> R;
   constexpr int CHUNKS = S::kRow / 16, E = 4, BLOCK = 16 * S::kRow;
   constexpr int STEPS = D / (2 * E);      // products of a score: 8 dims each
+  constexpr int kChain = 4;               // of them whose large products are summed in the matrix instructions
   constexpr int ROWS = 32 / CHUNKS > 0 ? 32 / CHUNKS : 1;  // rows that one copy of a warp covers
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const long long group = a.q_heads / a.kv_heads;
@@ -684,37 +686,48 @@ __device__ __forceinline__ void attend_part32(const PagedArgs& a, unsigned char*
   for (int i = 0; i < count; ++i) {
     const uint32_t k_at = mine + stage * BLOCK;
     // scores of 16 keys x 8 heads: rows keys g, g + 8, columns heads 2t, 2t + 1
-    float s[NT][4], s2[NT][4];
+    float s[NT][4], large[NT][4], small[NT][2][4];
 #pragma unroll
     for (int u = 0; u < NT; ++u)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[u][e] = s2[u][e] = 0.f;
+      for (int e = 0; e < 4; ++e) s[u][e] = small[u][0][e] = small[u][1][e] = 0.f;
 #pragma unroll
     for (int j = 0; j < STEPS; ++j) {
-      uint32_t k[4];
+      uint32_t k[4], kh[4], kl[4];
       load_matrices(k_at + k_lane + (((2 * j + k_chunk) ^ k_swizzle) << 4), k);
+      split4(k, kh, kl);
 #pragma unroll
       for (int u = 0; u < NT; ++u) {
-        float(&to)[4] = j & 1 ? s2[u] : s[u];
         uint32_t qh[2], ql[2];
         split_here(q[u][j][0], qh[0], ql[0]);
         split_here(q[u][j][1], qh[1], ql[1]);
-        mma_fp32(to, k, qh, ql);
+        if (j % kChain == 0)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) large[u][e] = 0.f;
+        mma_tf32(large[u], kh, qh[0], qh[1]);
+        mma_tf32(small[u][0], kl, qh[0], qh[1]);
+        mma_tf32(small[u][1], kh, ql[0], ql[1]);
+        if (j % kChain == kChain - 1)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[u][e] += large[u][e];
       }
     }
-    // an infinite key has no parts (inf - inf): such a block's scores are summed term by term
+    // parts of infinite or huge keys may cancel (inf - inf): such a block's scores are summed term by term
     bool lost = false;
 #pragma unroll
     for (int u = 0; u < NT; ++u)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) lost |= s[u][e] + s2[u][e] != s[u][e] + s2[u][e];
+      for (int e = 0; e < 4; ++e) {
+        s[u][e] += small[u][0][e] + small[u][1][e];
+        lost |= s[u][e] != s[u][e];
+      }
     if (__any_sync(0xffffffffu, lost)) {
 #pragma unroll
       for (int u = 0; u < NT; ++u)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int row = g + 8 * (e >> 1), head = u * 8 + 2 * t + (e & 1);
-          s[u][e] = s2[u][e] = 0.f;
+          s[u][e] = 0.f;
           if (head < heads) {
             const float* p = static_cast<const float*>(a.q) + b * a.qs[0] + (hk * group + h0 + head) * a.qs[1];
             for (int d = 0; d < dim; ++d)
@@ -730,13 +743,10 @@ __device__ __forceinline__ void attend_part32(const PagedArgs& a, unsigned char*
     uint32_t ph[NT][2][2], pl[NT][2][2];  // weights as the second operand: keys t and t + 4 of each half, head g
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
+      float(&z)[4] = s[u];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[u][e] = (s[u][e] + s2[u][e]) * a.scale_log2;
-      if (part)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (!(live >> (e >> 1) & 1u)) s[u][e] = -INFINITY;
-      float top0 = fmaxf(s[u][0], s[u][2]), top1 = fmaxf(s[u][1], s[u][3]);
+      for (int e = 0; e < 4; ++e) z[e] = part && !(live >> (e >> 1) & 1u) ? -INFINITY : z[e] * a.scale_log2;
+      float top0 = fmaxf(z[0], z[2]), top1 = fmaxf(z[1], z[3]);
       if (__any_sync(0xffffffffu, top0 > m[u][0] + R::kSlack || top1 > m[u][1] + R::kSlack)) {
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) {
@@ -759,8 +769,14 @@ __device__ __forceinline__ void attend_part32(const PagedArgs& a, unsigned char*
         }
       }
       const float r0 = m[u][0] == -INFINITY ? 0.f : m[u][0], r1 = m[u][1] == -INFINITY ? 0.f : m[u][1];
-      const float p[4] = {exp2_fast(s[u][0] - r0), exp2_fast(s[u][1] - r1), exp2_fast(s[u][2] - r0),
-                          exp2_fast(s[u][3] - r1)};
+      float p[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        // the weight that the products take: what they cut from the low part is not in the total either
+        uint32_t hi, lo;
+        split(__float_as_uint(exp2_fast(z[e] - (e & 1 ? r1 : r0))), hi, lo);
+        p[e] = __uint_as_float(hi) + __uint_as_float(lo & 0xffffe000u);
+      }
       l[u][0] += p[0] + p[2];
       l[u][1] += p[1] + p[3];
 #pragma unroll
@@ -773,7 +789,8 @@ __device__ __forceinline__ void attend_part32(const PagedArgs& a, unsigned char*
         }
     }
 #pragma unroll
-    for (int j = 0; j < D / 16; ++j)
+    for (int j = 0; j < D / 16; ++j) {
+      uint32_t vh[2][4], vl[2][4];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         uint32_t v[4];
@@ -782,9 +799,22 @@ __device__ __forceinline__ void attend_part32(const PagedArgs& a, unsigned char*
           const int row = 8 * x + t + 4 * (e >> 1);
           v[e] = load_word(v_at + row * S::kRow + (((4 * j + (g >> 2) + 2 * (e & 1)) ^ swizzle(row)) << 4) + (g & 3) * 4);
         }
-#pragma unroll
-        for (int u = 0; u < NT; ++u) mma_fp32(o[u][j], v, ph[u][x], pl[u][x]);
+        split4(v, vh[x], vl[x]);
       }
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};  // of the block: the small products first
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          mma_tf32(sum, vl[x], ph[u][x][0], ph[u][x][1]);
+          mma_tf32(sum, vh[x], pl[u][x][0], pl[u][x][1]);
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) mma_tf32(sum, vh[x], ph[u][x][0], ph[u][x][1]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[u][j][e] += sum[e];
+      }
+    }
     next_piece(2 * i + 1);
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
@@ -815,7 +845,7 @@ __device__ __forceinline__ long long tiles_of(const PagedArgs& a, long long b, i
 // Equal shares of all sequences' tiles, one per resident CTA: no CTA waits for a longer sequence, and a
 // long cache is split as finely as the GPU is wide. Bound by memory: 256 sequences of 512 to 6144
 // positions (28 q / 4 KV heads x 128, fp16) 269 to 279 us, 2 of 100001 to 130000 (40 / 8, bf16) 145 to
-// 149 us, 0.97 of the copy bandwidth measured on this GPU; the first in fp32 693 us (0.78).
+// 149 us, 0.97 of the copy bandwidth measured on this GPU; the first in fp32 609 to 664 us (0.82 to 0.89).
 template <typename T, int D, int NT, bool WHOLE>
 __global__ void __launch_bounds__(Shape<T, D, NT>::kWarps * 32, Shape<T, D, NT>::kResident)
     paged_attention_share_kernel(PagedArgs a, PlanArgs plan) {

@@ -583,7 +583,8 @@ int speckv_paged_append(const void* key, const void* value, const void* query, v
  * length 0 (or less) gives zeros; an infinite value makes its output NaN. out is contiguous
  * (batch, 1, q_heads, dim). strides: 8 element strides, (b, h) of query and (page, head, position)
  * of key_pages and value_pages. Head dims to 256: rows of whole 16-byte pieces at 16-byte aligned
- * strides take the tensor-core kernels (fp32 in three tf32 products, to 2^-22; dims 64, 128 and 256
+ * strides take the tensor-core kernels (fp32 in three tf32 products, to 2^-21, where a
+ * value within 2^-12 of the type's largest counts as infinite; dims 64, 128 and 256
  * with pages of a multiple of 16 positions run best), other views a CUDA-core kernel.
  * workspace (16-byte aligned, workspace_bytes at least speckv_paged_attention_workspace of the
  * same sizes on the same device; it holds nothing between calls) may be shared by calls that

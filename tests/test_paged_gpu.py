@@ -713,3 +713,61 @@ def test_captured_step_of_a_cache(dtype):
                                          torch.tensor([38, 24, 63], device='cuda'), query=new[1][0], rotation=tables),
                     kp, vp, captured.page_table(), captured.lengths, dim ** -0.5, 16, dtype)
     assert _ops.device_error() is None
+
+
+@pytest.mark.parametrize('hq,hkv,dim,page,lengths', [
+    (16, 2, 128, 16, [200, 1000, 4000]), (28, 4, 128, 64, [2500] * 9), (8, 8, 64, 32, [3000, 700, 41]),
+    (4, 2, 256, 16, [3000, 500]), (32, 2, 128, 16, [9000, 300]), (6, 2, 96, 16, [1500, 90]), (8, 1, 128, 16, [130000])])
+def test_attention_in_fp32_has_a_bound_of_its_own(hq, hkv, dim, page, lengths):
+    """Over the outputs of a call, whose single errors are of either sign.
+
+    Signed mean, with values above 1: an output is a mean of its values, each off by 2^-23 to either side (its
+    parts), summed by blocks of 16 keys whose two large products are cut toward zero, 2^-24 of the sum each, then
+    in rounded additions. So the mean over the outputs is low by 2^-23 and scatters with the rounding of single
+    outputs (2^-22 each at most): 2^-23 + 2^-22 / sqrt(outputs).
+    Root mean square over that of the outputs, with normal q, k, v and a scale of D^-1/2, where a score is D products
+    of D^-1/2 and a weight's relative error counts as a value's does. A product of two operands in parts is off
+    by 2^-21 of itself (2^-23 for each, 2^-22 dropped): 2^-21 for the score's, 2^-21 for the values'. Four
+    instructions' sums are cut by 2^-23 each: 2^-21 for a score (the parts of D / 32 sums of 32, independent); two for
+    the values of a block, 2^-22. The scaled score's rounding, its distance's and the exponential's: 2^-22 each.
+    Together sqrt(3 2^-42 + 4 2^-44) = 2^-20."""
+    g = gen(21 + dim)
+    batch, scale = len(lengths), dim ** -0.5
+    n = torch.tensor(lengths, device='cuda')
+    for slack in (0, -(-13000 // page)):
+        kp, vp, table = filled(batch, hkv, dim, page, lengths, torch.float32, g, slack=slack)
+        q = randn(batch, hq, 1, dim, dtype=torch.float32, g=g)
+        above = vp.abs() + 1.0
+        out, low = paged_attention(q, kp, vp, table, n).double(), paged_attention(q, kp, above, table, n).double()
+        own, signed = [], []
+        for b, m in enumerate(lengths):
+            slot = torch.arange(m, device='cuda')
+            where = table[b][slot // page]
+            k, v, w = (x[where, :, slot % page].transpose(0, 1).double() for x in (kp, vp, above))
+            p = torch.softmax(q[b, :, 0].double().view(hkv, hq // hkv, dim) @ k.transpose(1, 2) * scale, -1)
+            ref = p @ v
+            own.append((out[b, 0].view_as(ref) - ref) / ref.square().mean().sqrt())
+            ref = p @ w
+            signed.append((low[b, 0].view_as(ref) - ref) / ref)
+        own, signed = (torch.cat([x.flatten() for x in part]) for part in (own, signed))
+        assert signed.mean().abs() <= 2.0 ** -23 + 2.0 ** -22 / signed.numel() ** 0.5, signed.mean().item()
+        assert own.square().mean().sqrt() <= 2.0 ** -20, own.square().mean().sqrt().item()
+
+
+@pytest.mark.parametrize('dim,slack', [(128, 0), (64, 900), (96, 0)])
+def test_attention_keys_of_the_types_lowest_value(dim, slack):
+    """fp32 keys that hold the type's lowest value, whose first part rounds to -inf, weigh nothing beside the
+    others where their products are negative, and everything where they are positive."""
+    g = gen(22)
+    kp, vp, table = filled(1, 1, dim, 16, [300], torch.float32, g, slack=slack)
+    q = torch.zeros(1, 2, 1, dim, device='cuda')
+    q[0, 0, 0, 1], q[0, 1, 0, 1] = 0.25, -0.25
+    kp[:, :, :, 1] = 0.0
+    kp[table[0, 2], 0, 5, 1] = torch.finfo(torch.float32).min
+    out = paged_attention(q, kp, vp, table, torch.tensor([300], device='cuda'), 1.0)[0, 0].double()
+    slot = torch.arange(300, device='cuda')
+    v = vp[table[0][slot // 16], 0, slot % 16].double()
+    rest = (v.sum(0) - v[37]) / 299
+    # equal weights of 1, summed exactly: the values' parts, 20 roundings of sums and one of the quotient
+    assert ((out[0] - rest).abs() <= 24 * 2.0 ** -24 * v.abs().mean(0) + 2.0 ** -23 * v.abs().mean(0)).all()
+    assert ((out[1] - v[37]).abs() <= 2.0 ** -22 * v[37].abs()).all()

@@ -44,7 +44,7 @@ def paged_attention(query, key_pages, value_pages, page_table, lengths, scale=No
 
     ``query`` (batch, q_heads, 1, head_dim); pools and ``page_table`` as for ``paged_append``;
     ``lengths`` (batch,) int64. Query head h reads KV head h // (q_heads // kv_heads). A sequence
-    of length 0 gives zeros, an infinite value NaN. fp32 products are taken to 2^-21 and summed in fp32
+    of length 0 gives zeros, an infinite value makes its outputs infinite or NaN. fp32 products are taken to 2^-21 and summed in fp32
     (a value within 2^-12 of the type's largest counts as infinite). Returns (batch, 1, q_heads,
     head_dim). Head dims to 256. Inference only: no gradient flows through it.
     """

@@ -580,7 +580,8 @@ int speckv_paged_append(const void* key, const void* value, const void* query, v
 /* Attention of one new token per sequence over a paged cache:
  *   out[b][0][hq][:] = softmax_c(q[b][hq] . k_c * scale) v_c,   c < lengths[b]
  * with KV head hq / (q_heads / kv_heads). lengths is a device array of batch int64; a sequence of
- * length 0 (or less) gives zeros; an infinite value makes its output NaN. out is contiguous
+ * length 0 (or less) gives zeros; an infinite value makes its outputs infinite or
+ * NaN (which of them depends on the kernel and on how the weight rounds). out is contiguous
  * (batch, 1, q_heads, dim). strides: 8 element strides, (b, h) of query and (page, head, position)
  * of key_pages and value_pages. Head dims to 256: rows of whole 16-byte pieces at 16-byte aligned
  * strides take the tensor-core kernels (fp32 in three tf32 products, to 2^-21, where a

@@ -771,3 +771,27 @@ def test_attention_keys_of_the_types_lowest_value(dim, slack):
     # equal weights of 1, summed exactly: the values' parts, 20 roundings of sums and one of the quotient
     assert ((out[0] - rest).abs() <= 24 * 2.0 ** -24 * v.abs().mean(0) + 2.0 ** -23 * v.abs().mean(0)).all()
     assert ((out[1] - v[37]).abs() <= 2.0 ** -22 * v[37].abs()).all()
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('dim,off,slack', [(128, 0, 0), (128, 0, 900), (128, 1, 0), (96, 0, 0), (41, 0, 0)])
+def test_attention_infinite_values(dtype, dim, off, slack):
+    """An infinite value makes its dim of its KV head's outputs infinite or NaN, in every kernel and launch form,
+    and no other; behind the length it is not there."""
+    g = gen(15)
+    lengths = [3000, 40, 700]
+    kp, vp, table = filled(3, 2, dim, 16, lengths, dtype, g, slack=slack)
+    if off:  # off 16-byte alignment
+        kp, vp = (torch.zeros(p.numel() + 1, device='cuda', dtype=dtype)[1:].view(p.shape).copy_(p) for p in (kp, vp))
+    q = randn(3, 8, 1, dim, dtype=dtype, g=g)
+    n = torch.tensor(lengths, device='cuda')
+    want = paged_attention(q, kp, vp, table, n)
+    check_attention(want, q, kp, vp, table, lengths, dim ** -0.5, 16, dtype)
+    vp[table[0, 9], 0, 3, 17] = math.inf
+    vp[table[1, 1], 1, 2, 5] = -math.inf
+    vp[table[2, 43], 1, 13, 7] = math.inf  # position 701 of 700
+    out = paged_attention(q, kp, vp, table, n)
+    lost = torch.zeros_like(out, dtype=torch.bool)
+    lost[0, 0, :4, 17] = lost[1, 0, 4:, 5] = True
+    assert torch.equal(~out.isfinite(), lost) and torch.equal(out[~lost], want[~lost])
+    assert _ops.device_error() is None

@@ -795,3 +795,34 @@ def test_attention_infinite_values(dtype, dim, off, slack):
     lost[0, 0, :4, 17] = lost[1, 0, 4:, 5] = True
     assert torch.equal(~out.isfinite(), lost) and torch.equal(out[~lost], want[~lost])
     assert _ops.device_error() is None
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('hq,hkv,dim,page,off,slack', [
+    (4, 2, 128, 16, 0, 0), (4, 2, 128, 16, 0, 900), (4, 2, 128, 24, 0, 0), (4, 2, 128, 24, 0, 600), (4, 2, 64, 16, 0, 900),
+    (4, 2, 256, 16, 0, 900), (20, 1, 128, 16, 0, 900), (4, 2, 128, 16, 1, 0), (4, 2, 40, 7, 0, 0), (4, 2, 80, 16, 0, 900)])
+def test_bad_pages_in_every_kernel(dtype, hq, hkv, dim, page, off, slack):
+    """Pages outside the pools, inside an item of one CTA, of a cluster and of several shares: reported, and the
+    outputs are those without these pages' positions, in every kernel, launch form and type."""
+    g = gen(8)
+    lengths = [4000, 6 * page + 3, 33]
+    kp, vp, table = filled(3, hkv, dim, page, lengths, dtype, g, slack=slack)
+    if off:
+        kp, vp = (torch.zeros(p.numel() + 1, device='cuda', dtype=dtype)[1:].view(p.shape).copy_(p) for p in (kp, vp))
+    q = randn(3, hq, 1, dim, dtype=dtype, g=g)
+    for bad in (-1, kp.shape[0], 1 << 45):
+        t = table.clone()
+        t[0, 5], t[0, 90], t[1, 2] = bad, bad, bad
+        out = paged_attention(q, kp, vp, t, torch.tensor(lengths, device='cuda'))
+        err = _ops.device_error()
+        assert err is not None and err[0] == 'page table'
+        for b, gone in enumerate(((5, 90), (2,), ())):
+            rest = [i for i in range(table.shape[1]) if i not in gone]
+            check_attention(out[b:b + 1], q[b:b + 1], kp, vp, table[b:b + 1, rest], [lengths[b] - len(gone) * page],
+                            dim ** -0.5, page, dtype)
+    if table.shape[1] * page == lengths[0]:  # a length past the table counts to its end, one below zero not at all
+        out = paged_attention(q, kp, vp, table, torch.tensor([1 << 40, lengths[1], -5], device='cuda'))
+        err = _ops.device_error()
+        assert err is not None and err[0] == 'page table'
+        check_attention(out, q, kp, vp, table, [*lengths[:2], 0], dim ** -0.5, page, dtype)
+    assert _ops.device_error() is None

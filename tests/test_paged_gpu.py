@@ -826,3 +826,49 @@ def test_bad_pages_in_every_kernel(dtype, hq, hkv, dim, page, off, slack):
         assert err is not None and err[0] == 'page table'
         check_attention(out, q, kp, vp, table, [*lengths[:2], 0], dim ** -0.5, page, dtype)
     assert _ops.device_error() is None
+
+
+@pytest.mark.parametrize('dtype,dim', [(torch.bfloat16, 128), (torch.float16, 128), (torch.float32, 64)])
+def test_prompts_through_the_plain_calls(dtype, dim):
+    """Prompts enter beside a live sequence: stored, queries and keys rotated by the same launch, attention of
+    their own rows; then a step of one token for all."""
+    from analysis_spec_b200.tree_attention import prompt_mask, tree_verify_attention
+    g = gen(16)
+    hq, hkv, lengths = 8, 2, [9, 33, 1]
+    cache = PagedKVCache(20, 16, batch_capacity=4, max_length=80)
+    tables = rotation_tables(80, dim)
+    kept = []
+    for group in ([20], lengths):
+        first, masks = cache.admit(len(group)), {}
+        cache.begin(group, first)
+        q, k, v = (randn(len(group), h, max(group), dim, dtype=dtype, g=g) for h in (hq, hkv, hkv))
+        qk = cache.append(k, v, 0, query=torch.cat((q, k), 1), rotation=tables)
+        q, k = qk.split((hq, hkv), 1)
+        out, _ = tree_verify_attention(None, q, k, v, prompt_mask(masks, q))
+        for b, n in enumerate(group):
+            kept.append((k[b, :, :n], v[b, :, :n]))
+            kp, vp = cache._pools[0]
+            slot = torch.arange(n, device='cuda')
+            at = cache.page_table()[first + b][slot // 16]
+            assert torch.equal(kp[at, :, slot % 16].transpose(0, 1), k[b, :, :n])
+            # a row sees the rows up to itself. The verify attention holds its weights in the dtype once: each is off
+            # by u of itself, in the products and not in their total, which adds 2 u max |v| to the bound above
+            heads, u = torch.arange(hq, device='cuda') // (hq // hkv), torch.finfo(dtype).eps / 2
+            qq, kk, vv = q[b, :, :n].double(), k[b, heads, :n].double(), v[b, heads, :n].double()
+            hidden = torch.ones(n, n, dtype=torch.bool, device='cuda').triu(1)
+            ref = torch.softmax((qq @ kk.transpose(1, 2) * dim ** -0.5).masked_fill(hidden, -math.inf), -1) @ vv
+            ds = dim ** 0.5 * 2.0 ** -23 * (qq.abs() @ kk.abs().transpose(1, 2)).max()
+            tol = u * ref.abs() + 2 * (2 * ds + u + 2.0 ** -20 + n * 2.0 ** -24) * vv.abs().amax()
+            assert ((out[b, :n].transpose(0, 1).double() - ref).abs() <= tol).all()
+    cache.begin()
+    q, k, v = (randn(4, h, 1, dim, dtype=dtype, g=g) for h in (hq, hkv, hkv))
+    q = cache.append(k, v, 0, query=q, rotation=tables)
+    out = cache.attend(q, 0)
+    kp, vp = cache._pools[0]
+    assert cache.lengths == [21, 10, 34, 2]
+    check_attention(out, q, kp, vp, cache.page_table(), cache.lengths, dim ** -0.5, 16, dtype)
+    for b, (k, v) in enumerate(kept):
+        slot = torch.arange(k.shape[1], device='cuda')
+        at = cache.page_table()[b][slot // 16]
+        assert torch.equal(kp[at, :, slot % 16].transpose(0, 1), k) and torch.equal(vp[at, :, slot % 16].transpose(0, 1), v)
+    assert _ops.device_error() is None

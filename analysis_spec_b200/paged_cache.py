@@ -244,7 +244,7 @@ class PagedKVCache(Cache):
             self.begin(counts, device=device)
         except Exception:
             if fresh:  # the sequences of a prompt that did not enter
-                self.release([True] * batch)
+                self._drop_all()
             raise
 
     def update(self, key_states, value_states, layer_idx, *args, **kwargs):
@@ -278,7 +278,12 @@ class PagedKVCache(Cache):
     def reset(self):
         """Drops every sequence and the next forward's prompt lengths; the pools stay."""
         self._prompts = None
-        self.release([True] * len(self.lengths))
+        self._drop_all()
+
+    def _drop_all(self):
+        for held in self._held:
+            self._free += reversed(held)
+        self.lengths, self._held, self._step = [], [], None
 
     def _unsupported(self, *args, **kwargs):
         raise NotImplementedError('a paged cache admits and releases whole sequences (admit, release); its rows are '

@@ -367,3 +367,21 @@ def test_tangents_are_refused():
                 token_logprobs(logits, t)
     with pytest.raises(RuntimeError, match='no CPU path'):
         token_logprobs(x, t)
+
+
+def test_a_first_forward_inside_a_capture_leaves_nothing(monkeypatch):
+    """Refused with its reason, and the sequences it admitted are gone."""
+    monkeypatch.setattr(_ops, 'paged_append', lambda *a: None)
+    cache = PagedKVCache(8, 4, batch_capacity=2, max_length=16)
+    k = torch.zeros(2, 1, 3, 8)
+    cache.update(k, k, 0)
+    cache.reset()
+    assert cache.free_pages == 8 and cache.lengths == []
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
+        m.setattr(cache, '_device', torch.device('cuda'))
+        with pytest.raises(RuntimeError, match='begin.. decides and copies'):
+            cache.update(k, k, 0)
+    assert cache.free_pages == 8 and cache.lengths == []
+    cache.update(k, k, 0)
+    assert cache.lengths == [3, 3] and cache.free_pages == 6

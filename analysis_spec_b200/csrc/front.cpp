@@ -6,6 +6,7 @@
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 
 #include <c10/cuda/CUDAGuard.h>
@@ -128,6 +129,9 @@ Maybe paged_append(const Tensor& key, const Tensor& value, const Tensor& key_pag
   } else if (out != nullptr) {
     value_error(fn, "query_out without query");
   }
+  for (const Tensor* written : {&key_pages, &value_pages, out})  // expanded: rows would be stored over each other
+    if (written != nullptr && at::has_internal_overlap(*written) == at::MemOverlap::Yes)
+      value_error(fn, "the pages and query_out are written and must not overlap themselves (an expanded tensor does)");
   const int dev = one_device(fn, {&key, &value, &key_pages, &value_pages, &page_table, &starts, counts, query, cos, sin,
                                   positions, out});
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);

@@ -385,3 +385,17 @@ def test_a_first_forward_inside_a_capture_leaves_nothing(monkeypatch):
     assert cache.free_pages == 8 and cache.lengths == []
     cache.update(k, k, 0)
     assert cache.lengths == [3, 3] and cache.free_pages == 6
+
+
+def test_append_refuses_to_write_expanded_tensors():
+    bf = torch.bfloat16
+    k, n = torch.zeros(2, 2, 3, 64, dtype=bf), torch.zeros(2, dtype=torch.long)
+    good = dict(key=k, value=k, key_pages=torch.zeros(4, 2, 16, 64, dtype=bf), value_pages=torch.zeros(4, 2, 16, 64, dtype=bf),
+                page_table=torch.zeros(2, 2, dtype=torch.long), starts=n, query=k)
+    one = good['key_pages'][:1].expand(4, 2, 16, 64)
+    for kw in (dict(key_pages=one), dict(value_pages=one), dict(query_out=k[:1].expand(2, 2, 3, 64))):
+        with pytest.raises(ValueError, match='overlap themselves'):
+            paged_append(**{**good, **kw})
+    for kw in (dict(key=k[:1].expand(2, 2, 3, 64)), dict(query=k[:, :1].expand(2, 4, 3, 64)), dict(query_out=k)):
+        with pytest.raises(RuntimeError, match='no CPU path'):  # read only, or in place
+            paged_append(**{**good, **kw})

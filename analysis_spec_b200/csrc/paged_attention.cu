@@ -37,7 +37,8 @@ constexpr int kScalarWarps = 8;
 constexpr int kScalarDims = 8;  // dims per lane: head dims to 256
 
 // CTA per (sequence, query head), a key per warp and step: head dims and views off 16-byte boundaries. Reads
-// the cache once per query head and waits for each key: 30 times the time of the kernels below.
+// the cache once per query head and waits for each key: 20 to 34 times the time of the kernels below (4000 keys of
+// 8 / 1 heads x 128: 420 us in bf16, 414 in fp32).
 template <typename T>
 __global__ void __launch_bounds__(kScalarWarps * 32) paged_attention_scalar_kernel(PagedArgs a) {
   const long long b = blockIdx.x / a.q_heads, hq = blockIdx.x % a.q_heads;
@@ -844,8 +845,8 @@ __device__ __forceinline__ long long tiles_of(const PagedArgs& a, long long b, i
 
 // Equal shares of all sequences' tiles, one per resident CTA: no CTA waits for a longer sequence, and a
 // long cache is split as finely as the GPU is wide. Bound by memory: 256 sequences of 512 to 6144
-// positions (28 q / 4 KV heads x 128, fp16) 269 to 279 us, 2 of 100001 to 130000 (40 / 8, bf16) 145 to
-// 149 us, 0.97 of the copy bandwidth measured on this GPU; the first in fp32 609 to 664 us (0.82 to 0.89).
+// positions (28 q / 4 KV heads x 128, fp16) 267 to 283 us, 2 of 100001 to 130000 (40 / 8, bf16) 144 to
+// 150 us, 0.96 or more of the copy bandwidth measured on this GPU; the first in fp32 609 to 664 us (0.82 to 0.89).
 template <typename T, int D, int NT, bool WHOLE>
 __global__ void __launch_bounds__(Shape<T, D, NT>::kWarps * 32, Shape<T, D, NT>::kResident)
     paged_attention_share_kernel(PagedArgs a, PlanArgs plan) {
@@ -955,7 +956,7 @@ __global__ void __launch_bounds__(Shape<T, D, NT>::kWarps * 32, Shape<T, D, NT>:
 // Few items: a cluster of CTAs each, an equal run of its tiles per CTA, joined through the cluster's
 // shared memory. One launch, no workspace. Where each of its CTAs has an SM to itself, eight warps share
 // the work (WIDE): one warp per scheduler leaves most of the issue slots empty. Bound by latency: 64
-// sequences of 256 to 2048 positions (16 / 2 heads, bf16) 23.7 us: a block of 16 keys a warp costs 1.3 us
+// sequences of 256 to 2048 positions (16 / 2 heads, bf16) 23.8 to 24.1 us: a block of 16 keys a warp costs 1.3 us
 // of dependent loads and products (11 of them in the longest sequence's CTAs), the rest is launch,
 // length, page and joins; one of 200 positions 8.2 us a call, 6.3 in a captured graph.
 template <typename T, int D, int NT, bool WHOLE, bool WIDE>

@@ -365,12 +365,15 @@ template <typename T> __device__ __forceinline__ float widest(float c) {
 // only those (about k kRuns' share of a thread each), are read again, and all their entries that
 // reach it are ranked by (value, index). Those are all of the row's: so if they are k or more, the
 // k first of them are the row's. If not (or if they are too many, or NaN is among the logits),
-// k scans of the row find them.
+// k scans of the row find them, entry by entry. That costs: with five finite logits a row and ten alternatives
+// (a masked vocabulary) 3904 x 151680 bf16 take 6.6 ms and 4 x 151644 fp32 73 us; ties that fill more than
+// kRunList runs (3904 x 32000 whole numbers) 0.93 ms instead of 70 us. In a cluster it is the run of a CTA that
+// has to hold k finite logits.
 //
-// 3904 x 151680 bf16 with ten alternatives takes 234 to 240 us (0.76 of the copy bandwidth measured on
-// this GPU), 201 without (0.9): an exponential and the products around it keep the issue slots two thirds
-// busy, and what follows a row's last logit is hidden by the SM's other CTAs in part only. 4 x 151644
-// fp32: 12.3 us, 9.1 without alternatives.
+// 3904 x 151680 bf16 with ten alternatives takes 205 to 243 us, from GPU to GPU (0.75 to 0.9 of the copy
+// bandwidth measured on one), 179 to 201 without (0.9 or more): an exponential and the products around it keep
+// the issue slots two thirds busy, and what follows a row's last logit is hidden by the SM's other CTAs in part
+// only. 4 x 151644 fp32: 12.3 us, 8.3 to 9.1 without alternatives.
 constexpr int kRuns = 8, kRunList = 128;
 
 template <typename T, int THREADS, bool TOP>
@@ -666,8 +669,8 @@ constexpr int kGradSpan = 4;  // 32-byte vectors a thread handles
 // CTA per (row, run of vectors). One exponential and one product chain an entry:
 //   dx = p (u + v y) with y = log2 p, p = 2^y, u = -(sum of gradients + g_H H) / T,
 //   v = -g_H ln(2) / T; the token and the alternatives add their own gradient afterwards.
-// Bound by memory: forward and gradient of 4096 x 151644 bf16 take 592 to 608 us (0.92 of the copy
-// bandwidth measured on this GPU).
+// Bound by memory: forward and gradient of 4096 x 151644 bf16 take 559 to 608 us (0.9 to 0.98 of the
+// copy bandwidth measured on one GPU), of 1024 x 151644 fp32 297 us (0.97).
 template <typename T>
 __global__ void __launch_bounds__(kGradThreads) token_logprobs_backward_kernel(ScoreArgs a, int runs) {
   constexpr int N = 32 / sizeof(T);
@@ -687,8 +690,8 @@ __global__ void __launch_bounds__(kGradThreads) token_logprobs_backward_kernel(S
   }
   const T* x = static_cast<const T*>(a.logits) + offset;
   // The gradient's vectors are aligned; the logits' lie alike, or (a view such as logits[:, :-1]) only
-  // their words do, or (of an odd vocabulary) lie across two words each: 1024 x 151643 bf16 with its
-  // forward 209 us, 190 where they lie alike, 546 entry by entry.
+  // their words do, or (of an odd offset) lie across two words each: 1024 x 151643 bf16 in a pitch of
+  // 151644 with its forward 189 to 209 us, 164 to 190 where they lie alike, 546 entry by entry.
   const uintptr_t apart = (reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(g)) & 31;
   Bytes32 in[kGradSpan];
 #pragma unroll
@@ -793,13 +796,13 @@ int launch_scores(const char* fn, const ScoreArgs& a, cudaStream_t s) {
   const int sms = sm_count();
   if (sms == 0) return fail(SPECKV_ECUDA, "%s: no SM count", fn);
   // A cluster per row while that makes no more than two CTAs an SM (four fit, but clusters do not pack:
-  // 148 x 151680 bf16 20.0 us, 28.7 with twice the CTAs) and leaves each thread a vector.
+  // 148 x 151680 bf16 18.6 to 20.0 us, 28.7 with twice the CTAs) and leaves each thread a vector.
   int ctas = 1;
   while (ctas < 8 && rows * ctas <= sms && vectors / (ctas * 2) >= 256) ctas *= 2;
   if (rows * ctas >= (1ll << 31)) return fail(SPECKV_ENOSUPPORT, "%s: too many rows", fn);
   // What follows a row's last logit takes a CTA 2 to 6 us: at vocabularies to 128 K entries of 16 bits
   // twice the CTAs of half the threads hide more of it (3904 x 32000 bf16, ten alternatives: 71 us
-  // instead of 86), longer rows want the wider CTA (900 x 151644 fp32: 109 us, 123 with 128 threads).
+  // instead of 86), longer rows want the wider CTA (900 x 151644 fp32: 102 to 106 us, 123 with 128 threads).
   if (ctas == 1 && vectors <= 8192)
     return a.top > 0 ? launch_scores_as<T, 128, true>(fn, a, 1, s) : launch_scores_as<T, 128, false>(fn, a, 1, s);
   return a.top > 0 ? launch_scores_as<T, 256, true>(fn, a, ctas, s) : launch_scores_as<T, 256, false>(fn, a, ctas, s);

@@ -194,8 +194,8 @@ __device__ __forceinline__ void rotate(uint4& px, uint4& py, const float (&c)[N]
 // token) are in such rounds at once.
 // Memory bound where tokens are many: 8 prompts to 4001 tokens, 40 q / 8 KV heads x 128 in fp16,
 // 113 to 116 us (0.94 or more of the copy bandwidth measured on this GPU; in fp32 219, 0.99); latency bound
-// below: 64 x 61 rows of 16 / 2
-// heads 10.3 us (0.63), one row each of 256 sequences 6.6 us, the cost of the host call.
+// below: 64 x 61 rows of 16 / 2 heads 10.3 us (0.63), one row each of 256 sequences 6.6 us, the cost of the
+// host call.
 constexpr int kHeads = 3;
 
 template <typename T, bool INTERLEAVED, int THREADS>

@@ -9,6 +9,7 @@
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -358,6 +359,21 @@ struct ScoreFunction : public torch::autograd::Function<ScoreFunction> {
   }
 };
 
+// A captured backward pass joins the stream on which a leaf's gradient is accumulated. Where a graph outside
+// the capture keeps that node alive on another stream, the join breaks the capture from within the autograd
+// engine and the process ends: refused while that can still be an error.
+void check_capture(const Tensor& logits) {
+  if (!logits.is_cuda() || !logits.is_leaf()) return;
+  const c10::cuda::CUDAGuard guard(logits.device());
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(logits);
+  if (node == nullptr) return;
+  const auto stream = node->stream();
+  if (stream.has_value() && *stream != c10::cuda::getCurrentCUDAStream(logits.get_device()).unwrap())
+    throw std::runtime_error("token_logprobs: these logits are a leaf of an autograd graph made outside this capture, "
+                             "which is still alive; drop its outputs first");
+}
+
 py::tuple token_logprobs(const Tensor& logits, const Maybe& tokens, const Maybe& rows, int64_t top,
                          double temperature) {
   auto item = [](const Tensor& t) -> py::object { return t.defined() ? py::cast(t) : py::none(); };
@@ -367,6 +383,7 @@ py::tuple token_logprobs(const Tensor& logits, const Maybe& tokens, const Maybe&
     if (get(rows) != nullptr)
       value_error("token_logprobs", "rows selects verified rows of a rollout and carries no gradient; detach the "
                                     "logits or index them first");
+    check_capture(logits);
     const auto out = ScoreFunction::apply(logits, tokens, top, temperature);
     const size_t at = get(tokens) != nullptr ? 1 : 0;
     return py::make_tuple(at ? item(out[0]) : py::none(), item(out[at]), top > 0 ? item(out[at + 1]) : py::none(),

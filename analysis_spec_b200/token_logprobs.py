@@ -31,6 +31,7 @@ def token_logprobs(logits, tokens=None, *, rows=None, top=0, temperature=1.0):
     the vocabulary or a row outside the logits is skipped and reported by ``_ops.device_error``.
     A row of -inf alone has log-probability -inf and entropy 0; NaN or +inf in a row makes its
     numbers NaN. The outputs carry a gradient to ``logits`` (not twice differentiable;
-    forward-mode tangents are refused).
+    forward-mode tangents are refused). Before a backward pass is captured into a CUDA graph, drop every
+    eager graph of the same leaves: torch ends the process otherwise (refused where ``logits`` are the leaf).
     """
     return TokenLogprobs(*_ops.token_logprobs(logits, tokens, rows, top, temperature))

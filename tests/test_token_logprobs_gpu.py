@@ -446,3 +446,32 @@ def test_references_that_pass_the_fused_products_border(rows, vocab):
     # ... and one entry past 2^20, far enough above the rest for a new reference (10 in powers of two)
     x = torch.where(one, border + (1 + j % 9) / 16, border - 7.0 - (1 + j % 16) / 16).float()
     check_forward(token_logprobs(x, tokens, top=1), x, tokens, 1, 1.0)
+
+
+def test_capture_beside_a_live_eager_graph_is_refused():
+    """Before anything is launched; two calls of one capture are no such case, nor is a call without a gradient."""
+    g = gen(7)
+    x = some_logits(3, 501, torch.float32, g).requires_grad_(True)
+    tokens = torch.randint(0, 501, (3,), device='cuda', generator=g)
+    want = token_logprobs(x, tokens).logprobs  # alive, on the default stream
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match='still alive'):
+            token_logprobs(x, tokens)
+        with torch.no_grad():
+            plain = token_logprobs(x, tokens).logprobs
+        other = token_logprobs(x.detach().requires_grad_(True), tokens).logprobs.detach()
+    graph.replay()
+    torch.cuda.synchronize()
+    want = want.detach()  # its graph is gone
+    assert torch.equal(plain, want) and torch.equal(other, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        first, second = token_logprobs(x, tokens), token_logprobs(x, tokens, temperature=2.0)
+        grad, = torch.autograd.grad(first.logprobs.sum() + second.entropy.sum(), x)
+        first, second = first.logprobs.detach(), second.entropy.detach()
+    graph.replay()
+    torch.cuda.synchronize()
+    r, s = token_logprobs(x, tokens), token_logprobs(x, tokens, temperature=2.0)
+    again, = torch.autograd.grad(r.logprobs.sum() + s.entropy.sum(), x)
+    assert torch.equal(first, r.logprobs) and torch.equal(second, s.entropy) and torch.equal(grad, again)

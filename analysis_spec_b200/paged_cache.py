@@ -44,9 +44,10 @@ def paged_attention(query, key_pages, value_pages, page_table, lengths, scale=No
 
     ``query`` (batch, q_heads, 1, head_dim); pools and ``page_table`` as for ``paged_append``;
     ``lengths`` (batch,) int64. Query head h reads KV head h // (q_heads // kv_heads). A sequence
-    of length 0 gives zeros, an infinite value makes its outputs infinite or NaN. fp32 products are taken to 2^-21 and summed in fp32
-    (a value within 2^-12 of the type's largest counts as infinite). Returns (batch, 1, q_heads,
-    head_dim). Head dims to 256. Inference only: no gradient flows through it.
+    of length 0 gives zeros, an infinite value makes its outputs infinite or NaN. fp32 products are
+    taken to 2^-21 and summed in fp32 (a value within 2^-12 of the type's largest counts as
+    infinite). Returns (batch, 1, q_heads, head_dim). Head dims to 256. Inference only: no gradient
+    flows through it.
     """
     return _ops.paged_attention(query, key_pages, value_pages, page_table, lengths,
                                 query.shape[-1] ** -0.5 if scale is None else scale, out)
@@ -177,8 +178,9 @@ class PagedKVCache(Cache):
             self._device = torch.device(device if device is not None else 'cuda')
         self._outside_capture('begin')
         if self._table is None:
-            self._table = torch.zeros((self.batch_capacity, self.table_pages), dtype=torch.long, device=self._device)
-            self._numbers = torch.zeros(3 * self.batch_capacity, dtype=torch.long, device=self._device)
+            with torch.inference_mode(False):  # written again in either mode
+                self._table = torch.zeros((self.batch_capacity, self.table_pages), dtype=torch.long, device=self._device)
+                self._numbers = torch.zeros(3 * self.batch_capacity, dtype=torch.long, device=self._device)
             self._device = self._table.device
         for i, want in enumerate(wants):
             for _ in range(want):

@@ -399,3 +399,18 @@ def test_append_refuses_to_write_expanded_tensors():
     for kw in (dict(key=k[:1].expand(2, 2, 3, 64)), dict(query=k[:, :1].expand(2, 4, 3, 64)), dict(query_out=k)):
         with pytest.raises(RuntimeError, match='no CPU path'):  # read only, or in place
             paged_append(**{**good, **kw})
+
+
+@pytest.mark.parametrize('first', [True, False])
+def test_begin_inside_and_outside_inference_mode(first):
+    """What one mode has made, a begin in the other writes to."""
+    cache = PagedKVCache(16, 4, batch_capacity=2, max_length=24)
+    cache.admit(2)
+    for mode in (first, not first, first):
+        with torch.inference_mode(mode):
+            cache.begin([3, 5], device='cpu')
+    assert cache._step[3].tolist() == [9, 15] and cache.page_table()[:, 0].tolist() != [0, 0]
+    with torch.inference_mode(first):
+        assert cache.release([True, False]) == [1]
+    cache.begin(4)
+    assert cache._step[3].tolist() == [19]

@@ -32,11 +32,12 @@ def dense_mask_visibility(attention_mask, mask, batch, rows, kv_len):
     """Bits for the additive `mask` (`attention_mask` cut to kv_len columns), cached on
     `attention_mask` per (shape, in-place version): every layer of a forward gets the same
     mask tensor, so the conversion (one launch and one 4-byte read-back) runs once per
-    forward. Returns None when the mask holds values other than 0 and the dtype's lowest
+    forward (once per layer for a mask made in inference mode, which has no version). Returns None when the mask holds values other than 0 and the dtype's lowest
     value / -inf (such a mask keeps the dense kernel)."""
-    key = (kv_len, rows, batch, attention_mask._version)
+    versioned = not attention_mask.is_inference()
+    key = (kv_len, rows, batch, attention_mask._version if versioned else None)
     cached = getattr(attention_mask, '_speckv_dense_bits', None)
-    if cached is not None and cached[0] == key:
+    if versioned and cached is not None and cached[0] == key:
         return cached[1]
     dev = mask.device
     bits = torch.empty((batch, rows, _ops.visibility_words(kv_len)), dtype=torch.int32, device=dev)
@@ -56,10 +57,11 @@ def prompt_mask(prompt, query):
     dict `prompt` (one per forward), so that its visibility bits are built once for all layers."""
     batch, rows = query.shape[0], query.shape[2]
     if prompt.get('shape') != (batch, rows, query.dtype):
-        hidden = torch.ones((rows, rows), dtype=torch.bool, device=query.device).triu(1)
-        mask = torch.zeros((rows, rows), dtype=query.dtype, device=query.device)
-        mask.masked_fill_(hidden, torch.finfo(query.dtype).min)
-        prompt.update(shape=(batch, rows, query.dtype), mask=mask.expand(batch, 1, rows, rows))
+        with torch.inference_mode(False):  # a mask with a version, on which its bits are kept
+            hidden = torch.ones((rows, rows), dtype=torch.bool, device=query.device).triu(1)
+            mask = torch.zeros((rows, rows), dtype=query.dtype, device=query.device)
+            mask.masked_fill_(hidden, torch.finfo(query.dtype).min)
+            prompt.update(shape=(batch, rows, query.dtype), mask=mask.expand(batch, 1, rows, rows))
     return prompt['mask']
 
 

@@ -872,3 +872,25 @@ def test_prompts_through_the_plain_calls(dtype, dim):
         at = cache.page_table()[b][slot // 16]
         assert torch.equal(kp[at, :, slot % 16].transpose(0, 1), k) and torch.equal(vp[at, :, slot % 16].transpose(0, 1), v)
     assert _ops.device_error() is None
+
+
+def test_prompt_and_steps_in_either_inference_mode():
+    """The transformers protocol inside and outside inference mode gives the same numbers."""
+    from analysis_spec_b200.tree_attention import tree_verify_attention
+    g = gen(17)
+    rows = [randn(2, h, 12, 128, dtype=torch.bfloat16, g=g) for h in (8, 2, 2)]
+    got = []
+    for modes in ((True, False, True), (False, True, False)):
+        cache, outs = PagedKVCache(12, 8, batch_capacity=2, max_length=40), []
+        cache.prompt_lengths([10, 3])
+        for inside, (lo, hi) in zip(modes, ((0, 10), (10, 11), (11, 12))):
+            with torch.inference_mode(inside):
+                q, k, v = (x[:, :, lo:hi].clone() for x in rows)
+                for layer in range(2):
+                    k2, v2 = cache.update(k, v, layer)
+                    outs.append(tree_verify_attention(None, q, k2, v2, None)[0].clone())
+        got.append(outs)
+        assert cache.lengths == [12, 5]
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
+    assert _ops.device_error() is None

@@ -414,3 +414,24 @@ def test_begin_inside_and_outside_inference_mode(first):
         assert cache.release([True, False]) == [1]
     cache.begin(4)
     assert cache._step[3].tolist() == [19]
+
+
+def test_masks_in_inference_mode(monkeypatch):
+    """Masks made in inference mode have no version: a prompt's mask keeps its bits all the same, another one is
+    converted again for each layer rather than trusted to be unchanged."""
+    from analysis_spec_b200 import tree_attention
+    made = []
+
+    monkeypatch.setattr(_ops, 'mask_bits', lambda mask, bits, first, flag: (made.append(mask), flag.zero_()))
+    with torch.inference_mode():
+        query = torch.zeros(2, 4, 5, 128, dtype=torch.bfloat16)
+        prompt = {}
+        masks = [tree_attention.prompt_mask(prompt, query) for _ in range(3)]
+        assert masks[0] is masks[1] and masks[0][1, 0].isfinite().all() and masks[0][0, 0, 1, 2] < -1e38
+        for mask in masks:
+            assert tree_attention.dense_mask_visibility(mask, mask, 2, 5, 5) is not None
+        assert len(made) == 1
+        other = torch.zeros(2, 1, 5, 5, dtype=torch.bfloat16)
+        for _ in range(2):
+            assert tree_attention.dense_mask_visibility(other, other, 2, 5, 5) is not None
+        assert len(made) == 3
